@@ -42,26 +42,26 @@ def _attend(name, q_heads, kv_heads, head_dim, block, slots, tokens, rows, k, dt
 def listed():
     return [
         # one question over a small library of passages: every score, latency counts
-        _index("score one, 100k x 384", "score", 100_000, 384, 1),
+        _index("score one 100k x 384", "score", 100_000, 384, 1),
         # three questions at once over a ragged library with an odd dimension
-        _index("score three, 1000003 x 300", "score", 1_000_003, 300, 3),
+        _index("score three 1000003 x 300", "score", 1_000_003, 300, 3),
         # a server's batch: the scores of eight questions, 1024 values a vector
-        _index("score eight, 2M x 1024", "score", 2_000_000, 1024, 8),
+        _index("score eight 2M x 1024", "score", 2_000_000, 1024, 8),
         # the passages that one question is answered with, over a small and a large library
         _index("top 10 of 100k x 384", "topk", 100_000, 384, 1, 10),
         _index("top 100 of 4M x 768", "topk", 4_000_000, 768, 1, 100),
         # sixteen questions at once, vectors of a small embedding model
-        _index("top 10 of 1.5M x 256, sixteen", "topk", 1_500_000, 256, 16, 10),
+        _index("top 10 of 1.5M x 256 sixteen", "topk", 1_500_000, 256, 16, 10),
         # one sequence's next token behind a prompt of 4096 tokens: latency counts
-        _attend("one token, 4k", 32, 8, 128, 64, 1, 4096, 1, 16, "bf16"),
+        _attend("one token 4k", 32, 8, 128, 64, 1, 4096, 1, 16, "bf16"),
         # a serving batch: the next token of sixteen sequences of up to 32768 tokens
-        _attend("sixteen tokens, 32k", 32, 8, 128, 64, 16, 32768, 1, 32, "bf16"),
+        _attend("sixteen tokens 32k", 32, 8, 128, 64, 16, 32768, 1, 32, "bf16"),
         # the next token of two sequences of half a million tokens, an odd length
-        _attend("two tokens, 500k", 32, 8, 128, 64, 2, 500_011, 1, 64, "f16"),
+        _attend("two tokens 500k", 32, 8, 128, 64, 2, 500_011, 1, 64, "f16"),
         # four drafted tokens for each of eight sequences, a key/value head for every query head, two slots next to empty
-        _attend("drafts, 12 heads of 64", 12, 12, 64, 32, 8, 5000, 4, 12, "f16", "tokens", True),
+        _attend("drafts 12 heads of 64", 12, 12, 64, 32, 8, 5000, 4, 12, "f16", "tokens", True),
         # a chunk of a long prompt: its keys' blocks are made first
-        _attend("prompt chunk, 2048 of 16k", 32, 8, 128, 64, 1, 16384, 2048, 16, "bf16", "tokens", False, True),
+        _attend("prompt chunk 2048 of 16k", 32, 8, 128, 64, 1, 16384, 2048, 16, "bf16", "tokens", False, True),
     ]
 
 
