@@ -73,6 +73,17 @@ SIGNATURES = {
     "fi8_bin_index_create_empty": (C.c_int, [_P, _I64, _I32, _I32, _P, _I32, _I64, _P]),
     "fi8_bin_upload_rows": (C.c_int, [_P, _I64, _P, _P, _P, _I64]),
     "fi8_bin_upload_finish": (C.c_int, [_P]),
+    "fi8_i4_create": (C.c_int, [_P, _P, _P, _P, _I64, _I32, _I64, _P]),
+    "fi8_i4_create_f32": (C.c_int, [_P, _P, _I64, _I32, _I64, _P]),
+    "fi8_i4_create_empty": (C.c_int, [_P, _I64, _I32, _I64, _P]),
+    "fi8_i4_set_rows_async": (C.c_int, [_P, _I64, _P, _I64, _P]),
+    "fi8_i4_read_rows": (C.c_int, [_P, _P, _P, _P]),
+    "fi8_i4_destroy": (C.c_int, [_P]),
+    "fi8_i4_info": (C.c_int, [_P, _P, _P]),
+    "fi8_i4_score_batch": (C.c_int, [_P, _P, _I32, _P]),
+    "fi8_i4_score_async": (C.c_int, [_P, _P, _I32, _P, _P]),
+    "fi8_i4_topk_batch": (C.c_int, [_P, _P, _I32, _I32, _P, _I64, _P, _P]),
+    "fi8_i4_topk_async": (C.c_int, [_P, _P, _I32, _I32, _P, _I64, _P, _P]),
 }
 
 

@@ -191,6 +191,37 @@ class B200Backend:
                 raise Fi8Error(1, f"gpu: center len {center.shape[0]} != dim {dim}")
         return BinaryI8Index(self.ctx, codes, words, center, bq, scales, n, dim, overquery, id_base)
 
+    def NewI4Index(self, codes, mults, scales, n: int, dim: int, id_base: int = 0) -> "I4Index":
+        """A FlatI4 shard from packed rows (fi8_i4_create): codes [n, G, 16] and
+        mults [n, G] uint8, scales [n], with G = ceil(dim / 32)."""
+        codes = np.ascontiguousarray(codes, dtype=np.uint8).reshape(-1)
+        mults = np.ascontiguousarray(mults, dtype=np.uint8).reshape(-1)
+        scales = _f32(scales).reshape(-1)
+        groups = (dim + 31) // 32
+        if n <= 0 or dim <= 0:
+            raise Fi8Error(1, f"gpu: empty 4-bit index (n={n} dim={dim})")
+        if codes.shape[0] != n * groups * 16 or mults.shape[0] != n * groups or scales.shape[0] != n:
+            raise Fi8Error(1, "gpu: 4-bit index shape mismatch")
+        h = C.c_void_p()
+        check(lib().fi8_i4_create(self.ctx.handle, _p(codes), _p(mults), _p(scales), n, dim, id_base, C.byref(h)))
+        return I4Index(self.ctx, h, n, dim, id_base)
+
+    def NewI4IndexFromFloats(self, vecs, id_base: int = 0) -> "I4Index":
+        """A FlatI4 shard of vecs [n, dim] float32, quantized on the device
+        (fi8_i4_create_f32)."""
+        v = _f32(vecs)
+        if v.ndim != 2 or v.shape[0] == 0 or v.shape[1] == 0:
+            raise Fi8Error(1, f"gpu: empty 4-bit index (shape {v.shape})")
+        h = C.c_void_p()
+        check(lib().fi8_i4_create_f32(self.ctx.handle, _p(v), v.shape[0], v.shape[1], id_base, C.byref(h)))
+        return I4Index(self.ctx, h, v.shape[0], v.shape[1], id_base)
+
+    def NewI4IndexEmpty(self, n: int, dim: int, id_base: int = 0) -> "I4Index":
+        """A FlatI4 shard of n zero rows to fill with I4Index.set_rows_async."""
+        h = C.c_void_p()
+        check(lib().fi8_i4_create_empty(self.ctx.handle, n, dim, id_base, C.byref(h)))
+        return I4Index(self.ctx, h, n, dim, id_base)
+
 
 class I8Index:
     """A device-resident FlatI8 shard: I8Index + I8BatchIndex + I8TopKIndex."""
@@ -534,6 +565,86 @@ class BinaryI8Index:
             check(lib().fi8_bin_index_destroy(self._h))
             self._h = None
             self._ih = None
+
+    def __del__(self):
+        try:
+            self.Close()
+        except Exception:
+            pass
+
+
+class I4Index:
+    """A device-resident FlatI4 shard: rows in 4 bits a value with group scales
+    (include/fi8.h has the format), scored and searched as an I8Index's are."""
+
+    def __init__(self, ctx: Context, h, n: int, dim: int, id_base: int):
+        self._h, self.ctx, self.n, self.dim, self.id_base = h, ctx, n, dim, id_base
+
+    def set_rows_async(self, row0: int, d_vecs: int, rows: int, stream: int = 0) -> None:
+        """Quantize rows float32 rows at device address d_vecs into rows
+        [row0, row0 + rows)."""
+        check(lib().fi8_i4_set_rows_async(self._h, row0, C.c_void_p(d_vecs), rows, C.c_void_p(stream or None)))
+
+    def read_rows(self):
+        """The rows, copied to the host: codes [n, G, 16], mults [n, G], scales [n]."""
+        groups = (self.dim + 31) // 32
+        codes = np.empty((self.n, groups, 16), np.uint8)
+        mults = np.empty((self.n, groups), np.uint8)
+        scales = np.empty(self.n, np.float32)
+        check(lib().fi8_i4_read_rows(self._h, _p(codes), _p(mults), _p(scales)))
+        return codes, mults, scales
+
+    def Score(self, q: Sequence[float], dst: np.ndarray) -> None:
+        """Fills dst[j] with the score of q against row j."""
+        self.ScoreBatch([q], dst)
+
+    def ScoreBatch(self, queries, dst: np.ndarray) -> None:
+        """Fills dst [M*n] with the scores of M queries."""
+        Q = self._queries(queries)
+        M = Q.shape[0]
+        if dst.size != M * self.n or dst.dtype != np.float32 or not dst.flags.c_contiguous:
+            raise Fi8Error(1, f"gpu: batch dst len {dst.size} != M*N {M * self.n}")
+        check(lib().fi8_i4_score_batch(self._h, _p(Q), M, _p(dst)))
+
+    def TopKBatch(self, queries, k: int) -> list[list[Hit]]:
+        return self.QueryFilterBatch(queries, k, None)
+
+    def QueryFilterBatch(self, queries, k: int, keep) -> list[list[Hit]]:
+        """keep: a boolean array over global ids, or None."""
+        idx, sc = self.topk_arrays(queries, k, keep=keep)
+        return [[Hit(int(i), float(s)) for i, s in zip(idx[m], sc[m]) if i >= 0] for m in range(idx.shape[0])]
+
+    def topk_arrays(self, queries, k: int, keep=None):
+        """(int32 [M,k], float32 [M,k]), index -1 = empty."""
+        Q = self._queries(queries)
+        M = Q.shape[0]
+        idx = np.empty((M, max(k, 0)), np.int32)
+        sc = np.empty((M, max(k, 0)), np.float32)
+        bm = None if keep is None else keep_bitmap(keep)
+        check(lib().fi8_i4_topk_batch(self._h, _p(Q), M, k, None if bm is None else _p(bm),
+                                      0 if keep is None else len(keep), _p(idx), _p(sc)))
+        return idx, sc
+
+    def score_async(self, d_q: int, M: int, d_dst: int, stream: int = 0) -> None:
+        """Device-resident scores [M, n]; takes device addresses."""
+        check(lib().fi8_i4_score_async(self._h, C.c_void_p(d_q), M, C.c_void_p(d_dst), C.c_void_p(stream or None)))
+
+    def topk_async(self, d_q: int, M: int, k: int, d_keys: int, stream: int = 0, d_keep: int = 0,
+                   keep_nbits: int = 0) -> None:
+        """Device-resident top-k into packed keys [M, k] (unpack_keys)."""
+        check(lib().fi8_i4_topk_async(self._h, C.c_void_p(d_q), M, k, C.c_void_p(d_keep or None), keep_nbits,
+                                      C.c_void_p(d_keys), C.c_void_p(stream or None)))
+
+    def Close(self) -> None:
+        if self._h:
+            check(lib().fi8_i4_destroy(self._h))
+            self._h = None
+
+    def _queries(self, queries) -> np.ndarray:
+        Q = _f32(queries).reshape(len(queries), -1) if len(queries) else np.empty((0, self.dim), np.float32)
+        if Q.shape[1] != self.dim:
+            raise Fi8Error(1, f"gpu: batch query dim {Q.shape[1]} != index dim {self.dim}")
+        return Q
 
     def __del__(self):
         try:

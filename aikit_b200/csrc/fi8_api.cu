@@ -23,14 +23,17 @@
 #include "fi8_build.cuh"
 #include "fi8_device.cuh"
 #include "fi8_gemm.cuh"
+#include "fi8_host.h"
 #include "fi8_scan.cuh"
 #include "fi8_stage.h"
 
 using namespace fi8;
 
 namespace {
-
 thread_local std::string g_last_error;
+}  // namespace
+
+namespace fi8 {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -47,56 +50,9 @@ int cuda_fail(cudaError_t e, const char* what) {
   return fail(code, "%s: %s", what, cudaGetErrorString(e));
 }
 
-#define FI8_CUDA(call, what)                      \
-  do {                                            \
-    cudaError_t e_ = (call);                      \
-    if (e_ != cudaSuccess) return cuda_fail(e_, what); \
-  } while (0)
+}  // namespace fi8
 
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-  }
-};
-
-template <typename T>
-int ensure_device(T** p, size_t* cap, size_t need, const char* what) {
-  if (*cap >= need && *p) return FI8_OK;
-  if (*p) cudaFree(*p);
-  *p = nullptr;
-  *cap = 0;
-  const size_t n = std::max<size_t>(need, 1);
-  cudaError_t e = cudaMalloc(reinterpret_cast<void**>(p), n * sizeof(T));
-  if (e != cudaSuccess) {
-    *p = nullptr;
-    return cuda_fail(e, what);
-  }
-  *cap = n;
-  return FI8_OK;
-}
-
-template <typename T>
-int ensure_host(T** p, size_t* cap, size_t need, const char* what) {
-  if (*cap >= need && *p) return FI8_OK;
-  if (*p) cudaFreeHost(*p);
-  *p = nullptr;
-  *cap = 0;
-  const size_t n = std::max<size_t>(need, 1);
-  cudaError_t e = cudaMallocHost(reinterpret_cast<void**>(p), n * sizeof(T));
-  if (e != cudaSuccess) {
-    *p = nullptr;
-    return cuda_fail(e, what);
-  }
-  *cap = n;
-  return FI8_OK;
-}
+namespace {
 
 // Queries handled per scan launch in the multi-query (one pass per query)
 // form; bounds the per-launch scratch.
@@ -104,11 +60,6 @@ constexpr int32_t kScanMaxM = 64;
 constexpr int64_t kRowAlign = 256;  // n is padded to a multiple of this
 
 }  // namespace
-
-struct fi8_ctx {
-  int device = 0;
-  int sm_count = 0;
-};
 
 struct fi8_index {
   fi8_ctx* ctx = nullptr;

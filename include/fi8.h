@@ -360,6 +360,62 @@ int fi8_bin_rerank_async(fi8_bin* b, const float* d_q, int32_t M, const uint64_t
 int fi8_bin_prefilter_async_keep(fi8_bin* b, const float* d_q, int32_t M, int32_t cand, const uint64_t* d_keep,
                                  int64_t nbits, uint64_t* d_keys, int32_t sorted, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * FlatI4: rows in 4 bits a value with group scales, scored and searched as a
+ * FlatI8's are, from about half of its bytes. The reference has no such type;
+ * these entry points are additive.
+ *
+ * A row's dim values are padded with zeros to G = ceil(dim / 32) groups. It has
+ *   codes  [G * 16] bytes: byte i of a group holds value i + 8 in its low nibble
+ *          and value 16 + i in its high one (codes -8..7, stored plus 8),
+ *   mults  [G] bytes: the group's multiplier m,
+ *   scale  f32: the row stands for scale * m * code.
+ * A query is quantized to int8 as FlatI8's queries are, and
+ *   score = float32(dot) * qscale * scale, dot = sum of m * sum(code * q8),
+ * with an exact int32 dot: scores have one value, and a top-k one answer
+ * (score desc, index asc; NaN excluded). dim is at most 4096.
+ *
+ * Threading and streams as for fi8_index: calls on one index are serialized on
+ * the host and must not overlap on the GPU when they are top-k calls or host
+ * forms (they share the index's scratch); score_async calls use none and may.
+ * The async forms run in stream order on stream (NULL: the legacy default
+ * stream), never synchronize and never allocate, so they can be captured.
+ * ------------------------------------------------------------------------- */
+typedef struct fi8_i4 fi8_i4; /* a device-resident FlatI4 shard */
+
+/* From host rows (codes [n*G*16], mults [n*G], scales [n]; copied), from host
+ * float32 rows vecs [n*dim] (quantized on the device), or n zero rows to fill
+ * with fi8_i4_set_rows_async. id_base as for fi8_index_create. */
+int fi8_i4_create(fi8_ctx* ctx, const uint8_t* codes, const uint8_t* mults, const float* scales, int64_t n, int32_t dim,
+                  int64_t id_base, fi8_i4** out);
+int fi8_i4_create_f32(fi8_ctx* ctx, const float* vecs, int64_t n, int32_t dim, int64_t id_base, fi8_i4** out);
+int fi8_i4_create_empty(fi8_ctx* ctx, int64_t n, int32_t dim, int64_t id_base, fi8_i4** out);
+
+/* Quantize device rows d_vecs [rows*dim] f32 into rows [row0, row0 + rows):
+ * scale = max|row| / 1785 (an all-zero row: 1), m = ceil(max|group| * (255 /
+ * max|row|)), code = round half away(value * (1 / (m * scale))) in -7..7 (NaN:
+ * 0), in float32 arithmetic. */
+int fi8_i4_set_rows_async(fi8_i4* idx, int64_t row0, const float* d_vecs, int64_t rows, void* stream);
+
+/* The rows, copied to the host in fi8_i4_create's layout (waits for the device). */
+int fi8_i4_read_rows(fi8_i4* idx, uint8_t* codes, uint8_t* mults, float* scales);
+int fi8_i4_destroy(fi8_i4* idx);
+int fi8_i4_info(fi8_i4* idx, int64_t* n, int32_t* dim);
+
+/* Scores of M queries q [M*dim] against every row: dst [M*n]. Eight queries
+ * share one pass over the rows. */
+int fi8_i4_score_batch(fi8_i4* idx, const float* q, int32_t M, float* dst);
+int fi8_i4_score_async(fi8_i4* idx, const float* d_q, int32_t M, float* d_dst, void* stream);
+
+/* Top-k of M queries, as fi8_topk_batch_keep and fi8_topk_batch_async_keep:
+ * keep (NULL: every row) is a bitmap over global ids. k is at most 2048
+ * (FI8_ERR_DECLINED above, and for k <= 0); the host form declines k >= n too,
+ * the async form pads with empty keys. d_keys [M*k], fi8_keys_unpack's layout. */
+int fi8_i4_topk_batch(fi8_i4* idx, const float* q, int32_t M, int32_t k, const uint64_t* keep, int64_t nbits,
+                      int32_t* out_idx, float* out_score);
+int fi8_i4_topk_async(fi8_i4* idx, const float* d_q, int32_t M, int32_t k, const uint64_t* d_keep, int64_t nbits,
+                      uint64_t* d_keys, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
