@@ -26,6 +26,18 @@ _P = C.c_void_p
 _I32 = C.c_int32
 _I64 = C.c_int64
 
+FI8_BF16 = 1
+FI8_F16 = 2
+
+
+class KbDesc(C.Structure):
+    """fi8_kb_desc."""
+
+    _fields_ = [("dtype", _I32), ("slots", _I32), ("kv_heads", _I32), ("q_heads", _I32), ("head_dim", _I32),
+                ("block", _I32), ("max_rows", _I32), ("max_select", _I32), ("capacity", _I64), ("d_k", _P), ("d_v", _P),
+                ("slot_stride", _I64), ("head_stride", _I64), ("token_stride", _I64)]
+
+
 # name -> (restype, argtypes); the complete exported surface of include/fi8.h
 SIGNATURES = {
     "fi8_last_error": (C.c_char_p, []),
@@ -84,6 +96,14 @@ SIGNATURES = {
     "fi8_i4_score_async": (C.c_int, [_P, _P, _I32, _P, _P]),
     "fi8_i4_topk_batch": (C.c_int, [_P, _P, _I32, _I32, _P, _I64, _P, _P]),
     "fi8_i4_topk_async": (C.c_int, [_P, _P, _I32, _I32, _P, _I64, _P, _P]),
+    "fi8_kb_create": (C.c_int, [_P, _P, _P]),
+    "fi8_kb_destroy": (C.c_int, [_P]),
+    "fi8_kb_update_async": (C.c_int, [_P, _P, _P, _P, _I32, _I32, _P]),
+    "fi8_kb_select_async": (C.c_int, [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _I32, _P, _P]),
+    "fi8_kb_attend_async": (C.c_int, [_P, _P, _I64, _P, _P, _I32, _P, _I32, C.c_float, _P, _P, _P]),
+    "fi8_kb_query_async": (C.c_int, [_P, _P, _I64, _P, _P, _I32, _I32, _I32, _I32, C.c_float, _P, _P, _P, _P]),
+    "fi8_kb_read_rows": (C.c_int, [_P, _I32, _P, _P, _P]),
+    "fi8_kb_sync": (C.c_int, [_P]),
 }
 
 

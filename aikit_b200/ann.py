@@ -222,6 +222,21 @@ class B200Backend:
         check(lib().fi8_i4_create_empty(self.ctx.handle, n, dim, id_base, C.byref(h)))
         return I4Index(self.ctx, h, n, dim, id_base)
 
+    def NewKeyBlocks(self, d_k: int, d_v: int, *, dtype: str, slots: int, kv_heads: int, q_heads: int, head_dim: int,
+                     capacity: int, block: int, max_rows: int, max_select: int, slot_stride: int, head_stride: int,
+                     token_stride: int) -> "KeyBlocks":
+        """Block rows over a key/value cache at device addresses d_k and d_v
+        (fi8_kb_create): dtype "bf16" or "f16", strides in values."""
+        from ._ffi import FI8_BF16, FI8_F16, KbDesc
+        types = {"bf16": FI8_BF16, "f16": FI8_F16}
+        if dtype not in types:
+            raise Fi8Error(1, f"gpu: key/value cache of type {dtype!r} (bf16 or f16)")
+        desc = KbDesc(types[dtype], slots, kv_heads, q_heads, head_dim, block, max_rows, max_select, capacity,
+                      d_k, d_v, slot_stride, head_stride, token_stride)
+        h = C.c_void_p()
+        check(lib().fi8_kb_create(self.ctx.handle, C.byref(desc), C.byref(h)))
+        return KeyBlocks(self.ctx, h, desc)
+
 
 class I8Index:
     """A device-resident FlatI8 shard: I8Index + I8BatchIndex + I8TopKIndex."""
@@ -645,6 +660,71 @@ class I4Index:
         if Q.shape[1] != self.dim:
             raise Fi8Error(1, f"gpu: batch query dim {Q.shape[1]} != index dim {self.dim}")
         return Q
+
+    def __del__(self):
+        try:
+            self.Close()
+        except Exception:
+            pass
+
+
+class KeyBlocks:
+    """Block-sparse attention over a key/value cache (include/fi8.h, fi8_kb_*):
+    a FlatI4 row a block chooses which blocks a query reads. The cache stays the
+    caller's. Addresses are device addresses; slots and lengths are int32."""
+
+    def __init__(self, ctx: Context, h, desc):
+        self._h, self.ctx = h, ctx
+        self.slots, self.kv_heads, self.q_heads, self.head_dim = desc.slots, desc.kv_heads, desc.q_heads, desc.head_dim
+        self.block, self.capacity = desc.block, desc.capacity
+        self._width = desc.q_heads * desc.head_dim
+
+    def update_async(self, d_slot: int, d_from: int, d_to: int, count: int, max_tokens: int, stream: int = 0) -> None:
+        """Make the rows of the blocks that tokens [from, to) of each slot fill."""
+        check(lib().fi8_kb_update_async(self._h, C.c_void_p(d_slot), C.c_void_p(d_from), C.c_void_p(d_to), count,
+                                        max_tokens, C.c_void_p(stream or None)))
+
+    def select_async(self, d_q: int, d_slot: int, d_len: int, rows: int, k: int, d_sel: int, first: int = 1,
+                     last: int = 1, stream: int = 0, q_stride: int = 0) -> None:
+        """Choose k blocks a (row, key/value head) into d_sel [rows, kv_heads, k]
+        int32. q_stride: values between query rows (0: none between them)."""
+        check(lib().fi8_kb_select_async(self._h, C.c_void_p(d_q), q_stride or self._width, C.c_void_p(d_slot),
+                                        C.c_void_p(d_len), rows, k, first, last, C.c_void_p(d_sel),
+                                        C.c_void_p(stream or None)))
+
+    def attend_async(self, d_q: int, d_slot: int, d_len: int, rows: int, k: int, scale: float, d_sel: int, d_out: int,
+                     d_lse: int = 0, stream: int = 0, q_stride: int = 0) -> None:
+        """Attention over the blocks of d_sel into d_out [rows, q_heads, head_dim]
+        and, if given, d_lse [rows, q_heads] float32."""
+        check(lib().fi8_kb_attend_async(self._h, C.c_void_p(d_q), q_stride or self._width, C.c_void_p(d_slot),
+                                        C.c_void_p(d_len), rows, C.c_void_p(d_sel), k, scale, C.c_void_p(d_out),
+                                        C.c_void_p(d_lse or None), C.c_void_p(stream or None)))
+
+    def query_async(self, d_q: int, d_slot: int, d_len: int, rows: int, k: int, scale: float, d_sel: int, d_out: int,
+                    d_lse: int = 0, first: int = 1, last: int = 1, stream: int = 0, q_stride: int = 0) -> None:
+        """select_async, then attend_async."""
+        check(lib().fi8_kb_query_async(self._h, C.c_void_p(d_q), q_stride or self._width, C.c_void_p(d_slot),
+                                       C.c_void_p(d_len), rows, k, first, last, scale, C.c_void_p(d_sel),
+                                       C.c_void_p(d_out), C.c_void_p(d_lse or None), C.c_void_p(stream or None)))
+
+    def read_rows(self, slot: int):
+        """A slot's block rows, copied to the host: codes [kv_heads, blocks, G, 16],
+        mults [kv_heads, blocks, G], scales [kv_heads, blocks]."""
+        shape, groups = (self.kv_heads, self.capacity // self.block), (self.head_dim + 31) // 32
+        codes = np.empty((*shape, groups, 16), np.uint8)
+        mults = np.empty((*shape, groups), np.uint8)
+        scales = np.empty(shape, np.float32)
+        check(lib().fi8_kb_read_rows(self._h, slot, _p(codes), _p(mults), _p(scales)))
+        return codes, mults, scales
+
+    def sync(self) -> None:
+        """Wait for the device; raises if a call met a slot or length outside the cache."""
+        check(lib().fi8_kb_sync(self._h))
+
+    def Close(self) -> None:
+        if self._h:
+            check(lib().fi8_kb_destroy(self._h))
+            self._h = None
 
     def __del__(self):
         try:

@@ -19,9 +19,10 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 
-CUDA_SOURCES = ["fi8_api.cu", "fi8_scan.cu", "fi8_gemm.cu", "fi8_binary.cu", "fi8_build.cu", "fi8_i4.cu", "fi8_i4_api.cu"]
+CUDA_SOURCES = ["fi8_api.cu", "fi8_scan.cu", "fi8_gemm.cu", "fi8_binary.cu", "fi8_build.cu", "fi8_i4.cu", "fi8_i4_api.cu",
+                "fi8_kb.cu", "fi8_kb_api.cu"]
 CUDA_HEADERS = ["fi8_device.cuh", "fi8_scan.cuh", "fi8_select.cuh", "fi8_gemm.cuh", "fi8_binary.cuh", "fi8_build.cuh", "fi8_stage.h",
-                "fi8_host.h", "fi8_i4.cuh", "fi8_i4q.cuh"]
+                "fi8_host.h", "fi8_i4.cuh", "fi8_i4q.cuh", "fi8_kb.cuh"]
 SYNTH_SOURCES = ["synth.c"]
 
 NVCC = os.environ.get("NVCC", "nvcc")
@@ -53,7 +54,7 @@ def build_fi8(force: bool = False, ptxas: bool = False) -> str:
     if not (force or ptxas) and not _stale(LIB_FI8, deps):
         return LIB_FI8
     os.makedirs(LIBDIR, exist_ok=True)
-    cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O2",
+    cmd = [NVCC, *ARCH, "-lineinfo", "-O3", "-std=c++17", "--threads", "0", "-Xcompiler", "-fPIC,-O2",
            "-shared", "-o", LIB_FI8, *srcs, "-lcudart"]
     if ptxas:
         cmd.insert(1, "-Xptxas=-v")

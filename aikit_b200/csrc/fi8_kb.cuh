@@ -1,0 +1,53 @@
+// fi8_kb.cuh -- KeyBlocks: block-sparse attention over a key/value cache whose
+// blocks are chosen by their FlatI4 rows.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+#include "fi8_i4.cuh"
+
+namespace fi8 {
+
+constexpr int32_t kKbMaxHeadDim = 256;
+constexpr int32_t kKbMaxBlock = 128;
+constexpr int32_t kKbMaxGroup = 64;       // query heads of a key/value head
+constexpr int32_t kKbMaxSelect = 1024;    // blocks a query row may read
+constexpr int32_t kKbMaxBlocks = 49152;   // blocks of a slot: their scores fit one CTA's shared memory
+constexpr int32_t kKbMaxRows = 65535;     // query rows of a call
+
+// Everything a launch needs. Strides in elements.
+struct KbParams {
+  const void* k;
+  const void* v;
+  int64_t slot_stride, head_stride, token_stride;
+  int64_t capacity;
+  int32_t slots, kv_heads, q_heads, head_dim, block, max_blocks;
+  bool f16;
+  // one row a (slot, kv head, full block): [slots][kv_heads][max_blocks]
+  uint8_t* codes;
+  uint8_t* mults;
+  float* scales;
+  int32_t groups, mpitch;
+  unsigned int* err;  // device error flags (kKbErrRow)
+  // a call's query rows
+  const void* q;
+  int64_t q_stride;
+  const int32_t* slot;
+  const int32_t* len;
+  int32_t rows, select, first, last;
+  int32_t* sel;  // [rows][kv_heads][select]
+  float scale;
+  void* out;
+  float* lse;
+};
+
+constexpr unsigned int kKbErrRow = 2u;  // a slot, length or range outside the cache
+
+cudaError_t kb_update_launch(const KbParams& p, const int32_t* slot, const int32_t* from, const int32_t* to,
+                             int32_t count, int32_t max_tokens, cudaStream_t stream);
+cudaError_t kb_select_launch(const KbParams& p, cudaStream_t stream);
+cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream);
+
+}  // namespace fi8

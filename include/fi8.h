@@ -416,6 +416,94 @@ int fi8_i4_topk_batch(fi8_i4* idx, const float* q, int32_t M, int32_t k, const u
 int fi8_i4_topk_async(fi8_i4* idx, const float* d_q, int32_t M, int32_t k, const uint64_t* d_keep, int64_t nbits,
                       uint64_t* d_keys, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * KeyBlocks: attention over a long key/value cache that reads only the blocks
+ * a cheap score selects -- the FlatBinaryI8 idea (a prefilter, then the real
+ * thing on its shortlist) inside a model. The cache stays the caller's; the
+ * handle keeps one FlatI4 row a (slot, key/value head, full block): the mean of
+ * the block's keys. No counterpart in the reference.
+ *
+ * The cache holds slots sequences of up to capacity tokens. The key of (slot,
+ * head, token) starts at d_k + slot * slot_stride + head * head_stride + token *
+ * token_stride (in values; head_dim contiguous values follow), its value at the
+ * same place of d_v. Addresses are 16-byte aligned, strides multiples of 8.
+ * head_dim is a multiple of 16 up to 256, block 16, 32, 64 or 128, capacity at
+ * most 49152 blocks, and a key/value head has at most 64 query heads.
+ *
+ * A query row has q_heads * head_dim values of the cache's type (rows q_stride
+ * values apart, 16-byte aligned), a slot, and the number len of its slot's
+ * tokens that it sees. Rows of one call may share a slot (drafted tokens, a
+ * prompt's chunk: len grows by one). Slots and lengths are read on the device;
+ * one outside the cache makes its row see nothing and is reported by
+ * fi8_kb_sync (FI8_ERR_DEVICE).
+ *
+ * Streams: every async call runs in stream order on stream (NULL: the legacy
+ * default stream), allocates nothing and never synchronizes, so it can be
+ * captured. A handle has no scratch: calls that only read may overlap, and an
+ * update must be ordered before the calls that need its blocks.
+ * ------------------------------------------------------------------------- */
+#define FI8_BF16 1
+#define FI8_F16 2
+
+typedef struct fi8_kb fi8_kb; /* block rows over one layer's cache */
+
+typedef struct fi8_kb_desc {
+  int32_t dtype;       /* FI8_BF16 or FI8_F16: keys, values, queries, outputs */
+  int32_t slots;
+  int32_t kv_heads;
+  int32_t q_heads;     /* a multiple of kv_heads; head i reads key/value head i / (q_heads / kv_heads) */
+  int32_t head_dim;
+  int32_t block;       /* tokens of a block */
+  int32_t max_rows;    /* query rows of a call, at most 65535 */
+  int32_t max_select;  /* blocks a row may read, at most 1024 */
+  int64_t capacity;    /* tokens of a slot */
+  const void* d_k;
+  const void* d_v;
+  int64_t slot_stride, head_stride, token_stride;
+} fi8_kb_desc;
+
+int fi8_kb_create(fi8_ctx* ctx, const fi8_kb_desc* desc, fi8_kb** out);
+int fi8_kb_destroy(fi8_kb* kb);
+
+/* Make the rows of every block that is full once tokens [d_from[i], d_to[i]) of
+ * slot d_slot[i] are in the cache, i < count, from block d_from[i] / block on.
+ * max_tokens bounds d_to[i] - d_from[i] (tokens past it may keep old rows). A
+ * row is the keys' mean (summed exactly, rounded to float32), quantized as
+ * fi8_i4_set_rows_async does. The same slot may not come twice with ranges that
+ * share a block. */
+int fi8_kb_update_async(fi8_kb* kb, const int32_t* d_slot, const int32_t* d_from, const int32_t* d_to, int32_t count,
+                        int32_t max_tokens, void* stream);
+
+/* Choose the blocks of rows query rows: d_sel [rows][kv_heads][k] block numbers,
+ * ascending, -1 padded. A row of len tokens sees ceil(len / block) blocks. If
+ * these are at most k, all; else the first `first`, the last `last` (at least
+ * one: the newest block may not be full) and the best others, k in all, by
+ * (score desc, number asc); a block's score is the largest FlatI4 score of the
+ * head group's queries against its row (NaN scores last). */
+int fi8_kb_select_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int32_t* d_slot, const int32_t* d_len,
+                        int32_t rows, int32_t k, int32_t first, int32_t last, int32_t* d_sel, void* stream);
+
+/* Attention over chosen blocks (d_sel as above, in any order; numbers outside
+ * the row's blocks are skipped, one that is repeated counts again):
+ * d_out [rows][q_heads][head_dim] = softmax(scale * q.k) v over the tokens below
+ * len of those blocks, and d_lse [rows][q_heads] (or NULL) the natural log of
+ * the softmax's sum. A row that sees nothing gets zeros and -inf. */
+int fi8_kb_attend_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int32_t* d_slot, const int32_t* d_len,
+                        int32_t rows, const int32_t* d_sel, int32_t k, float scale, void* d_out, float* d_lse,
+                        void* stream);
+
+/* Both: select into d_sel, then attend. */
+int fi8_kb_query_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int32_t* d_slot, const int32_t* d_len,
+                       int32_t rows, int32_t k, int32_t first, int32_t last, float scale, int32_t* d_sel, void* d_out,
+                       float* d_lse, void* stream);
+
+/* A slot's block rows, copied to the host (waits for the device): codes
+ * [kv_heads][capacity / block][G * 16], mults [..][G], scales [..]. */
+int fi8_kb_read_rows(fi8_kb* kb, int32_t slot, uint8_t* codes, uint8_t* mults, float* scales);
+
+/* Wait for the device and report a slot, length or range that a call refused. */
+int fi8_kb_sync(fi8_kb* kb);
+
 #ifdef __cplusplus
 }
 #endif
