@@ -1,5 +1,5 @@
 // fi8_i4.cuh -- FlatI4 rows: vectors in 4 bits a value, and the kernels over
-// them (row quantization, scores, exact top-k of scores).
+// them (row quantization, scores, exact top-k).
 //
 // Format. dim values are padded with zeros to G = ceil(dim / 32) groups of 32.
 // A group's codes c in [-8, 7] are the nibbles c + 8 of 16 bytes (byte i: value
@@ -15,6 +15,12 @@
 // is a whole number: any order of summation gives the same int32, every score
 // float32(dot) * qscale * s has one value, and top-k ties are exact. |dot| is
 // at most 8 * 255 * 127 * dim, so dim <= 4096 stays below 2^31 (8288 would).
+//
+// Device layout. Eight rows are interleaved word by word: lane l = 4 r + t of a
+// warp owns word t of row r, as the operand of an 8-bit matrix instruction
+// wants it, and its words of four groups are 16 neighbouring bytes. So a warp
+// reads 8 rows x 4 groups with one 16-byte load a lane, 512 contiguous bytes,
+// straight into operand registers.
 #pragma once
 
 #include <cstddef>
@@ -25,52 +31,61 @@ namespace fi8 {
 
 constexpr int32_t kI4Group = 32;
 constexpr int32_t kI4MaxDim = 4096;
-constexpr int32_t kI4MaxBatch = 8;       // queries of one score launch (a pass over the rows)
+constexpr int32_t kI4MaxBatch = 16;  // queries of one pass over the rows
 constexpr int32_t kI4MaxK = 2048;
-constexpr int32_t kI4SelectTile = 1024;  // scores a select CTA reads at a time
-constexpr int32_t kI4SelectCtas = 296;   // select CTAs of a launch, all queries together (two an SM)
+constexpr int32_t kI4Tile = 32;      // rows that a warp scores together
 
 inline int32_t i4_groups(int32_t dim) { return (dim + kI4Group - 1) / kI4Group; }
-// Bytes of a row's multipliers: whole words.
-inline int32_t i4_mult_pitch(int32_t groups) { return (groups + 3) / 4 * 4; }
 
-// Rows on the device. codes [n][groups * 16], mults [n][mpitch], scales [n].
+// Rows on the device, n rounded up to whole tiles. A block of 8 rows has
+//   codes [groups / 4 quads][32 lanes][4 groups] words, then, when groups is no
+//         multiple of 4, [32 lanes][groups % 4] words;
+//   mults [(groups + 3) / 4][8 rows] words, a byte a group.
 struct I4Rows {
-  uint8_t* codes;
-  uint8_t* mults;
+  uint32_t* codes;
+  uint32_t* mults;
   float* scales;
   int64_t n;
-  int32_t dim, groups, mpitch;
+  int32_t dim, groups;
 };
+
+inline int64_t i4_tiles(int64_t n) { return (n + kI4Tile - 1) / kI4Tile; }
+inline size_t i4_code_bytes(int64_t n, int32_t groups) { return (size_t)i4_tiles(n) * kI4Tile * groups * 16; }
+inline size_t i4_mult_bytes(int64_t n, int32_t groups) { return (size_t)i4_tiles(n) * kI4Tile * ((groups + 3) / 4) * 4; }
 
 // Quantize float32 rows v [rows][dim] into rows [row0, row0 + rows).
 cudaError_t i4_quantize_launch(const I4Rows& r, int64_t row0, const float* v, int64_t rows, cudaStream_t stream);
 
-// Scores of M <= kI4MaxBatch queries q [M][dim] against rows [row0, row0 + rows):
-// dst[m * ld + (row - row0)].
+// Rows [row0, row0 + rows) from or to the row-major format: codes
+// [rows][groups * 16], mults [rows][groups], scales [rows] (all on the device).
+cudaError_t i4_pack_launch(const I4Rows& r, int64_t row0, int64_t rows, const uint8_t* codes, const uint8_t* mults,
+                           const float* scales, cudaStream_t stream);
+cudaError_t i4_unpack_launch(const I4Rows& r, int64_t row0, int64_t rows, uint8_t* codes, uint8_t* mults, float* scales,
+                             cudaStream_t stream);
+
+// Scores of M <= kI4MaxBatch queries q [M][dim] against rows [row0, row0 + rows),
+// row0 a whole tile: dst[m * ld + (row - row0)].
 cudaError_t i4_score_launch(const I4Rows& r, int64_t row0, int64_t rows, const float* q, int32_t M, float* dst,
                             int64_t ld, int32_t sm_count, cudaStream_t stream);
 
-// Top-k of M score rows, exact under (score desc, index asc), NaN excluded.
-struct I4Select {
-  const float* scores;   // [M][ld], 16-byte aligned, ld a multiple of 4
-  int64_t ld, rows;
-  uint32_t id0;          // global id of score 0
+// Top-k of M <= kI4MaxBatch queries over all rows.
+struct I4TopK {
+  const float* q;        // [M][dim]
+  int32_t M, k;
+  uint32_t id_base;      // global id of row 0
   const uint64_t* keep;  // optional keep bitmap over global ids
   int64_t keep_nbits;
-  int32_t k, kp, cap, nslots;
-  int32_t ctas;          // CTAs of a query
-  unsigned long long* gthr;  // [M] shared threshold (zero at rest)
-  unsigned int* counter;     // [M][blocks] (zero at rest)
-  unsigned int* counter2;    // [M] (zero at rest)
-  uint64_t* lvl1;            // [M][ctas][kp]
-  uint64_t* lvl2;            // [M][blocks][kp]
-  uint64_t* out;             // [M][k] sorted keys, 0 = empty
+  uint32_t* best;        // [kI4MaxBatch][tiles] scratch: rank of each tile's best score
+  uint32_t* list;        // [kI4MaxBatch][kI4MaxK] scratch: the tiles that can hold the top k
+  uint64_t* cand;        // [kI4MaxBatch][i4_cand(n)] scratch: their rows' keys
+  uint64_t* out;         // [M][k] sorted keys, 0 = empty
 };
-
-// Fills kp, cap, nslots and ctas for a shape; returns the dynamic shared memory.
-size_t i4_select_plan(I4Select* s, int32_t M);
-cudaError_t i4_select_launch(const I4Select& s, int32_t M, size_t smem, cudaStream_t stream);
+// Keys that a query's tiles can hold.
+inline int64_t i4_cand(int64_t n) {
+  const int64_t tiles = i4_tiles(n);
+  return (tiles < kI4MaxK ? tiles : kI4MaxK) * kI4Tile;
+}
+cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, cudaStream_t stream);
 
 #ifdef __CUDACC__
 

@@ -1,8 +1,8 @@
 // fi8_i4_api.cu -- the C entry points of FlatI4 (include/fi8.h, fi8_i4_*).
 //
 // The async forms allocate nothing: an index owns, from its creation on, the
-// score scratch and the select lists that its largest call needs, so they can
-// be captured into a graph and their addresses never change.
+// scratch that its largest call needs (in one allocation with its rows), so
+// they can be captured into a graph and their addresses never change.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -12,16 +12,16 @@
 #include "fi8_device.cuh"
 #include "fi8_host.h"
 #include "fi8_i4.cuh"
-#include "fi8_scan.cuh"
 #include "fi8_stage.h"
 
 using namespace fi8;
 
 namespace {
 
-// Scores of a top-k pass held at once. 64 MB stay in the 126 MB L2, so the
-// select reads them from there; a larger pass runs as row ranges.
-constexpr int64_t kScoreScratch = 16 << 20;
+// Scores that the host form of score_batch holds on the device at once.
+constexpr int64_t kHostScores = 16 << 20;
+// Bytes of packed rows that an upload or a read holds on the device at once.
+constexpr size_t kPackBytes = (size_t)64 << 20;
 
 }  // namespace
 
@@ -33,14 +33,10 @@ struct fi8_i4 {
   cudaStream_t stream = nullptr;  // the host-pointer forms and the uploads
   std::mutex mu;
 
-  // top-k scratch
-  float* d_scores = nullptr;
-  int64_t scores_cap = 0;
-  uint64_t* d_lists = nullptr;  // sorted keys of the row ranges of a pass, null when there is one range
-  uint64_t* d_lvl1 = nullptr;
-  uint64_t* d_lvl2 = nullptr;
-  unsigned long long* d_gthr = nullptr;  // [8], zero at rest
-  unsigned int* d_counter = nullptr;     // zero at rest; the last 8 are the block tickets
+  unsigned char* d_base = nullptr;  // rows and top-k scratch
+  uint32_t* d_best = nullptr;
+  uint32_t* d_list = nullptr;
+  uint64_t* d_cand = nullptr;
   // staging of the host-pointer forms
   float* d_q = nullptr;
   size_t q_cap = 0;
@@ -50,30 +46,17 @@ struct fi8_i4 {
   size_t h_keys_cap = 0;
   uint64_t* d_keep = nullptr;
   size_t keep_cap = 0;
+  float* d_scores = nullptr;
+  size_t scores_cap = 0;
 };
 
 namespace {
 
-constexpr int32_t kCounters = kI4SelectCtas + kI4MaxBatch;  // block tickets of every query, then one a query
-
-// Rows of one range of a pass of M queries.
-int64_t range_rows(const fi8_i4* x, int32_t M) {
-  const int64_t most = x->scores_cap / M / kI4SelectTile * kI4SelectTile;
-  return std::min<int64_t>(x->rows.n, most);
-}
-
 void i4_free(fi8_i4* x) {
   DeviceGuard g(x->device);
   if (x->stream) cudaStreamSynchronize(x->stream);
-  cudaFree(x->rows.codes);
-  cudaFree(x->rows.mults);
-  cudaFree(x->rows.scales);
+  cudaFree(x->d_base);
   cudaFree(x->d_scores);
-  cudaFree(x->d_lists);
-  cudaFree(x->d_lvl1);
-  cudaFree(x->d_lvl2);
-  cudaFree(x->d_gthr);
-  cudaFree(x->d_counter);
   cudaFree(x->d_q);
   cudaFree(x->d_keys);
   cudaFree(x->d_keep);
@@ -101,36 +84,34 @@ int i4_alloc(fi8_ctx* ctx, int64_t n, int32_t dim, int64_t id_base, const char* 
   r.n = n;
   r.dim = dim;
   r.groups = i4_groups(dim);
-  r.mpitch = i4_mult_pitch(r.groups);
-  const int64_t n_tile = (n + kI4SelectTile - 1) / kI4SelectTile * kI4SelectTile;
-  x->scores_cap = std::min<int64_t>(kI4MaxBatch * n_tile, kScoreScratch);
-  size_t lists = 0;
-  for (int32_t m = 1; m <= kI4MaxBatch; m++) {
-    const int64_t per = range_rows(x, m), ranges = (n + per - 1) / per;
-    if (ranges > 1) lists = std::max(lists, (size_t)ranges * m * kI4MaxK);
-  }
-  const size_t ctas = (size_t)std::min<int64_t>(kI4SelectCtas, kI4MaxBatch * (n_tile / kI4SelectTile));
+  // one allocation: codes, multipliers, scales, then the scratch
+  size_t at = 0;
+  auto part = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+  };
+  const size_t tiles = (size_t)i4_tiles(n);
+  const size_t codes = part(i4_code_bytes(n, r.groups)), mults = part(i4_mult_bytes(n, r.groups));
+  const size_t scales = part(tiles * kI4Tile * sizeof(float)), rows_end = at;
+  const size_t best = part((size_t)kI4MaxBatch * tiles * sizeof(uint32_t));
+  const size_t list = part((size_t)kI4MaxBatch * kI4MaxK * sizeof(uint32_t));
+  const size_t cand = part((size_t)kI4MaxBatch * i4_cand(n) * sizeof(uint64_t));
   cudaError_t e = cudaStreamCreateWithFlags(&x->stream, cudaStreamNonBlocking);
-  if (e == cudaSuccess) e = cudaMalloc(&r.codes, (size_t)n * r.groups * 16);
-  if (e == cudaSuccess) e = cudaMalloc(&r.mults, (size_t)n * r.mpitch);
-  if (e == cudaSuccess) e = cudaMalloc(&r.scales, (size_t)n * sizeof(float));
-  if (e == cudaSuccess) e = cudaMalloc(&x->d_scores, (size_t)x->scores_cap * sizeof(float));
-  if (e == cudaSuccess && lists) e = cudaMalloc(&x->d_lists, lists * sizeof(uint64_t));
-  if (e == cudaSuccess) e = cudaMalloc(&x->d_lvl1, ctas * kI4MaxK * sizeof(uint64_t));
-  if (e == cudaSuccess) e = cudaMalloc(&x->d_lvl2, (ctas / 8 + kI4MaxBatch) * kI4MaxK * sizeof(uint64_t));
-  if (e == cudaSuccess) e = cudaMalloc(&x->d_gthr, kI4MaxBatch * sizeof(unsigned long long));
-  if (e == cudaSuccess) e = cudaMalloc(&x->d_counter, kCounters * sizeof(unsigned int));
-  if (e == cudaSuccess) e = cudaMemsetAsync(r.codes, 0, (size_t)n * r.groups * 16, x->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(r.mults, 0, (size_t)n * r.mpitch, x->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(r.scales, 0, (size_t)n * sizeof(float), x->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(x->d_gthr, 0, kI4MaxBatch * sizeof(unsigned long long), x->stream);
-  if (e == cudaSuccess) e = cudaMemsetAsync(x->d_counter, 0, kCounters * sizeof(unsigned int), x->stream);
+  if (e == cudaSuccess) e = cudaMalloc(&x->d_base, at);
+  if (e == cudaSuccess) e = cudaMemsetAsync(x->d_base, 0, rows_end, x->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(x->stream);
   if (e != cudaSuccess) {
     const int rc = cuda_fail(e, "gpu: device allocation failed");
     i4_free(x);
     return rc;
   }
+  r.codes = reinterpret_cast<uint32_t*>(x->d_base + codes);
+  r.mults = reinterpret_cast<uint32_t*>(x->d_base + mults);
+  r.scales = reinterpret_cast<float*>(x->d_base + scales);
+  x->d_best = reinterpret_cast<uint32_t*>(x->d_base + best);
+  x->d_list = reinterpret_cast<uint32_t*>(x->d_base + list);
+  x->d_cand = reinterpret_cast<uint64_t*>(x->d_base + cand);
   *out = x;
   return FI8_OK;
 }
@@ -147,35 +128,19 @@ int launch_scores(fi8_i4* x, const float* d_q, int32_t M, float* d_dst, cudaStre
 
 int launch_topk(fi8_i4* x, const float* d_q, int32_t M, int32_t k, const uint64_t* d_keep, int64_t nbits,
                 uint64_t* d_keys, cudaStream_t st) {
-  const int64_t n = x->rows.n;
   for (int32_t m0 = 0; m0 < M; m0 += kI4MaxBatch) {
-    const int32_t mm = std::min(kI4MaxBatch, M - m0);
-    const int64_t per = range_rows(x, mm), ranges = (n + per - 1) / per;
-    uint64_t* out = d_keys + (size_t)m0 * k;
-    for (int64_t i = 0; i < ranges; i++) {
-      const int64_t row0 = i * per, rows = std::min(per, n - row0);
-      I4Select s{};
-      s.scores = x->d_scores;
-      s.ld = (rows + 3) / 4 * 4;
-      s.rows = rows;
-      s.id0 = x->id_base + (uint32_t)row0;
-      s.keep = d_keep;
-      s.keep_nbits = nbits;
-      s.k = k;
-      s.gthr = x->d_gthr;
-      s.counter = x->d_counter;
-      s.counter2 = x->d_counter + kI4SelectCtas;
-      s.lvl1 = x->d_lvl1;
-      s.lvl2 = x->d_lvl2;
-      s.out = ranges == 1 ? out : x->d_lists + (size_t)i * mm * k;
-      const size_t smem = i4_select_plan(&s, mm);
-      FI8_CUDA(i4_score_launch(x->rows, row0, rows, d_q + (size_t)m0 * x->rows.dim, mm, x->d_scores, s.ld,
-                               x->sm_count, st),
-               "i4_score_launch");
-      FI8_CUDA(i4_select_launch(s, mm, smem, st), "i4_select_launch");
-    }
-    if (ranges > 1)
-      FI8_CUDA(merge_keys_launch(x->d_lists, (int32_t)ranges, mm, k, out, st), "merge_keys_launch");
+    I4TopK p{};
+    p.q = d_q + (size_t)m0 * x->rows.dim;
+    p.M = std::min(kI4MaxBatch, M - m0);
+    p.k = k;
+    p.id_base = x->id_base;
+    p.keep = d_keep;
+    p.keep_nbits = nbits;
+    p.best = x->d_best;
+    p.list = x->d_list;
+    p.cand = x->d_cand;
+    p.out = d_keys + (size_t)m0 * k;
+    FI8_CUDA(i4_topk_launch(x->rows, p, x->sm_count, st), "i4_topk_launch");
   }
   return FI8_OK;
 }
@@ -188,6 +153,28 @@ int stage_queries(fi8_i4* x, const float* q, int32_t M) {
   FI8_CUDA(cudaMemcpyAsync(x->d_q, q, count * sizeof(float), cudaMemcpyHostToDevice, x->stream), "H2D queries");
   return FI8_OK;
 }
+
+// A part of the rows in the row-major format, on the device.
+struct PackBuffer {
+  int64_t rows = 0;
+  unsigned char* base = nullptr;
+  uint8_t* codes = nullptr;
+  uint8_t* mults = nullptr;
+  float* scales = nullptr;
+  cudaError_t error;
+  explicit PackBuffer(const I4Rows& r) {
+    const size_t row = (size_t)r.groups * 17 + 4;
+    rows = std::max<int64_t>(1, std::min<int64_t>(r.n, (int64_t)(kPackBytes / row)));
+    error = cudaMalloc(&base, rows * row);
+    if (error != cudaSuccess) return;
+    scales = reinterpret_cast<float*>(base + rows * r.groups * 16);
+    codes = base;
+    mults = base + rows * (r.groups * 16 + 4);
+  }
+  ~PackBuffer() { cudaFree(base); }
+  PackBuffer(const PackBuffer&) = delete;
+  PackBuffer& operator=(const PackBuffer&) = delete;
+};
 
 // Upload through pinned buffers; the host threads of the stager may throw.
 template <typename F>
@@ -221,14 +208,23 @@ int fi8_i4_create(fi8_ctx* ctx, const uint8_t* codes, const uint8_t* mults, cons
   int rc = i4_alloc(ctx, n, dim, id_base, "fi8_i4_create", &x);
   if (rc != FI8_OK) return rc;
   DeviceGuard g(x->device);
-  const I4Rows& r = x->rows;
-  const cudaError_t e = with_stager([&](PinnedStager& stage) {
-    cudaError_t c = stage.put_rows(r.codes, (size_t)r.groups * 16, codes, (size_t)r.groups * 16, (size_t)r.groups * 16,
-                                   n, x->stream);
-    if (c == cudaSuccess) c = stage.put_rows(r.mults, r.mpitch, mults, r.groups, r.groups, n, x->stream);
-    if (c == cudaSuccess) c = stage.put_rows(r.scales, 4, scales, 4, 4, n, x->stream);
-    return c;
-  });
+  const PackBuffer b(x->rows);
+  cudaError_t e = b.error;
+  if (e == cudaSuccess)
+    e = with_stager([&](PinnedStager& stage) {
+      const size_t cb = (size_t)x->rows.groups * 16, mb = x->rows.groups;
+      cudaError_t c = cudaSuccess;
+      for (int64_t r0 = 0; c == cudaSuccess && r0 < n; r0 += b.rows) {
+        // stream order keeps the next chunk's copies behind this chunk's kernel
+        const int64_t rows = std::min(b.rows, n - r0);
+        c = stage.put_rows(b.codes, cb, codes + (size_t)r0 * cb, cb, cb, rows, x->stream);
+        if (c == cudaSuccess) c = stage.put_rows(b.mults, mb, mults + (size_t)r0 * mb, mb, mb, rows, x->stream);
+        if (c == cudaSuccess) c = stage.put_rows(b.scales, 4, scales + r0, 4, 4, rows, x->stream);
+        if (c == cudaSuccess) c = i4_pack_launch(x->rows, r0, rows, b.codes, b.mults, b.scales, x->stream);
+      }
+      return c;
+    });
+  if (e == cudaSuccess) e = cudaStreamSynchronize(x->stream);
   if (e != cudaSuccess) {
     rc = cuda_fail(e, "gpu: device upload failed");
     i4_free(x);
@@ -289,11 +285,18 @@ int fi8_i4_read_rows(fi8_i4* idx, uint8_t* codes, uint8_t* mults, float* scales)
   std::lock_guard<std::mutex> lk(idx->mu);
   DeviceGuard g(idx->device);
   const I4Rows& r = idx->rows;
+  const PackBuffer b(r);
+  FI8_CUDA(b.error, "fi8_i4_read_rows");
   FI8_CUDA(cudaDeviceSynchronize(), "sync");  // rows set on any stream
-  FI8_CUDA(cudaMemcpy(codes, r.codes, (size_t)r.n * r.groups * 16, cudaMemcpyDeviceToHost), "fi8_i4_read_rows");
-  FI8_CUDA(cudaMemcpy2D(mults, r.groups, r.mults, r.mpitch, r.groups, (size_t)r.n, cudaMemcpyDeviceToHost),
-           "fi8_i4_read_rows");
-  FI8_CUDA(cudaMemcpy(scales, r.scales, (size_t)r.n * sizeof(float), cudaMemcpyDeviceToHost), "fi8_i4_read_rows");
+  const size_t cb = (size_t)r.groups * 16, mb = r.groups;
+  for (int64_t r0 = 0; r0 < r.n; r0 += b.rows) {
+    const int64_t rows = std::min(b.rows, r.n - r0);
+    FI8_CUDA(i4_unpack_launch(r, r0, rows, b.codes, b.mults, b.scales, idx->stream), "i4_unpack_launch");
+    FI8_CUDA(cudaMemcpyAsync(codes + (size_t)r0 * cb, b.codes, rows * cb, cudaMemcpyDeviceToHost, idx->stream), "D2H codes");
+    FI8_CUDA(cudaMemcpyAsync(mults + (size_t)r0 * mb, b.mults, rows * mb, cudaMemcpyDeviceToHost, idx->stream), "D2H mults");
+    FI8_CUDA(cudaMemcpyAsync(scales + r0, b.scales, rows * 4, cudaMemcpyDeviceToHost, idx->stream), "D2H scales");
+  }
+  FI8_CUDA(cudaStreamSynchronize(idx->stream), "sync");
   return FI8_OK;
 }
 
@@ -323,9 +326,11 @@ int fi8_i4_score_batch(fi8_i4* idx, const float* q, int32_t M, float* dst) {
   const int64_t n = x->rows.n;
   int rc = stage_queries(x, q, M);
   if (rc != FI8_OK) return rc;
+  const int64_t per = std::min<int64_t>(i4_tiles(n) * kI4Tile, kHostScores / kI4MaxBatch);
+  rc = ensure_device(&x->d_scores, &x->scores_cap, (size_t)(std::min(M, kI4MaxBatch) * per), "staging scores");
+  if (rc != FI8_OK) return rc;
   for (int32_t m0 = 0; m0 < M; m0 += kI4MaxBatch) {
     const int32_t mm = std::min(kI4MaxBatch, M - m0);
-    const int64_t per = range_rows(x, mm);
     for (int64_t row0 = 0; row0 < n; row0 += per) {
       const int64_t rows = std::min(per, n - row0);
       FI8_CUDA(i4_score_launch(x->rows, row0, rows, x->d_q + (size_t)m0 * x->rows.dim, mm, x->d_scores, rows,

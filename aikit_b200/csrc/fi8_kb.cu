@@ -5,6 +5,7 @@
 
 #include <cmath>
 
+#include "fi8_cluster.cuh"
 #include "fi8_i4q.cuh"
 #include "fi8_kb.cuh"
 #include "fi8_select.cuh"
@@ -325,27 +326,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-
 // Byte offset of 16-byte chunk c of row r in a tile of DP-element rows; the
 // chunk index is permuted by the row so that eight rows' equal chunks fall
 // into different banks.

@@ -43,6 +43,9 @@ struct KbParams {
   float* lse;
 };
 
+// Bytes of a block row's multipliers: whole words.
+inline int32_t kb_mult_pitch(int32_t groups) { return (groups + 3) / 4 * 4; }
+
 constexpr unsigned int kKbErrRow = 2u;  // a slot, length or range outside the cache
 
 cudaError_t kb_update_launch(const KbParams& p, const int32_t* slot, const int32_t* from, const int32_t* to,

@@ -123,7 +123,7 @@ int fi8_kb_create(fi8_ctx* ctx, const fi8_kb_desc* desc, fi8_kb** out) {
   p.max_blocks = (int32_t)(d.capacity / d.block);
   p.f16 = d.dtype == FI8_F16;
   p.groups = i4_groups(d.head_dim);
-  p.mpitch = i4_mult_pitch(p.groups);
+  p.mpitch = kb_mult_pitch(p.groups);
   const size_t rows = (size_t)d.slots * d.kv_heads * p.max_blocks + 1;  // never an empty allocation
   DeviceGuard g(b->device);
   cudaError_t e = cudaMalloc(&p.codes, rows * p.groups * 16);

@@ -402,7 +402,7 @@ int fi8_i4_read_rows(fi8_i4* idx, uint8_t* codes, uint8_t* mults, float* scales)
 int fi8_i4_destroy(fi8_i4* idx);
 int fi8_i4_info(fi8_i4* idx, int64_t* n, int32_t* dim);
 
-/* Scores of M queries q [M*dim] against every row: dst [M*n]. Eight queries
+/* Scores of M queries q [M*dim] against every row: dst [M*n]. Sixteen queries
  * share one pass over the rows. */
 int fi8_i4_score_batch(fi8_i4* idx, const float* q, int32_t M, float* dst);
 int fi8_i4_score_async(fi8_i4* idx, const float* d_q, int32_t M, float* d_dst, void* stream);
