@@ -1,6 +1,7 @@
 // fi8_i4.cu -- FlatI4: scores of 4-bit rows (a matrix-vector product with
 // group scales), the row quantizer, and the exact top-k.
 #include "fi8_cluster.cuh"
+#include "fi8_cp_async.cuh"
 #include "fi8_i4.cuh"
 #include "fi8_i4q.cuh"
 
@@ -10,10 +11,11 @@ namespace {
 
 constexpr int kWarps = 8;
 
-// Word index of lane l's word of group g in its block of 8 rows.
-__device__ __forceinline__ int i4_word_at(int g, int lane, int groups) {
-  const int full = groups & ~3;
-  return g < full ? (g >> 2) * 128 + lane * 4 + (g & 3) : full * 32 + lane * (groups & 3) + (g - full);
+// Word index, in its tile, of word t of group g of row r (0 .. 31).
+__device__ __forceinline__ int i4_word_at(int g, int r, int t, int groups) {
+  const int full = groups & ~3, block = r >> 3, lane = (r & 7) * 4 + t;
+  return g < full ? (g >> 2) * 512 + (block * 32 + lane) * 4 + (g & 3)
+                  : full * 128 + (block * (groups & 3) + g - full) * 32 + lane;
 }
 
 // ---------------------------------------------------------------------------
@@ -36,16 +38,19 @@ __device__ __forceinline__ void i4_write_block(const I4Rows& r, int64_t row0, in
     if (lane == 0) r.scales[row] = scale;
   }
   __syncthreads();
-  uint32_t* codes = r.codes + (size_t)block * G * 32;
-  uint32_t* mults = r.mults + (size_t)block * quads * 8;
+  uint32_t* codes = r.codes + (size_t)(block >> 2) * G * 128;
+  uint32_t* mults = r.mults + (size_t)(block >> 2) * quads * 32;
+  const int in_tile = (int)(block & 3) * 8;
   for (int i = threadIdx.x; i < G * 32; i += kWarps * 32) {
-    const int g = i >> 5, l = i & 31;
-    const int64_t at = block * 8 + (l >> 2);
-    if (at >= row0 && at < row0 + rows) codes[i4_word_at(g, l, G)] = s_codes[(l >> 2) * G * 4 + g * 4 + (l & 3)];
+    const int g = i >> 5, rr = (i & 31) >> 2, t = i & 3;
+    const int64_t at = block * 8 + rr;
+    if (at >= row0 && at < row0 + rows) codes[i4_word_at(g, in_tile + rr, t, G)] = s_codes[rr * G * 4 + g * 4 + t];
   }
   for (int i = threadIdx.x; i < quads * 8; i += kWarps * 32) {
-    const int64_t at = block * 8 + (i & 7);
-    if (at >= row0 && at < row0 + rows) mults[i] = reinterpret_cast<const uint32_t*>(s_mults)[(i & 7) * quads + (i >> 3)];
+    const int rr = i & 7, quad = i >> 3;
+    const int64_t at = block * 8 + rr;
+    if (at >= row0 && at < row0 + rows)
+      mults[quad * 32 + in_tile + rr] = reinterpret_cast<const uint32_t*>(s_mults)[rr * quads + quad];
   }
 }
 
@@ -88,12 +93,12 @@ __global__ void __launch_bounds__(kWarps * 32) i4_unpack_kernel(I4Rows r, int64_
   const int lane = threadIdx.x & 31, G = r.groups, quads = (G + 3) / 4;
   const int64_t i = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (i >= rows) return;
-  const int64_t row = row0 + i, block = row / 8;
-  const int rr = (int)(row & 7);
+  const int64_t row = row0 + i, tile = row / kI4Tile;
+  const int rr = (int)(row % kI4Tile);
   uint32_t* out = reinterpret_cast<uint32_t*>(codes + (size_t)i * G * 16);
-  for (int j = lane; j < G * 4; j += 32) out[j] = r.codes[(size_t)block * G * 32 + i4_word_at(j >> 2, rr * 4 + (j & 3), G)];
+  for (int j = lane; j < G * 4; j += 32) out[j] = r.codes[(size_t)tile * G * 128 + i4_word_at(j >> 2, rr, j & 3, G)];
   for (int g = lane; g < G; g += 32)
-    mults[(size_t)i * G + g] = (uint8_t)(r.mults[((size_t)block * quads + (g >> 2)) * 8 + rr] >> (8 * (g & 3)));
+    mults[(size_t)i * G + g] = (uint8_t)(r.mults[((size_t)tile * quads + (g >> 2)) * 32 + rr] >> (8 * (g & 3)));
   if (lane == 0) scales[i] = r.scales[row];
 }
 
@@ -104,51 +109,55 @@ __global__ void __launch_bounds__(kWarps * 32) i4_unpack_kernel(I4Rows r, int64_
 // at -8 * sum(q8), the nibbles' offset, and enter the totals times the rows'
 // multipliers: a row's 16 bytes cost the same few instructions for one query
 // as for eight, and the rows' bytes bound the kernel. The queries' fragments
-// lie in shared memory, 16 bytes a lane and group. The words of the next four
-// groups are loaded while the present ones are multiplied.
+// lie in shared memory, 16 bytes a lane and group. A warp's words pass through
+// a ring of its own, kStages quads (four groups) deep, filled by asynchronous
+// copies; nothing but the warp itself waits for it.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int c0, int c1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], const uint2 b, const int4 c) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c0), "r"(c1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
 }
 
-// Four blocks of 8 rows, up to four groups: the lane's words and multipliers.
-struct I4Frag {
-  uint32_t w[4][4];
-  uint32_t m[4];
+constexpr int kStages = 4;
+constexpr int kScoreCtas = 2;              // CTAs an SM at most
+constexpr size_t kSmemSm = 228 * 1024;     // an SM's shared memory; a CTA takes 1 KB more than it asks for
+
+// One quad of a tile: the lanes' words of four blocks of 8 rows (a tile's last
+// quad may have fewer groups, [4 blocks][groups][32 lanes] words from the start
+// of w), the rows' multipliers.
+struct I4Stage {
+  uint4 w[4][32];
+  uint32_t m[32];
 };
 
-__device__ __forceinline__ void i4_load(I4Frag& f, const I4Rows& r, int64_t tile, int quad, int lane) {
-  const int G = r.groups, full = G >> 2, quads = (G + 3) >> 2;
-  const uint32_t* codes = r.codes + (size_t)tile * 4 * G * 32 + quad * 128;
-  const uint32_t* mults = r.mults + ((size_t)tile * 4 * quads + quad) * 8 + (lane >> 2);
+// The next quad to fetch for a warp: where its words and multipliers lie.
+struct I4Cursor {
+  const uint32_t* codes;  // of the quad, at the lane's first 16 bytes
+  const uint32_t* mults;
+  int quad;
+};
+
+__device__ __forceinline__ void i4_fetch(I4Stage& s, const I4Cursor& at, int G, int lane) {
+  const int pieces = min(4, G - at.quad * 4);  // of 32 x 16 bytes: a group of four blocks each
 #pragma unroll
-  for (int b = 0; b < 4; b++) {
-    const uint32_t* at = codes + (size_t)b * G * 32;
-    if (quad < full) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + lane);
-      f.w[b][0] = v.x, f.w[b][1] = v.y, f.w[b][2] = v.z, f.w[b][3] = v.w;
-    } else {
-      const int rest = G & 3;
-#pragma unroll
-      for (int j = 0; j < 3; j++) f.w[b][j] = j < rest ? __ldg(at + lane * rest + j) : 0u;
-    }
-    f.m[b] = __ldg(mults + (size_t)b * quads * 8);
-  }
+  for (int i = 0; i < 4; i++)
+    if (i < pieces) cp_async16(smem_u32(&s.w[i][lane]), at.codes + i * 128, true);
+  if (lane < 8) cp_async16(smem_u32(&s.m[4 * lane]), at.mults, true);
 }
 
-// Shared memory of a query set: fragments [groups][NT][32 lanes] uint4, scales.
+// Shared memory of a query set, for each group and eight queries: the start
+// values of the lanes' four results (int4), then their operands (uint2).
 template <int NT>
-__host__ __device__ constexpr size_t i4_frag_bytes(int groups) { return (size_t)groups * NT * 512; }
+__host__ __device__ constexpr size_t i4_frag_bytes(int groups) { return (size_t)groups * NT * 32 * 24; }
 inline size_t i4_query_bytes(int groups, int nt) { return (size_t)8 * nt * groups * (kI4Group + 4); }
 
 // Quantize the M queries of a launch (a warp each) and lay out their fragments:
 // lane 4 n + t gets query n's bytes 4t.. and 16 + 4t.. of the group, and the
 // start values of queries 2t and 2t + 1. Queries past M are zero.
 template <int NT>
-__device__ __forceinline__ void i4_queries(const float* q, int M, int dim, int groups, unsigned char* scratch, uint4* frags,
-                                           float* scales) {
+__device__ __forceinline__ void i4_queries(const float* q, int M, int dim, int groups, unsigned char* scratch, int4* starts,
+                                           uint2* ops, float* scales) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int8_t* q8 = reinterpret_cast<int8_t*>(scratch);
   int* off = reinterpret_cast<int*>(scratch + (size_t)8 * NT * groups * kI4Group);
@@ -163,10 +172,39 @@ __device__ __forceinline__ void i4_queries(const float* q, int M, int dim, int g
   for (int i = threadIdx.x; i < groups * NT * 32; i += kWarps * 32) {
     const int l = i & 31, nt = (i >> 5) % NT, g = (i >> 5) / NT, n = nt * 8 + (l >> 2), t = l & 3;
     const int8_t* at = q8 + ((size_t)n * groups + g) * kI4Group + 4 * t;
-    frags[i] = make_uint4(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + 16),
-                          (uint32_t)off[(nt * 8 + 2 * t) * groups + g], (uint32_t)off[(nt * 8 + 2 * t + 1) * groups + g]);
+    ops[i] = make_uint2(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + 16));
+    const int c0 = off[(nt * 8 + 2 * t) * groups + g], c1 = off[(nt * 8 + 2 * t + 1) * groups + g];
+    starts[i] = make_int4(c0, c1, c0, c1);
   }
   __syncthreads();
+}
+
+// DEPTH groups of a quad into the totals of 32 rows.
+template <int NT, int DEPTH>
+__device__ __forceinline__ void i4_multiply(int (&tot)[2][NT][4], const uint32_t (&w)[4][4], const uint32_t (&mult)[4],
+                                            const int4* starts, const uint2* ops) {
+#pragma unroll
+  for (int j = 0; j < DEPTH; j++) {
+    int4 c[NT];
+    uint2 b[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) c[n] = starts[(j * NT + n) * 32], b[n] = ops[(j * NT + n) * 32];
+#pragma unroll
+    for (int a = 0; a < 2; a++) {
+      const uint32_t w0 = w[2 * a][j], w1 = w[2 * a + 1][j];
+      const uint32_t op[4] = {w0 & 0x0F0F0F0Fu, w1 & 0x0F0F0F0Fu, (w0 >> 4) & 0x0F0F0F0Fu, (w1 >> 4) & 0x0F0F0F0Fu};
+      const int m0 = (int)__byte_perm(mult[2 * a], 0, 0x4440 + j), m1 = (int)__byte_perm(mult[2 * a + 1], 0, 0x4440 + j);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        int d[4];
+        mma_u8s8(d, op, b[n], c[n]);
+        tot[a][n][0] += m0 * d[0];
+        tot[a][n][1] += m0 * d[1];
+        tot[a][n][2] += m1 * d[2];
+        tot[a][n][3] += m1 * d[3];
+      }
+    }
+  }
 }
 
 struct I4ScoreArgs {
@@ -188,16 +226,43 @@ __global__ void __launch_bounds__(kWarps * 32) i4_score_kernel(I4ScoreArgs p) {
   __shared__ float s_scale[8 * NT];
   const I4Rows& r = p.r;
   const int G = r.groups, quads = (G + 3) >> 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint4* frags = reinterpret_cast<uint4*>(smem);
+  int4* starts = reinterpret_cast<int4*>(smem);
+  uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
+  I4Stage* ring = reinterpret_cast<I4Stage*>(smem + i4_frag_bytes<NT>(G)) + warp * kStages;
   if (TOPK) pdl_launch_dependents();
-  i4_queries<NT>(p.q, p.M, r.dim, G, smem + i4_frag_bytes<NT>(G), frags, s_scale);
+  i4_queries<NT>(p.q, p.M, r.dim, G, smem + i4_frag_bytes<NT>(G), starts, ops, s_scale);
+  starts += lane;
+  ops += lane;
 
+  // the copies run kStages - 1 quads ahead of the products, over the ends of tiles
   const int64_t step = (int64_t)gridDim.x * kWarps;
-  int64_t tile = (int64_t)blockIdx.x * kWarps + warp;
-  if (tile >= p.tiles) return;
-  I4Frag next;
-  i4_load(next, r, p.tile0 + tile, 0, lane);
+  int64_t tile = (int64_t)blockIdx.x * kWarps + warp, ahead = tile;
+  const int64_t next_codes = (step - 1) * G * 128 + (G & 3) * 128 + ((G & 3) ? 0 : 512), next_mults = (step - 1) * quads * 32 + 32;
+  I4Cursor cursor{r.codes + (size_t)(p.tile0 + tile) * G * 128 + lane * 4,
+                  r.mults + (size_t)(p.tile0 + tile) * quads * 32 + 4 * lane, 0};
+  int to = 0, from = 0;
+  auto fetch = [&]() {
+    if (ahead < p.tiles) i4_fetch(ring[to], cursor, G, lane);
+    cp_async_commit();
+    to = (to + 1) % kStages;
+    if (++cursor.quad == quads) {  // from a tile's last quad to the next tile's first
+      cursor.quad = 0;
+      ahead += step;
+      cursor.codes += next_codes;
+      cursor.mults += next_mults;
+    } else {
+      cursor.codes += 512;
+      cursor.mults += 32;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; i++) fetch();
   for (; tile < p.tiles; tile += step) {
+    // lane 4 r + t ends with rows r, r + 8, r + 16, r + 24 of the tile, queries 2t and 2t + 1
+    const int64_t row0 = tile * kI4Tile;
+    float scale[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) scale[b] = __ldg(r.scales + p.tile0 * kI4Tile + row0 + b * 8 + (lane >> 2));
     int tot[2][NT][4];
 #pragma unroll
     for (int a = 0; a < 2; a++)
@@ -206,59 +271,64 @@ __global__ void __launch_bounds__(kWarps * 32) i4_score_kernel(I4ScoreArgs p) {
 #pragma unroll
         for (int e = 0; e < 4; e++) tot[a][n][e] = 0;
     for (int quad = 0; quad < quads; quad++) {
-      const I4Frag f = next;
-      const bool more = quad + 1 < quads;
-      if (more || tile + step < p.tiles) i4_load(next, r, p.tile0 + (more ? tile : tile + step), more ? quad + 1 : 0, lane);
-      const int depth = min(4, G - quad * 4);
+      fetch();
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const I4Stage& s = ring[from];
+      uint32_t w[4][4], mult[4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (j >= depth) break;
+      for (int b = 0; b < 4; b++) mult[b] = s.m[b * 8 + (lane >> 2)];
+      const int4* c = starts + quad * 4 * NT * 32;
+      const uint2* b = ops + quad * 4 * NT * 32;
+      const int depth = G - quad * 4;
+      if (depth >= 4) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const uint4 b = frags[((quad * 4 + j) * NT + n) * 32 + lane];
-#pragma unroll
-          for (int a = 0; a < 2; a++) {
-            const uint32_t w0 = f.w[2 * a][j], w1 = f.w[2 * a + 1][j];
-            const uint32_t op[4] = {w0 & 0x0F0F0F0Fu, w1 & 0x0F0F0F0Fu, (w0 >> 4) & 0x0F0F0F0Fu, (w1 >> 4) & 0x0F0F0F0Fu};
-            int d[4];
-            mma_u8s8(d, op, b.x, b.y, (int)b.z, (int)b.w);
-            const int m0 = (int)((f.m[2 * a] >> (8 * j)) & 255u), m1 = (int)((f.m[2 * a + 1] >> (8 * j)) & 255u);
-            tot[a][n][0] += m0 * d[0];
-            tot[a][n][1] += m0 * d[1];
-            tot[a][n][2] += m1 * d[2];
-            tot[a][n][3] += m1 * d[3];
-          }
+        for (int i = 0; i < 4; i++) {
+          const uint4 v = s.w[i][lane];
+          w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
         }
-      }
-    }
-    // lane 4 r + t: rows r, r + 8, r + 16, r + 24 of the tile, queries 2t and 2t + 1
-    const int64_t row0 = tile * kI4Tile;
-    float scale[4];
+        __syncwarp();  // the stage may be filled again
+        i4_multiply<NT, 4>(tot, w, mult, c, b);
+      } else {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(s.w) + lane;
 #pragma unroll
-    for (int b = 0; b < 4; b++) scale[b] = __ldg(r.scales + p.tile0 * kI4Tile + row0 + b * 8 + (lane >> 2));
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int j = 0; j < 3; j++) w[i][j] = j < depth ? words[(i * depth + j) * 32] : 0u;
+        __syncwarp();
+        if (depth == 1) i4_multiply<NT, 1>(tot, w, mult, c, b);
+        else if (depth == 2) i4_multiply<NT, 2>(tot, w, mult, c, b);
+        else i4_multiply<NT, 3>(tot, w, mult, c, b);
+      }
+      from = (from + 1) % kStages;
+    }
     uint32_t alive = p.rows - row0 >= kI4Tile ? 0xFFFFFFFFu : (1u << (int)(p.rows - row0)) - 1u;
     if (TOPK && p.keep) alive &= keep_bits32(p.keep, p.keep_nbits, (uint64_t)p.id_base + (uint64_t)row0);
+    alive >>= lane >> 2;
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         const int m = n * 8 + 2 * (lane & 3) + c;
         const float qs = s_scale[m];
-        uint32_t best = 0;
+        // a NaN, and a row that is not there, loses against every score
+        float best = __uint_as_float(0x7FFFFFFFu);
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-          const float s = w8a8_score(tot[b >> 1][n][(b & 1) * 2 + c], qs, scale[b]);
-          const int i = b * 8 + (lane >> 2);
+          const int dot = tot[b >> 1][n][(b & 1) * 2 + c];
+          const bool there = (alive >> (b * 8)) & 1u;
+          float s = __fmul_rn(__fmul_rn(__int2float_rn(dot), qs), scale[b]);
+          if (qs == 0.0f) s = 0.0f;
           if (TOPK) {
-            if (((alive >> i) & 1u) && s == s) best = max(best, score_to_ord(s));
-          } else if (m < p.M && ((alive >> i) & 1u)) {
-            p.dst[(size_t)m * p.ld + row0 + i] = s;
+            best = fmaxf(best, there ? s : best);
+          } else if (m < p.M && there) {
+            p.dst[(size_t)m * p.ld + row0 + b * 8 + (lane >> 2)] = s == s ? s : w8a8_score(dot, qs, scale[b]);
           }
         }
         if (TOPK) {
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-          if (lane < 4 && m < p.M) p.best[(size_t)m * p.tiles + tile] = best;
+          for (int o = 4; o < 32; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+          if (lane < 4 && m < p.M) p.best[(size_t)m * p.tiles + tile] = best == best ? score_to_ord(best) : 0u;
         }
       }
   }
@@ -305,7 +375,7 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, y = blockIdx.y, G = r.groups;
   const uint32_t rank = cluster_rank(), nranks = cluster_size();
   int8_t* q8 = reinterpret_cast<int8_t*>(smem);             // [G * 32]
-  int* off = reinterpret_cast<int*>(q8 + G * kI4Group);     // [G]
+  int* off = reinterpret_cast<int*>(q8 + G * kI4Group);     // [G], 16-byte aligned
   // the held ranks, later the sort's keys
   uint32_t* held = reinterpret_cast<uint32_t*>(smem + ((G * (kI4Group + 4) + 15) & ~15));
   if (warp == 0) {
@@ -353,19 +423,30 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
   uint64_t* cand = p.cand + (size_t)y * p.cand_cap;
   const int quads = (G + 3) / 4;
   for (uint32_t i = rank * (kTopThreads / 32) + warp; i < need; i += nranks * (kTopThreads / 32)) {
-    const int64_t tile = __ldcg(list + i), row = tile * kI4Tile + lane, block = row / 8;
-    const uint32_t* codes = r.codes + (size_t)block * G * 32;
-    const uint32_t* mults = r.mults + (size_t)block * quads * 8 + (lane & 7);
+    const int64_t tile = __ldcg(list + i), row = tile * kI4Tile + lane;
+    const uint32_t* codes = r.codes + (size_t)tile * G * 128;
+    const uint32_t* mults = r.mults + (size_t)tile * quads * 32 + lane;
     int dot = 0;
-    for (int g = 0; g < G; g++) {
-      int acc = off[g];
+#pragma unroll 2
+    for (int quad = 0; quad < G >> 2; quad++) {
+      uint4 w[4];
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const uint32_t word = __ldg(codes + i4_word_at(g, (lane & 7) * 4 + w, G));
-        const int* qg = reinterpret_cast<const int*>(q8 + g * kI4Group);
-        acc = i4_dot_word(word, qg[w], qg[4 + w], acc);
-      }
-      dot += (int)((__ldg(mults + (g >> 2) * 8) >> (8 * (g & 3))) & 255u) * acc;
+      for (int t = 0; t < 4; t++) w[t] = __ldg(reinterpret_cast<const uint4*>(codes + i4_word_at(quad * 4, lane, t, G)));
+      const uint32_t m = __ldg(mults + quad * 32);
+      const int4* qg = reinterpret_cast<const int4*>(q8 + quad * 4 * kI4Group);
+      const int4 o = *reinterpret_cast<const int4*>(off + quad * 4);
+      dot += (int)(m & 255u) * i4_dot_group(make_uint4(w[0].x, w[1].x, w[2].x, w[3].x), qg[0], qg[1], o.x);
+      dot += (int)((m >> 8) & 255u) * i4_dot_group(make_uint4(w[0].y, w[1].y, w[2].y, w[3].y), qg[2], qg[3], o.y);
+      dot += (int)((m >> 16) & 255u) * i4_dot_group(make_uint4(w[0].z, w[1].z, w[2].z, w[3].z), qg[4], qg[5], o.z);
+      dot += (int)(m >> 24) * i4_dot_group(make_uint4(w[0].w, w[1].w, w[2].w, w[3].w), qg[6], qg[7], o.w);
+    }
+    for (int g = G & ~3; g < G; g++) {
+      uint32_t w[4];
+#pragma unroll
+      for (int t = 0; t < 4; t++) w[t] = __ldg(codes + i4_word_at(g, lane, t, G));
+      const int4* qg = reinterpret_cast<const int4*>(q8 + g * kI4Group);
+      dot += (int)((__ldg(mults + (g >> 2) * 32) >> (8 * (g & 3))) & 255u) *
+             i4_dot_group(make_uint4(w[0], w[1], w[2], w[3]), qg[0], qg[1], off[g]);
     }
     const float s = w8a8_score(dot, s_scale, __ldg(r.scales + row));
     const uint64_t id = (uint64_t)p.id_base + (uint64_t)row;
@@ -403,23 +484,37 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
   for (int i = tid; i < p.k; i += kTopThreads) p.out[(size_t)y * p.k + i] = i < have ? keys[i] : kEmptyKey;
 }
 
+// Fragments, then the queries' scratch, over which the rings lie afterwards.
+template <int NT>
+size_t score_smem(int groups) {
+  const size_t ring = sizeof(I4Stage) * kStages * kWarps, scratch = i4_query_bytes(groups, NT);
+  return i4_frag_bytes<NT>(groups) + (ring > scratch ? ring : scratch);
+}
+
 template <int NT, bool TOPK>
 cudaError_t score_launch(const I4ScoreArgs& p, int32_t sm_count, cudaStream_t stream) {
-  const size_t smem = i4_frag_bytes<NT>(p.r.groups) + i4_query_bytes(p.r.groups, NT);
-  auto fn = i4_score_kernel<NT, TOPK>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  int ctas = 0;
-  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, fn, kWarps * 32, smem);
-  if (e != cudaSuccess) return e;
-  const int64_t need = (p.tiles + kWarps - 1) / kWarps, most = (int64_t)sm_count * (ctas > 0 ? ctas : 1);
-  fn<<<(unsigned)(need < most ? need : most), kWarps * 32, smem, stream>>>(p);
+  const size_t smem = score_smem<NT>(p.r.groups);
+  const int64_t fit = (int64_t)(kSmemSm / (smem + 1024)), ctas = fit < kScoreCtas ? fit : kScoreCtas;
+  const int64_t need = (p.tiles + kWarps - 1) / kWarps, most = (int64_t)sm_count * ctas;
+  i4_score_kernel<NT, TOPK><<<(unsigned)(need < most ? need : most), kWarps * 32, smem, stream>>>(p);
   return cudaGetLastError();
 }
 
 size_t block_smem(int groups) { return (size_t)8 * groups * 16 + (size_t)8 * ((groups + 3) / 4) * 4; }
 
 }  // namespace
+
+// The limit is a property of the function on a device, so every index sets the
+// same one.
+cudaError_t i4_init() {
+  const int most = 227 * 1024 - 4096;  // the kernels' static shared memory stays below 4 KB
+  cudaError_t e = cudaFuncSetAttribute(i4_score_kernel<1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<2, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  return e;
+}
 
 cudaError_t i4_quantize_launch(const I4Rows& r, int64_t row0, const float* v, int64_t rows, cudaStream_t stream) {
   if (rows <= 0) return cudaSuccess;
@@ -446,7 +541,7 @@ cudaError_t i4_unpack_launch(const I4Rows& r, int64_t row0, int64_t rows, uint8_
 cudaError_t i4_score_launch(const I4Rows& r, int64_t row0, int64_t rows, const float* q, int32_t M, float* dst,
                             int64_t ld, int32_t sm_count, cudaStream_t stream) {
   if (rows <= 0) return cudaSuccess;
-  if (row0 % kI4Tile != 0 || M <= 0 || M > kI4MaxBatch) return cudaErrorInvalidValue;
+  if (row0 % kI4Tile != 0 || M <= 0 || M > i4_batch(r.groups)) return cudaErrorInvalidValue;
   I4ScoreArgs p{};
   p.r = r;
   p.tile0 = row0 / kI4Tile;
@@ -460,7 +555,7 @@ cudaError_t i4_score_launch(const I4Rows& r, int64_t row0, int64_t rows, const f
 }
 
 cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, cudaStream_t stream) {
-  if (p.M <= 0 || p.M > kI4MaxBatch || p.k <= 0 || p.k > kI4MaxK) return cudaErrorInvalidValue;
+  if (p.M <= 0 || p.M > i4_batch(r.groups) || p.k <= 0 || p.k > kI4MaxK) return cudaErrorInvalidValue;
   I4ScoreArgs a{};
   a.r = r;
   a.tiles = i4_tiles(r.n);
@@ -490,8 +585,6 @@ cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, c
   s.held = a.tiles <= (int64_t)kTopHeld * kTopCluster;
   const size_t smem = (((size_t)r.groups * (kI4Group + 4) + 15) & ~(size_t)15) + (size_t)kTopHeld * 4;
   static_assert(kTopHeld * 4 >= kTopSort * 8, "the sort reuses the held ranks");
-  e = cudaFuncSetAttribute(i4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kTopCluster;

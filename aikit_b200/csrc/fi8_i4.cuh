@@ -35,12 +35,16 @@ constexpr int32_t kI4MaxBatch = 16;  // queries of one pass over the rows
 constexpr int32_t kI4MaxK = 2048;
 constexpr int32_t kI4Tile = 32;      // rows that a warp scores together
 
+// Queries of one pass over rows of that many groups: their fragments and the
+// copies' rings fit in shared memory.
+inline int32_t i4_batch(int32_t groups) { return groups <= 96 ? kI4MaxBatch : kI4MaxBatch / 2; }
+
 inline int32_t i4_groups(int32_t dim) { return (dim + kI4Group - 1) / kI4Group; }
 
-// Rows on the device, n rounded up to whole tiles. A block of 8 rows has
-//   codes [groups / 4 quads][32 lanes][4 groups] words, then, when groups is no
-//         multiple of 4, [32 lanes][groups % 4] words;
-//   mults [(groups + 3) / 4][8 rows] words, a byte a group.
+// Rows on the device, n rounded up to whole tiles of 32. A tile has
+//   codes [groups / 4 quads][4 blocks of 8 rows][32 lanes][4 groups] words,
+//         then, when groups is no multiple of 4, [4][groups % 4][32] words;
+//   mults [(groups + 3) / 4 quads][32 rows] words, a byte a group.
 struct I4Rows {
   uint32_t* codes;
   uint32_t* mults;
@@ -53,6 +57,9 @@ inline int64_t i4_tiles(int64_t n) { return (n + kI4Tile - 1) / kI4Tile; }
 inline size_t i4_code_bytes(int64_t n, int32_t groups) { return (size_t)i4_tiles(n) * kI4Tile * groups * 16; }
 inline size_t i4_mult_bytes(int64_t n, int32_t groups) { return (size_t)i4_tiles(n) * kI4Tile * ((groups + 3) / 4) * 4; }
 
+// Once on each device, before the first launch on it.
+cudaError_t i4_init();
+
 // Quantize float32 rows v [rows][dim] into rows [row0, row0 + rows).
 cudaError_t i4_quantize_launch(const I4Rows& r, int64_t row0, const float* v, int64_t rows, cudaStream_t stream);
 
@@ -63,12 +70,12 @@ cudaError_t i4_pack_launch(const I4Rows& r, int64_t row0, int64_t rows, const ui
 cudaError_t i4_unpack_launch(const I4Rows& r, int64_t row0, int64_t rows, uint8_t* codes, uint8_t* mults, float* scales,
                              cudaStream_t stream);
 
-// Scores of M <= kI4MaxBatch queries q [M][dim] against rows [row0, row0 + rows),
+// Scores of M <= i4_batch(groups) queries q [M][dim] against rows [row0, row0 + rows),
 // row0 a whole tile: dst[m * ld + (row - row0)].
 cudaError_t i4_score_launch(const I4Rows& r, int64_t row0, int64_t rows, const float* q, int32_t M, float* dst,
                             int64_t ld, int32_t sm_count, cudaStream_t stream);
 
-// Top-k of M <= kI4MaxBatch queries over all rows.
+// Top-k of M <= i4_batch(groups) queries over all rows.
 struct I4TopK {
   const float* q;        // [M][dim]
   int32_t M, k;

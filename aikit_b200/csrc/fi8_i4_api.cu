@@ -98,6 +98,7 @@ int i4_alloc(fi8_ctx* ctx, int64_t n, int32_t dim, int64_t id_base, const char* 
   const size_t list = part((size_t)kI4MaxBatch * kI4MaxK * sizeof(uint32_t));
   const size_t cand = part((size_t)kI4MaxBatch * i4_cand(n) * sizeof(uint64_t));
   cudaError_t e = cudaStreamCreateWithFlags(&x->stream, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = i4_init();
   if (e == cudaSuccess) e = cudaMalloc(&x->d_base, at);
   if (e == cudaSuccess) e = cudaMemsetAsync(x->d_base, 0, rows_end, x->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(x->stream);
@@ -117,8 +118,8 @@ int i4_alloc(fi8_ctx* ctx, int64_t n, int32_t dim, int64_t id_base, const char* 
 }
 
 int launch_scores(fi8_i4* x, const float* d_q, int32_t M, float* d_dst, cudaStream_t st) {
-  for (int32_t m0 = 0; m0 < M; m0 += kI4MaxBatch) {
-    const int32_t mm = std::min(kI4MaxBatch, M - m0);
+  for (int32_t m0 = 0, most = i4_batch(x->rows.groups); m0 < M; m0 += most) {
+    const int32_t mm = std::min(most, M - m0);
     FI8_CUDA(i4_score_launch(x->rows, 0, x->rows.n, d_q + (size_t)m0 * x->rows.dim, mm,
                              d_dst + (size_t)m0 * x->rows.n, x->rows.n, x->sm_count, st),
              "i4_score_launch");
@@ -128,10 +129,10 @@ int launch_scores(fi8_i4* x, const float* d_q, int32_t M, float* d_dst, cudaStre
 
 int launch_topk(fi8_i4* x, const float* d_q, int32_t M, int32_t k, const uint64_t* d_keep, int64_t nbits,
                 uint64_t* d_keys, cudaStream_t st) {
-  for (int32_t m0 = 0; m0 < M; m0 += kI4MaxBatch) {
+  for (int32_t m0 = 0, most = i4_batch(x->rows.groups); m0 < M; m0 += most) {
     I4TopK p{};
     p.q = d_q + (size_t)m0 * x->rows.dim;
-    p.M = std::min(kI4MaxBatch, M - m0);
+    p.M = std::min(most, M - m0);
     p.k = k;
     p.id_base = x->id_base;
     p.keep = d_keep;
@@ -329,8 +330,8 @@ int fi8_i4_score_batch(fi8_i4* idx, const float* q, int32_t M, float* dst) {
   const int64_t per = std::min<int64_t>(i4_tiles(n) * kI4Tile, kHostScores / kI4MaxBatch);
   rc = ensure_device(&x->d_scores, &x->scores_cap, (size_t)(std::min(M, kI4MaxBatch) * per), "staging scores");
   if (rc != FI8_OK) return rc;
-  for (int32_t m0 = 0; m0 < M; m0 += kI4MaxBatch) {
-    const int32_t mm = std::min(kI4MaxBatch, M - m0);
+  for (int32_t m0 = 0, most = i4_batch(x->rows.groups); m0 < M; m0 += most) {
+    const int32_t mm = std::min(most, M - m0);
     for (int64_t row0 = 0; row0 < n; row0 += per) {
       const int64_t rows = std::min(per, n - row0);
       FI8_CUDA(i4_score_launch(x->rows, row0, rows, x->d_q + (size_t)m0 * x->rows.dim, mm, x->d_scores, rows,

@@ -56,7 +56,13 @@ __device__ __forceinline__ void i4_store_group(float x, int mult, float scale, u
 template <typename Load>
 __device__ __forceinline__ float i4_quantize_query(Load load, int dim, int groups, int8_t* q8, int* off, int lane) {
   float m = 0.0f;
-  for (int i = lane; i < dim; i += 32) m = absmax_step(m, load(i));
+  for (int i0 = lane; i0 < dim; i0 += 256) {  // eight loads in flight
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) v[u] = i0 + 32 * u < dim ? load(i0 + 32 * u) : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; u++) m = absmax_step(m, v[u]);
+  }
   m = warp_absmax(m);
   const float sc = m == 0.0f ? 0.0f : __fdiv_rn(m, 127.0f);
   const float inv = m == 0.0f ? 0.0f : __fdiv_rn(1.0f, sc);

@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "fi8_cluster.cuh"
+#include "fi8_cp_async.cuh"
 #include "fi8_i4q.cuh"
 #include "fi8_kb.cuh"
 #include "fi8_select.cuh"
@@ -300,15 +301,6 @@ struct AttendSmem {
   static_assert(kRing >= (size_t)kAttendWarps * 16 * (DP + 2) * 4, "the warps' partial results fit the ring");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;  // 0: the 16 bytes are zeros, src is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])

@@ -403,7 +403,7 @@ int fi8_i4_destroy(fi8_i4* idx);
 int fi8_i4_info(fi8_i4* idx, int64_t* n, int32_t* dim);
 
 /* Scores of M queries q [M*dim] against every row: dst [M*n]. Sixteen queries
- * share one pass over the rows. */
+ * (eight above 96 groups) share one pass over the rows. */
 int fi8_i4_score_batch(fi8_i4* idx, const float* q, int32_t M, float* dst);
 int fi8_i4_score_async(fi8_i4* idx, const float* d_q, int32_t M, float* d_dst, void* stream);
 
