@@ -598,7 +598,7 @@ class I4Index:
     def set_rows_async(self, row0: int, d_vecs: int, rows: int, stream: int = 0) -> None:
         """Quantize rows float32 rows at device address d_vecs into rows
         [row0, row0 + rows)."""
-        check(lib().fi8_i4_set_rows_async(self._h, row0, C.c_void_p(d_vecs), rows, C.c_void_p(stream or None)))
+        check(lib().fi8_i4_set_rows_async(self._h, row0, d_vecs, rows, stream))
 
     def read_rows(self):
         """The rows, copied to the host: codes [n, G, 16], mults [n, G], scales [n]."""
@@ -642,13 +642,13 @@ class I4Index:
 
     def score_async(self, d_q: int, M: int, d_dst: int, stream: int = 0) -> None:
         """Device-resident scores [M, n]; takes device addresses."""
-        check(lib().fi8_i4_score_async(self._h, C.c_void_p(d_q), M, C.c_void_p(d_dst), C.c_void_p(stream or None)))
+        check(lib().fi8_i4_score_async(self._h, d_q, M, d_dst, stream))
 
     def topk_async(self, d_q: int, M: int, k: int, d_keys: int, stream: int = 0, d_keep: int = 0,
                    keep_nbits: int = 0) -> None:
         """Device-resident top-k into packed keys [M, k] (unpack_keys)."""
-        check(lib().fi8_i4_topk_async(self._h, C.c_void_p(d_q), M, k, C.c_void_p(d_keep or None), keep_nbits,
-                                      C.c_void_p(d_keys), C.c_void_p(stream or None)))
+        check(lib().fi8_i4_topk_async(self._h, d_q, M, k, d_keep, keep_nbits,
+                                      d_keys, stream))
 
     def Close(self) -> None:
         if self._h:
@@ -681,31 +681,31 @@ class KeyBlocks:
 
     def update_async(self, d_slot: int, d_from: int, d_to: int, count: int, max_tokens: int, stream: int = 0) -> None:
         """Make the rows of the blocks that tokens [from, to) of each slot fill."""
-        check(lib().fi8_kb_update_async(self._h, C.c_void_p(d_slot), C.c_void_p(d_from), C.c_void_p(d_to), count,
-                                        max_tokens, C.c_void_p(stream or None)))
+        check(lib().fi8_kb_update_async(self._h, d_slot, d_from, d_to, count,
+                                        max_tokens, stream))
 
     def select_async(self, d_q: int, d_slot: int, d_len: int, rows: int, k: int, d_sel: int, first: int = 1,
                      last: int = 1, stream: int = 0, q_stride: int = 0) -> None:
         """Choose k blocks a (row, key/value head) into d_sel [rows, kv_heads, k]
         int32. q_stride: values between query rows (0: none between them)."""
-        check(lib().fi8_kb_select_async(self._h, C.c_void_p(d_q), q_stride or self._width, C.c_void_p(d_slot),
-                                        C.c_void_p(d_len), rows, k, first, last, C.c_void_p(d_sel),
-                                        C.c_void_p(stream or None)))
+        check(lib().fi8_kb_select_async(self._h, d_q, q_stride or self._width, d_slot,
+                                        d_len, rows, k, first, last, d_sel,
+                                        stream))
 
     def attend_async(self, d_q: int, d_slot: int, d_len: int, rows: int, k: int, scale: float, d_sel: int, d_out: int,
                      d_lse: int = 0, stream: int = 0, q_stride: int = 0) -> None:
         """Attention over the blocks of d_sel into d_out [rows, q_heads, head_dim]
         and, if given, d_lse [rows, q_heads] float32."""
-        check(lib().fi8_kb_attend_async(self._h, C.c_void_p(d_q), q_stride or self._width, C.c_void_p(d_slot),
-                                        C.c_void_p(d_len), rows, C.c_void_p(d_sel), k, scale, C.c_void_p(d_out),
-                                        C.c_void_p(d_lse or None), C.c_void_p(stream or None)))
+        check(lib().fi8_kb_attend_async(self._h, d_q, q_stride or self._width, d_slot,
+                                        d_len, rows, d_sel, k, scale, d_out,
+                                        d_lse, stream))
 
     def query_async(self, d_q: int, d_slot: int, d_len: int, rows: int, k: int, scale: float, d_sel: int, d_out: int,
                     d_lse: int = 0, first: int = 1, last: int = 1, stream: int = 0, q_stride: int = 0) -> None:
         """select_async, then attend_async."""
-        check(lib().fi8_kb_query_async(self._h, C.c_void_p(d_q), q_stride or self._width, C.c_void_p(d_slot),
-                                       C.c_void_p(d_len), rows, k, first, last, scale, C.c_void_p(d_sel),
-                                       C.c_void_p(d_out), C.c_void_p(d_lse or None), C.c_void_p(stream or None)))
+        check(lib().fi8_kb_query_async(self._h, d_q, q_stride or self._width, d_slot,
+                                       d_len, rows, k, first, last, scale, d_sel,
+                                       d_out, d_lse, stream))
 
     def read_rows(self, slot: int):
         """A slot's block rows, copied to the host: codes [kv_heads, blocks, G, 16],

@@ -22,7 +22,7 @@ LIBDIR = os.path.join(HERE, "lib")
 CUDA_SOURCES = ["fi8_api.cu", "fi8_scan.cu", "fi8_gemm.cu", "fi8_binary.cu", "fi8_build.cu", "fi8_i4.cu", "fi8_i4_api.cu",
                 "fi8_kb.cu", "fi8_kb_api.cu"]
 CUDA_HEADERS = ["fi8_device.cuh", "fi8_scan.cuh", "fi8_select.cuh", "fi8_gemm.cuh", "fi8_binary.cuh", "fi8_build.cuh", "fi8_stage.h",
-                "fi8_host.h", "fi8_cluster.cuh", "fi8_cp_async.cuh", "fi8_i4.cuh", "fi8_i4q.cuh", "fi8_kb.cuh"]
+                "fi8_host.h", "fi8_cluster.cuh", "fi8_kth.cuh", "fi8_cp_async.cuh", "fi8_i4.cuh", "fi8_i4q.cuh", "fi8_kb.cuh"]
 SYNTH_SOURCES = ["synth.c"]
 
 NVCC = os.environ.get("NVCC", "nvcc")

@@ -1,9 +1,12 @@
 // fi8_i4.cu -- FlatI4: scores of 4-bit rows (a matrix-vector product with
 // group scales), the row quantizer, and the exact top-k.
+#include <algorithm>
+
 #include "fi8_cluster.cuh"
 #include "fi8_cp_async.cuh"
 #include "fi8_i4.cuh"
 #include "fi8_i4q.cuh"
+#include "fi8_kth.cuh"
 
 namespace fi8 {
 
@@ -214,7 +217,8 @@ struct I4ScoreArgs {
   int M;
   float* dst;  // scores
   int64_t ld;
-  uint32_t* best;  // or the tiles' best ranks [M][tiles]
+  uint32_t* best;  // or the tiles' best ranks [M][best_ld]
+  int64_t best_ld;
   uint32_t id_base;
   const uint64_t* keep;
   int64_t keep_nbits;
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32) i4_score_kernel(I4ScoreArgs p) {
         if (TOPK) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-          if (lane < 4 && m < p.M) p.best[(size_t)m * p.tiles + tile] = best == best ? score_to_ord(best) : 0u;
+          if (lane < 4 && m < p.M) p.best[(size_t)m * p.best_ld + tile] = best == best ? score_to_ord(best) : 0u;
         }
       }
   }
@@ -342,13 +346,16 @@ __global__ void __launch_bounds__(kWarps * 32) i4_score_kernel(I4ScoreArgs p) {
 // writes one rank for 32 rows instead of 32 scores, and these k tiles are
 // scored again, row by row: k * 32 rows at most, whatever n is and however
 // many scores are equal.
-// A cluster per query: the threshold among the tiles, the list of tiles, their
-// rows' keys, and the last sort, by the CTA of rank 0.
+// The same holds for runs of tiles: the k best runs hold the k best tiles. So
+// a cluster per query reduces the tiles' ranks to runs (all its CTAs), the CTA
+// of rank 0 picks the runs and then the tiles, all CTAs score the tiles' rows,
+// and rank 0 sorts what is left. Few tiles need no runs.
 // ---------------------------------------------------------------------------
 constexpr int kTopThreads = 512;
 constexpr int kTopCluster = 8;
 constexpr int kTopSort = 4096;        // keys that a sort takes: two lists of the largest k
-constexpr int kTopHeld = 24 * 1024;   // tile ranks a CTA keeps in shared memory (more are read again in each pass)
+constexpr int kTopHeld = 48 * 1024;   // ranks that rank 0 can hold in shared memory (more are read again in each step)
+constexpr int kTopDirect = 8 * 1024;  // tiles that it picks from without runs
 
 struct I4SelectArgs {
   I4Rows r;
@@ -358,26 +365,31 @@ struct I4SelectArgs {
   uint32_t id_base;
   const uint64_t* keep;
   int64_t keep_nbits;
-  const uint32_t* best;
+  const uint32_t* best;  // [M][best_ld]
+  int64_t best_ld;
   uint32_t* list;
   uint64_t* cand;
   int64_t cand_cap;
   uint64_t* out;
-  int held;  // whether a CTA's ranks fit in shared memory
+  int run;   // tiles of a run, a power of two from 8; 0: none
+  int held;  // ranks held in shared memory
 };
 
 __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ KthShared s_kth;
   __shared__ float s_scale;
-  __shared__ uint32_t s_count;
+  __shared__ uint32_t s_count, s_floor, s_picks;
   const I4Rows& r = p.r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, y = blockIdx.y, G = r.groups;
   const uint32_t rank = cluster_rank(), nranks = cluster_size();
   int8_t* q8 = reinterpret_cast<int8_t*>(smem);             // [G * 32]
   int* off = reinterpret_cast<int*>(q8 + G * kI4Group);     // [G], 16-byte aligned
-  // the held ranks, later the sort's keys
+  // the runs' or tiles' ranks, later the sort's keys
   uint32_t* held = reinterpret_cast<uint32_t*>(smem + ((G * (kI4Group + 4) + 15) & ~15));
+  uint32_t* s_runs = held + p.held;  // [i4_picks(kI4MaxK)]
+  if (p.run) cluster_arrive();
+  __syncwarp();
   if (warp == 0) {
     const float* q = p.q + (size_t)y * r.dim;
     const float s = i4_quantize_query([&](int i) { return __ldg(q + i); }, r.dim, G, q8, off, lane);
@@ -385,70 +397,132 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
   }
   if (tid == 0) s_count = 0;
   pdl_wait_prior();  // the tiles' ranks
-  const int64_t t0 = p.tiles * rank / nranks, t1 = p.tiles * (rank + 1) / nranks;
-  const int n = (int)(t1 - t0);
-  const uint32_t* mine = p.best + (size_t)y * p.tiles + t0;
-  uint32_t some = 0;
-  for (int i = tid; i < n; i += kTopThreads) {
-    const uint32_t o = __ldcg(mine + i);
-    some += o != 0;
-    if (p.held) held[i] = o;
+  const uint32_t* best = p.best + (size_t)y * p.best_ld;
+  const int runs = p.run ? (int)((p.tiles + p.run - 1) / p.run) : 0;
+  if (p.run) {
+    // a few lanes reduce a run; the first of them writes to rank 0
+    cluster_wait();
+    const int lanes = min(8, p.run >> 2), per = p.run / (4 * lanes), sub = tid & (lanes - 1);
+    const int step = (int)nranks * (kTopThreads / lanes);
+    for (int base = (int)rank * (kTopThreads / lanes) + tid / lanes; base - tid / lanes < runs; base += 4 * step) {
+      uint32_t top[4] = {0, 0, 0, 0};
+      for (int i = 0; i < per; i++) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int run = base + u * step;
+          const int64_t at = (int64_t)run * p.run + (i * lanes + sub) * 4;
+          v[u] = run < runs && at < p.tiles ? __ldcg(reinterpret_cast<const uint4*>(best + at)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) top[u] = max(top[u], max(max(v[u].x, v[u].y), max(v[u].z, v[u].w)));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        for (int o = 1; o < lanes; o <<= 1) top[u] = max(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+        if (base + u * step < runs && sub == 0) st_cluster_u32(smem_u32(held + base + u * step), 0, top[u]);
+      }
+    }
+    cluster_sync();
   }
-  some = __reduce_add_sync(0xffffffffu, some);
-  if (lane == 0) s_kth.warp_gt[warp] = some;
-  __syncthreads();
-  if (tid == 0) {
-    uint32_t sum = 0;
-    for (int w = 0; w < kTopThreads / 32; w++) sum += s_kth.warp_gt[w];
-    s_kth.gt = sum;
-  }
-  cluster_sync();
-  uint32_t all = 0;  // tiles with a row to offer
-  for (uint32_t c = 0; c < nranks; c++) all += ld_cluster_u32(smem_u32(&s_kth.gt), c);
-  const uint32_t need = min((uint32_t)p.k, all);
-  uint32_t* list = p.list + (size_t)y * kI4MaxK;
-  uint32_t t = 0, ties = 0;
-  cluster_sync();  // s_kth.gt is written again
-  if (need > 0) {
-    auto get = [&](int i) { return p.held ? held[i] : __ldcg(mine + i); };
-    cluster_kth(get, n, need, &s_kth, nranks, &t, &ties);
-    cluster_place(get, n, t, ties, &s_kth, rank, nranks, [&](uint32_t at, int i) { list[at] = (uint32_t)(t0 + i); });
+  const uint32_t need = (uint32_t)min((int64_t)p.k, p.tiles);
+  uint32_t* list = p.list + (size_t)y * i4_picks(kI4MaxK);
+  if (rank == 0) {
+    Kth kth;
+    if (p.run) {
+      const uint32_t picks = (uint32_t)min(p.k, runs);
+      auto get_run = [&](int i) { return held[i]; };
+      kth = kth_rank(get_run, runs, picks, min((uint32_t)i4_picks((int)picks), (uint32_t)p.held / p.run), &s_kth);
+      kth_place(get_run, runs, kth, &s_kth, [&](uint32_t at, int i) { s_runs[at] = (uint32_t)i; });
+      const int n = (int)kth.count * p.run, shift = __ffs(p.run) - 1;
+      auto tile_of = [&](int i) { return (int64_t)s_runs[i >> shift] * p.run + (i & (p.run - 1)); };
+      auto rank_of = [&](int i) {
+        const int64_t tile = tile_of(i);
+        return tile < p.tiles ? __ldcg(best + tile) : 0u;
+      };
+      const bool fits = n <= p.held;
+      if (fits) {
+        for (int i0 = tid; i0 < n; i0 += 8 * kTopThreads) {  // eight loads in flight
+          uint32_t v[8];
+#pragma unroll
+          for (int u = 0; u < 8; u++) v[u] = i0 + u * kTopThreads < n ? rank_of(i0 + u * kTopThreads) : 0u;
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            if (i0 + u * kTopThreads < n) held[i0 + u * kTopThreads] = v[u];
+        }
+        __syncthreads();
+      }
+      auto get = [&](int i) { return fits ? held[i] : rank_of(i); };
+      kth = kth_rank(get, n, need, (uint32_t)i4_picks((int)need), &s_kth);
+      kth_place(get, n, kth, &s_kth, [&](uint32_t at, int i) { list[at] = (uint32_t)tile_of(i); });
+    } else {
+      const int n = (int)p.tiles;
+      for (int i0 = tid * 4; i0 < n; i0 += 4 * kTopThreads * 4) {  // four loads in flight
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          const int i = i0 + u * kTopThreads * 4;
+          v[u] = i < n ? __ldcg(reinterpret_cast<const uint4*>(best + i)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+          if (i0 + u * kTopThreads * 4 < n) *reinterpret_cast<uint4*>(held + i0 + u * kTopThreads * 4) = v[u];
+      }
+      __syncthreads();
+      auto get = [&](int i) { return held[i]; };
+      kth = kth_rank(get, n, need, (uint32_t)i4_picks((int)need), &s_kth);
+      kth_place(get, n, kth, &s_kth, [&](uint32_t at, int i) { list[at] = (uint32_t)i; });
+    }
+    if (tid == 0) {
+      s_floor = need == (uint32_t)p.k ? kth.t : 0u;  // fewer tiles than k offer every row
+      s_picks = kth.count;
+    }
   }
   cluster_sync();  // the list is complete
-  // k tiles bound the top k from below; fewer tiles offer every row they have
-  const uint32_t floor = need == (uint32_t)p.k ? t : 0u;
+  const uint32_t floor = ld_cluster_u32(smem_u32(&s_floor), 0), picks = ld_cluster_u32(smem_u32(&s_picks), 0);
 
-  // a warp per tile, a lane per row
+  // a warp per tile; lane 4 r + t has word t of rows r, r + 8, r + 16, r + 24
   const uint32_t count_at = smem_u32(&s_count);
   uint64_t* cand = p.cand + (size_t)y * p.cand_cap;
-  const int quads = (G + 3) / 4;
-  for (uint32_t i = rank * (kTopThreads / 32) + warp; i < need; i += nranks * (kTopThreads / 32)) {
-    const int64_t tile = __ldcg(list + i), row = tile * kI4Tile + lane;
-    const uint32_t* codes = r.codes + (size_t)tile * G * 128;
-    const uint32_t* mults = r.mults + (size_t)tile * quads * 32 + lane;
-    int dot = 0;
+  const int quads = (G + 3) / 4, t = lane & 3;
+  for (uint32_t i = rank * (kTopThreads / 32) + warp; i < picks; i += nranks * (kTopThreads / 32)) {
+    const int64_t tile = __ldcg(list + i), row = tile * kI4Tile + t * 8 + (lane >> 2);
+    if (tile >= p.tiles) continue;  // behind the last run's tiles, picked where nothing better was left
+    const uint32_t* codes = r.codes + (size_t)tile * G * 128 + lane * 4;
+    const uint32_t* mults = r.mults + (size_t)tile * quads * 32 + (lane >> 2);
+    const float scale = __ldg(r.scales + row);
+    int dot[4] = {0, 0, 0, 0};
+    auto group = [&](uint32_t w, uint32_t m, int g, int& dot) {
+      const int* qg = reinterpret_cast<const int*>(q8 + g * kI4Group) + t;
+      dot += (int)m * i4_dot_word(w, qg[0], qg[4], t == 0 ? off[g] : 0);
+    };
 #pragma unroll 2
     for (int quad = 0; quad < G >> 2; quad++) {
       uint4 w[4];
+      uint32_t m[4];
 #pragma unroll
-      for (int t = 0; t < 4; t++) w[t] = __ldg(reinterpret_cast<const uint4*>(codes + i4_word_at(quad * 4, lane, t, G)));
-      const uint32_t m = __ldg(mults + quad * 32);
-      const int4* qg = reinterpret_cast<const int4*>(q8 + quad * 4 * kI4Group);
-      const int4 o = *reinterpret_cast<const int4*>(off + quad * 4);
-      dot += (int)(m & 255u) * i4_dot_group(make_uint4(w[0].x, w[1].x, w[2].x, w[3].x), qg[0], qg[1], o.x);
-      dot += (int)((m >> 8) & 255u) * i4_dot_group(make_uint4(w[0].y, w[1].y, w[2].y, w[3].y), qg[2], qg[3], o.y);
-      dot += (int)((m >> 16) & 255u) * i4_dot_group(make_uint4(w[0].z, w[1].z, w[2].z, w[3].z), qg[4], qg[5], o.z);
-      dot += (int)(m >> 24) * i4_dot_group(make_uint4(w[0].w, w[1].w, w[2].w, w[3].w), qg[6], qg[7], o.w);
-    }
-    for (int g = G & ~3; g < G; g++) {
-      uint32_t w[4];
+      for (int b = 0; b < 4; b++) w[b] = __ldg(reinterpret_cast<const uint4*>(codes + quad * 512 + b * 128));
 #pragma unroll
-      for (int t = 0; t < 4; t++) w[t] = __ldg(codes + i4_word_at(g, lane, t, G));
-      const int4* qg = reinterpret_cast<const int4*>(q8 + g * kI4Group);
-      dot += (int)((__ldg(mults + (g >> 2) * 32) >> (8 * (g & 3))) & 255u) *
-             i4_dot_group(make_uint4(w[0], w[1], w[2], w[3]), qg[0], qg[1], off[g]);
+      for (int b = 0; b < 4; b++) m[b] = __ldg(mults + quad * 32 + b * 8);
+#pragma unroll
+      for (int b = 0; b < 4; b++) {
+        group(w[b].x, m[b] & 255u, quad * 4, dot[b]);
+        group(w[b].y, (m[b] >> 8) & 255u, quad * 4 + 1, dot[b]);
+        group(w[b].z, (m[b] >> 16) & 255u, quad * 4 + 2, dot[b]);
+        group(w[b].w, m[b] >> 24, quad * 4 + 3, dot[b]);
+      }
     }
-    const float s = w8a8_score(dot, s_scale, __ldg(r.scales + row));
+    for (int g = G & ~3; g < G; g++)
+#pragma unroll
+      for (int b = 0; b < 4; b++)
+        group(__ldg(codes - lane * 4 + i4_word_at(g, b * 8 + (lane >> 2), t, G)),
+              (__ldg(mults + (g >> 2) * 32 + b * 8) >> (8 * (g & 3))) & 255u, g, dot[b]);
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      dot[b] += __shfl_xor_sync(0xffffffffu, dot[b], 1);
+      dot[b] += __shfl_xor_sync(0xffffffffu, dot[b], 2);
+    }
+    const float s = w8a8_score(t == 0 ? dot[0] : t == 1 ? dot[1] : t == 2 ? dot[2] : dot[3], s_scale, scale);
     const uint64_t id = (uint64_t)p.id_base + (uint64_t)row;
     const bool ok = row < r.n && s == s && score_to_ord(s) >= floor && (!p.keep || keep_bit(p.keep, p.keep_nbits, id));
     const uint32_t mask = __ballot_sync(0xffffffffu, ok);
@@ -466,9 +540,22 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
   cluster_sync();  // the candidates are complete; no CTA reads another's shared memory after this
   if (rank != 0) return;
 
-  // sort what there is, at most kTopSort keys at a time behind the best k so far
   uint64_t* keys = reinterpret_cast<uint64_t*>(held);
+  uint64_t* out = p.out + (size_t)y * p.k;
   const int total = (int)s_count;
+  if (total <= kTopThreads) {
+    // one key a thread: its place is the number of larger keys
+    const uint64_t mine = tid < total ? __ldcg(cand + tid) : kEmptyKey;
+    keys[tid] = mine;
+    __syncthreads();
+    int place = 0;
+#pragma unroll 8
+    for (int i = 0; i < total; i++) place += keys[i] > mine;
+    if (tid < total && place < p.k) out[place] = mine;
+    for (int i = total + tid; i < p.k; i += kTopThreads) out[i] = kEmptyKey;
+    return;
+  }
+  // sort what there is, at most kTopSort keys at a time behind the best k so far
   int have = 0;
   for (int at = 0; at < total || have == 0;) {
     const int take = min(total - at, kTopSort - have);
@@ -481,7 +568,7 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
     have = min(have + take, p.k);
     if (at >= total) break;
   }
-  for (int i = tid; i < p.k; i += kTopThreads) p.out[(size_t)y * p.k + i] = i < have ? keys[i] : kEmptyKey;
+  for (int i = tid; i < p.k; i += kTopThreads) out[i] = i < have ? keys[i] : kEmptyKey;
 }
 
 // Fragments, then the queries' scratch, over which the rings lie afterwards.
@@ -507,12 +594,12 @@ size_t block_smem(int groups) { return (size_t)8 * groups * 16 + (size_t)8 * ((g
 // The limit is a property of the function on a device, so every index sets the
 // same one.
 cudaError_t i4_init() {
-  const int most = 227 * 1024 - 4096;  // the kernels' static shared memory stays below 4 KB
+  const int most = 227 * 1024 - 1024;  // beside the score kernels' static shared memory
   cudaError_t e = cudaFuncSetAttribute(i4_score_kernel<1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<2, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 12 * 1024);
   return e;
 }
 
@@ -563,6 +650,7 @@ cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, c
   a.q = p.q;
   a.M = p.M;
   a.best = p.best;
+  a.best_ld = i4_best_ld(r.n);
   a.id_base = p.id_base;
   a.keep = p.keep;
   a.keep_nbits = p.keep_nbits;
@@ -582,9 +670,15 @@ cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, c
   s.cand = p.cand;
   s.cand_cap = i4_cand(r.n);
   s.out = p.out;
-  s.held = a.tiles <= (int64_t)kTopHeld * kTopCluster;
-  const size_t smem = (((size_t)r.groups * (kI4Group + 4) + 15) & ~(size_t)15) + (size_t)kTopHeld * 4;
-  static_assert(kTopHeld * 4 >= kTopSort * 8, "the sort reuses the held ranks");
+  s.best_ld = a.best_ld;
+  // Runs of about sqrt(tiles / k) tiles: as many runs to pick from as tiles in
+  // the picked runs. Fewer and longer ones where the runs would not fit.
+  if (a.tiles > kTopDirect)
+    for (s.run = 8; a.tiles > (int64_t)s.run * s.run * 2 * p.k || a.tiles > (int64_t)s.run * kTopHeld;) s.run *= 2;
+  int64_t held = s.run ? (a.tiles + s.run - 1) / s.run : (a.tiles + 3) / 4 * 4;
+  if (s.run) held = std::max<int64_t>(held, std::min<int64_t>((int64_t)i4_picks(p.k) * s.run, kTopHeld));
+  s.held = (int)std::max<int64_t>(held, kTopSort * 2);
+  const size_t smem = (((size_t)r.groups * (kI4Group + 4) + 15) & ~(size_t)15) + ((size_t)s.held + (s.run ? i4_picks(p.k) : 0)) * 4;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kTopCluster;

@@ -82,15 +82,20 @@ struct I4TopK {
   uint32_t id_base;      // global id of row 0
   const uint64_t* keep;  // optional keep bitmap over global ids
   int64_t keep_nbits;
-  uint32_t* best;        // [kI4MaxBatch][tiles] scratch: rank of each tile's best score
-  uint32_t* list;        // [kI4MaxBatch][kI4MaxK] scratch: the tiles that can hold the top k
+  uint32_t* best;        // [kI4MaxBatch][i4_best_ld(n)] scratch, zero at rest past the tiles: rank of each tile's best score
+  uint32_t* list;        // [kI4MaxBatch][i4_picks(kI4MaxK)] scratch: tiles that hold the top k
   uint64_t* cand;        // [kI4MaxBatch][i4_cand(n)] scratch: their rows' keys
   uint64_t* out;         // [M][k] sorted keys, 0 = empty
 };
+// Ranks of a query's tiles, in whole fours.
+inline int64_t i4_best_ld(int64_t n) { return (i4_tiles(n) + 3) / 4 * 4; }
+// Tiles (or runs of tiles) that a top-k of k may look at: some more than k, so
+// that the search for their threshold ends early.
+__host__ __device__ constexpr int32_t i4_picks(int32_t k) { return k + k / 8 + 8; }
 // Keys that a query's tiles can hold.
 inline int64_t i4_cand(int64_t n) {
-  const int64_t tiles = i4_tiles(n);
-  return (tiles < kI4MaxK ? tiles : kI4MaxK) * kI4Tile;
+  const int64_t tiles = i4_tiles(n), most = i4_picks(kI4MaxK);
+  return (tiles < most ? tiles : most) * kI4Tile;
 }
 cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, cudaStream_t stream);
 

@@ -93,14 +93,14 @@ int i4_alloc(fi8_ctx* ctx, int64_t n, int32_t dim, int64_t id_base, const char* 
   };
   const size_t tiles = (size_t)i4_tiles(n);
   const size_t codes = part(i4_code_bytes(n, r.groups)), mults = part(i4_mult_bytes(n, r.groups));
-  const size_t scales = part(tiles * kI4Tile * sizeof(float)), rows_end = at;
-  const size_t best = part((size_t)kI4MaxBatch * tiles * sizeof(uint32_t));
-  const size_t list = part((size_t)kI4MaxBatch * kI4MaxK * sizeof(uint32_t));
+  const size_t scales = part(tiles * kI4Tile * sizeof(float));
+  const size_t best = part((size_t)kI4MaxBatch * i4_best_ld(n) * sizeof(uint32_t)), zero_end = at;
+  const size_t list = part((size_t)kI4MaxBatch * i4_picks(kI4MaxK) * sizeof(uint32_t));
   const size_t cand = part((size_t)kI4MaxBatch * i4_cand(n) * sizeof(uint64_t));
   cudaError_t e = cudaStreamCreateWithFlags(&x->stream, cudaStreamNonBlocking);
   if (e == cudaSuccess) e = i4_init();
   if (e == cudaSuccess) e = cudaMalloc(&x->d_base, at);
-  if (e == cudaSuccess) e = cudaMemsetAsync(x->d_base, 0, rows_end, x->stream);
+  if (e == cudaSuccess) e = cudaMemsetAsync(x->d_base, 0, zero_end, x->stream);
   if (e == cudaSuccess) e = cudaStreamSynchronize(x->stream);
   if (e != cudaSuccess) {
     const int rc = cuda_fail(e, "gpu: device allocation failed");
