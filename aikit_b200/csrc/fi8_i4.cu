@@ -14,13 +14,6 @@ namespace {
 
 constexpr int kWarps = 8;
 
-// Word index, in its tile, of word t of group g of row r (0 .. 31).
-__device__ __forceinline__ int i4_word_at(int g, int r, int t, int groups) {
-  const int full = groups & ~3, block = r >> 3, lane = (r & 7) * 4 + t;
-  return g < full ? (g >> 2) * 512 + (block * 32 + lane) * 4 + (g & 3)
-                  : full * 128 + (block * (groups & 3) + g - full) * 32 + lane;
-}
-
 // ---------------------------------------------------------------------------
 // Row quantization and the row-major format.
 // ---------------------------------------------------------------------------
@@ -71,7 +64,7 @@ __global__ void __launch_bounds__(kWarps * 32) i4_quantize_kernel(I4Rows r, int6
       const int j = g * kI4Group + lane;
       const float y = j < r.dim ? x[j] : 0.0f;
       const int mult = i4_group_mult(warp_absmax(absmax_step(0.0f, y)), up);
-      i4_store_group(y, mult, scale, codes + g * 16, lane);
+      i4_store_group(y, mult, scale, lane, [&](int t, uint32_t w) { reinterpret_cast<uint32_t*>(codes)[g * 4 + t] = w; });
       if (lane == 0) mults[g] = (uint8_t)mult;
     }
     return scale;
@@ -116,12 +109,6 @@ __global__ void __launch_bounds__(kWarps * 32) i4_unpack_kernel(I4Rows r, int64_
 // a ring of its own, kStages quads (four groups) deep, filled by asynchronous
 // copies; nothing but the warp itself waits for it.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], const uint2 b, const int4 c) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
-}
-
 constexpr int kStages = 4;
 constexpr int kScoreCtas = 2;              // CTAs an SM at most
 constexpr size_t kSmemSm = 228 * 1024;     // an SM's shared memory; a CTA takes 1 KB more than it asks for
@@ -147,67 +134,6 @@ __device__ __forceinline__ void i4_fetch(I4Stage& s, const I4Cursor& at, int G, 
   for (int i = 0; i < 4; i++)
     if (i < pieces) cp_async16(smem_u32(&s.w[i][lane]), at.codes + i * 128, true);
   if (lane < 8) cp_async16(smem_u32(&s.m[4 * lane]), at.mults, true);
-}
-
-// Shared memory of a query set, for each group and eight queries: the start
-// values of the lanes' four results (int4), then their operands (uint2).
-template <int NT>
-__host__ __device__ constexpr size_t i4_frag_bytes(int groups) { return (size_t)groups * NT * 32 * 24; }
-inline size_t i4_query_bytes(int groups, int nt) { return (size_t)8 * nt * groups * (kI4Group + 4); }
-
-// Quantize the M queries of a launch (a warp each) and lay out their fragments:
-// lane 4 n + t gets query n's bytes 4t.. and 16 + 4t.. of the group, and the
-// start values of queries 2t and 2t + 1. Queries past M are zero.
-template <int NT>
-__device__ __forceinline__ void i4_queries(const float* q, int M, int dim, int groups, unsigned char* scratch, int4* starts,
-                                           uint2* ops, float* scales) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int8_t* q8 = reinterpret_cast<int8_t*>(scratch);
-  int* off = reinterpret_cast<int*>(scratch + (size_t)8 * NT * groups * kI4Group);
-  for (int m = warp; m < 8 * NT; m += kWarps) {
-    const float* qm = q + (size_t)m * dim;
-    const int d = m < M ? dim : 0;
-    const float s = i4_quantize_query([&](int i) { return __ldg(qm + i); }, d, groups, q8 + (size_t)m * groups * kI4Group,
-                                      off + m * groups, lane);
-    if (lane == 0) scales[m] = s;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < groups * NT * 32; i += kWarps * 32) {
-    const int l = i & 31, nt = (i >> 5) % NT, g = (i >> 5) / NT, n = nt * 8 + (l >> 2), t = l & 3;
-    const int8_t* at = q8 + ((size_t)n * groups + g) * kI4Group + 4 * t;
-    ops[i] = make_uint2(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + 16));
-    const int c0 = off[(nt * 8 + 2 * t) * groups + g], c1 = off[(nt * 8 + 2 * t + 1) * groups + g];
-    starts[i] = make_int4(c0, c1, c0, c1);
-  }
-  __syncthreads();
-}
-
-// DEPTH groups of a quad into the totals of 32 rows.
-template <int NT, int DEPTH>
-__device__ __forceinline__ void i4_multiply(int (&tot)[2][NT][4], const uint32_t (&w)[4][4], const uint32_t (&mult)[4],
-                                            const int4* starts, const uint2* ops) {
-#pragma unroll
-  for (int j = 0; j < DEPTH; j++) {
-    int4 c[NT];
-    uint2 b[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) c[n] = starts[(j * NT + n) * 32], b[n] = ops[(j * NT + n) * 32];
-#pragma unroll
-    for (int a = 0; a < 2; a++) {
-      const uint32_t w0 = w[2 * a][j], w1 = w[2 * a + 1][j];
-      const uint32_t op[4] = {w0 & 0x0F0F0F0Fu, w1 & 0x0F0F0F0Fu, (w0 >> 4) & 0x0F0F0F0Fu, (w1 >> 4) & 0x0F0F0F0Fu};
-      const int m0 = (int)__byte_perm(mult[2 * a], 0, 0x4440 + j), m1 = (int)__byte_perm(mult[2 * a + 1], 0, 0x4440 + j);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        int d[4];
-        mma_u8s8(d, op, b[n], c[n]);
-        tot[a][n][0] += m0 * d[0];
-        tot[a][n][1] += m0 * d[1];
-        tot[a][n][2] += m1 * d[2];
-        tot[a][n][3] += m1 * d[3];
-      }
-    }
-  }
 }
 
 struct I4ScoreArgs {

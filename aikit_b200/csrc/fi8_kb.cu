@@ -9,6 +9,7 @@
 #include "fi8_cp_async.cuh"
 #include "fi8_i4q.cuh"
 #include "fi8_kb.cuh"
+#include "fi8_kth.cuh"
 #include "fi8_select.cuh"
 
 namespace fi8 {
@@ -54,15 +55,21 @@ struct Elem<true> {
 
 // A query row's slot and visible length; a row outside the cache is flagged
 // and sees nothing.
-__device__ __forceinline__ int kb_row(const KbParams& p, int r, int* slot) {
+__device__ __forceinline__ int kb_row_at(const KbParams& p, int r, int* slot) {
   const int s = __ldg(p.slot + r), n = __ldg(p.len + r);
   if (s < 0 || s >= p.slots || n < 0 || n > p.capacity) {
-    if (threadIdx.x == 0) atomicOr(p.err, kKbErrRow);
+    atomicOr(p.err, kKbErrRow);
     *slot = 0;
     return 0;
   }
   *slot = s;
   return n;
+}
+
+// w8a8_score where a NaN's bits do not matter.
+__device__ __forceinline__ float kb_score(int dot, float qscale, float rowscale) {
+  const float s = __fmul_rn(__fmul_rn(__int2float_rn(dot), qscale), rowscale);
+  return qscale == 0.0f ? 0.0f : s;
 }
 
 // ---------------------------------------------------------------------------
@@ -131,146 +138,313 @@ __global__ void __launch_bounds__(kUpdateThreads) kb_update_kernel(KbParams p, c
   float up;
   const float scale = i4_row_scale(rmax, &up);
   const int mult = i4_group_mult(gmax, up);
-  const int64_t row = ((int64_t)slot * p.kv_heads + h) * p.max_blocks + blk;
-  i4_store_group(x, mult, scale, p.codes + (row * p.groups + warp) * 16, lane);
+  const I4Rows r = kb_rows(p, (int64_t)slot * p.kv_heads + h);
+  const int tile = blk / kI4Tile, in_tile = blk % kI4Tile, quads = (p.groups + 3) / 4;
+  uint32_t* codes = r.codes + (size_t)tile * p.groups * 128;
+  i4_store_group(x, mult, scale, lane, [&](int t, uint32_t w) { codes[i4_word_at(warp, in_tile, t, p.groups)] = w; });
   if (lane == 0) {
-    p.mults[row * p.mpitch + warp] = (uint8_t)mult;
-    if (warp == 0) p.scales[row] = scale;
+    reinterpret_cast<uint8_t*>(r.mults + ((size_t)tile * quads + (warp >> 2)) * 32 + in_tile)[warp & 3] = (uint8_t)mult;
+    if (warp == 0) r.scales[blk] = scale;
   }
 }
 
 // ---------------------------------------------------------------------------
-// Selection: the score of every visible block (the largest of the head group's
+// Selection: the rank of every visible block (the largest of the head group's
 // FlatI4 scores), then the best by (score desc, index asc) with the first and
-// last blocks always in: a radix select over the scores' order-preserving
-// images, and a compaction in index order.
+// last blocks always in.
+// A CTA takes RT query rows and one key/value head. Their 8 NT query vectors
+// are the right operand of the score kernel's matrix product, 32 block rows
+// the left one: rows that share a slot, a prompt's chunk, read its block rows
+// once. The ranks lie in shared memory. Up to 1023 blocks are picked from registers,
+// by a warp a row or by the CTA for its one row; more by the CTA. With one row a CTA
+// and very many blocks, a cluster scores them and its rank 0 picks.
 // ---------------------------------------------------------------------------
 constexpr int kSelectThreads = 256;
-constexpr uint32_t kForced = 0xFFFFFFFFu;  // above every score's image
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kWarpPicks = 1024;  // blocks that a warp picks from
 
-// The smallest image t among the best `need` of n images, and how many of the
-// best have exactly that image. All threads of the CTA call it.
-__device__ void kb_threshold(const uint32_t* ord, int n, int need, uint32_t* hist, uint32_t* s_out, uint32_t* t,
-                             int* ties) {
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kSelectThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kSelectThreads)
-      if (shift == 24 || (ord[i] >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(hist + ((ord[i] >> shift) & 255), 1u);
-    __syncthreads();
-    if (threadIdx.x < 32) {  // lane l holds bins [255 - 8l - 7, 255 - 8l], counted from the top
-      uint32_t c[8], sum = 0;
-#pragma unroll
-      for (int i = 0; i < 8; i++) sum += c[i] = hist[255 - threadIdx.x * 8 - i];
-      uint32_t before = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
-        if ((int)threadIdx.x >= o) before += y;
-      }
-      before -= sum;
-      if (before < (uint32_t)need && before + sum >= (uint32_t)need) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          if (before < (uint32_t)need && before + c[i] >= (uint32_t)need) {
-            s_out[0] = 255 - threadIdx.x * 8 - i;
-            s_out[1] = (uint32_t)need - before;
-          }
-          before += c[i];
-        }
-      }
-    }
-    __syncthreads();
-    prefix |= s_out[0] << shift;
-    need = (int)s_out[1];
-    __syncthreads();
-  }
-  *t = prefix;
-  *ties = need;
-}
+struct KbSelectShape {
+  int rt;      // query rows of a CTA
+  int stride;  // ranks held for a row
+};
 
-template <bool F16>
-__global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ uint32_t s_hist[256];
-  __shared__ uint32_t s_out[2];
-  __shared__ int s_gt[8], s_eq[8];
-  const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int heads = p.q_heads / p.kv_heads, G = p.groups, D = p.head_dim;
-  int slot;
-  const int len = kb_row(p, r, &slot);
-  const int nb = (len + p.block - 1) / p.block;
-  int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
-  if (nb <= p.select) {  // every visible block
-    for (int i = tid; i < p.select; i += kSelectThreads) sel[i] = i < nb ? i : -1;
-    return;
+// One row's picks by a warp (WARPS = 1) or by the CTA's WARPS warps: ranks ord
+// [0 .. n) of the inner blocks, n < 32 E WARPS and n <= kWarpPicks; `need` of
+// them, behind `first` and before `last` blocks that are always in. The
+// threshold is found from the top bit down, two bits a step, from three counts
+// of at most 1023 in one word; the ranks stay in registers, and leading bits
+// that all share are skipped.
+template <int E, int WARPS>
+__device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* s_part) {
+  constexpr int kSpan = 32 * WARPS;
+  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5, tid = warp * 32 + lane;
+  for (int i = tid; i < first; i += kSpan) sel[i] = i;
+  for (int i = tid; i < last; i += kSpan) sel[first + need + i] = first + n + i;
+  if (need == 0) return;
+  // a warp's ranks are neighbours, so that its picks are
+  const int base = warp * 32 * E;
+  uint32_t v[E], top = 0, low = 0xFFFFFFFFu;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int i = base + e * 32 + lane;
+    v[e] = i < n ? ord[i] : 0u;
+    top = max(top, v[e]);
+    low = i < n ? min(low, v[e]) : low;
   }
-  int8_t* q8 = reinterpret_cast<int8_t*>(smem);
-  int* off = reinterpret_cast<int*>(q8 + (size_t)heads * G * kI4Group);
-  float* qs = reinterpret_cast<float*>(off + heads * G);
-  uint32_t* ord = reinterpret_cast<uint32_t*>(qs + heads);
-  using T = typename Elem<F16>::T;
-  for (int g = warp; g < heads; g += kSelectThreads / 32) {
-    const T* q = static_cast<const T*>(p.q) + (int64_t)r * p.q_stride + (int64_t)(h * heads + g) * D;
-    const float s = i4_quantize_query([&](int i) { return (float)q[i]; }, D, G, q8 + (size_t)g * G * kI4Group,
-                                      off + g * G, lane);
-    if (lane == 0) qs[g] = s;
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  if (WARPS > 1) {
+    if (lane == 0) s_part[2 * WARPS + warp] = top, s_part[3 * WARPS + warp] = low;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < WARPS ? s_part[2 * WARPS + lane] : 0u);
+    low = __reduce_min_sync(0xffffffffu, lane < WARPS ? s_part[3 * WARPS + lane] : 0xFFFFFFFFu);
   }
-  __syncthreads();
-  const int64_t row0 = ((int64_t)slot * p.kv_heads + h) * p.max_blocks;
-  for (int b = tid; b < nb; b += kSelectThreads) {
-    uint32_t best = 0;
-    if (b < p.first || b >= nb - p.last) {
-      best = kForced;
-    } else {
-      const uint4* codes = reinterpret_cast<const uint4*>(p.codes + (row0 + b) * G * 16);
-      const uint8_t* mults = p.mults + (row0 + b) * p.mpitch;
-      const float scale = __ldg(p.scales + row0 + b);
-      for (int g = 0; g < heads; g++) {
-        int dot = 0;
-        for (int c = 0; c < G; c++) {
-          const int4* qg = reinterpret_cast<const int4*>(q8 + ((size_t)g * G + c) * kI4Group);
-          dot += (int)__ldg(mults + c) * i4_dot_group(__ldg(codes + c), qg[0], qg[1], off[g * G + c]);
-        }
-        const float s = w8a8_score(dot, qs[g], scale);
-        if (s == s) best = max(best, score_to_ord(s));  // a NaN ranks below every score
-      }
+  int bits = 32 - __clz(top ^ low);
+  uint32_t t = bits == 32 ? 0u : top >> bits << bits, count = (uint32_t)n, above = 0;
+  for (int step = 0; bits > 0 && count > (uint32_t)need; step ^= 1) {
+    bits = max(0, bits - 2);  // an odd last bit: t + 2 and t + 3 count the ranks known to be above
+    const uint32_t t1 = t + (1u << bits), t2 = t + (2u << bits), t3 = t + (3u << bits);
+    uint32_t c = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) c += (v[e] >= t1 ? 1u : 0u) + (v[e] >= t2 ? 1u << 10 : 0u) + (v[e] >= t3 ? 1u << 20 : 0u);
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (WARPS > 1) {  // two sets of counts in turn: one barrier a step
+      if (lane == 0) s_part[step * WARPS + warp] = c;
+      __syncthreads();
+      c = __reduce_add_sync(0xffffffffu, lane < WARPS ? s_part[step * WARPS + lane] : 0u);
     }
-    ord[b] = best;
+    const uint32_t c1 = c & 1023u, c2 = (c >> 10) & 1023u, c3 = c >> 20;
+    if (c3 >= (uint32_t)need) t = t3, count = c3;
+    else if (c2 >= (uint32_t)need) t = t2, count = c2, above = c3;
+    else if (c1 >= (uint32_t)need) t = t1, count = c1, above = c2;
+    else above = c1;
   }
-  __syncthreads();
-  uint32_t t;
-  int ties;
-  kb_threshold(ord, nb, p.select, s_hist, s_out, &t, &ties);
-  // each warp compacts a segment: counts first, then places
-  const int seg = (nb + 255) / 256 * 32, b0 = min(nb, warp * seg), b1 = min(nb, b0 + seg);
-  int gt = 0, eq = 0;
-  for (int b = b0 + lane; b < b1; b += 32) {
-    gt += ord[b] > t;
-    eq += ord[b] == t;
+  // the ranks from t on; of the equal ones the first, when they are too many
+  const uint32_t ties = count == (uint32_t)need ? 0xFFFFFFFFu : (uint32_t)need - above;
+  uint32_t gt = 0, eq = 0;  // before this warp
+  if (WARPS > 1) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) c += base + e * 32 + lane < n ? (v[e] > t ? 1u : 0u) + (v[e] == t ? 1u << 16 : 0u) : 0u;
+    c = __reduce_add_sync(0xffffffffu, c);
+    __syncthreads();
+    if (lane == 0) s_part[warp] = c;
+    __syncthreads();
+    c = __reduce_add_sync(0xffffffffu, lane < warp ? s_part[lane] : 0u);
+    gt = c & 0xFFFFu, eq = c >> 16;
   }
-  gt = __reduce_add_sync(0xffffffffu, gt);
-  eq = __reduce_add_sync(0xffffffffu, eq);
-  if (lane == 0) {
-    s_gt[warp] = gt;
-    s_eq[warp] = eq;
-  }
-  __syncthreads();
-  gt = eq = 0;
-  for (int w = 0; w < warp; w++) {
-    gt += s_gt[w];
-    eq += s_eq[w];
-  }
-  for (int base = b0; base < b1; base += 32) {
-    const int b = base + lane;
-    const uint32_t o = b < b1 ? ord[b] : 0;
-    const bool is_gt = b < b1 && o > t, is_eq = b < b1 && o == t;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int i = base + e * 32 + lane;
+    const bool is_gt = i < n && v[e] > t, is_eq = i < n && v[e] == t;
     const uint32_t mgt = __ballot_sync(0xffffffffu, is_gt), meq = __ballot_sync(0xffffffffu, is_eq);
-    const int my_gt = gt + __popc(mgt & lanemask_lt()), my_eq = eq + __popc(meq & lanemask_lt());
-    if (is_gt || (is_eq && my_eq < ties)) sel[my_gt + min(my_eq, ties)] = b;
+    const uint32_t my_gt = gt + __popc(mgt & lanemask_lt()), my_eq = eq + __popc(meq & lanemask_lt());
+    if (is_gt || (is_eq && my_eq < ties)) sel[first + my_gt + min(my_eq, ties)] = first + i;
     gt += __popc(mgt);
     eq += __popc(meq);
+  }
+}
+
+// Quantize the query vectors of `columns` (row, head) pairs (LANES lanes each,
+// eight values a lane, all loads in flight together) and lay out their
+// fragments. Columns without a pair are zero.
+template <bool F16, int NT, int LANES>
+__device__ __forceinline__ void kb_queries(const KbParams& p, int row0, int columns, int heads, int h, unsigned char* scratch, int4* starts,
+                                           uint2* ops, float* scales) {
+  constexpr int kAtOnce = kSelectThreads / LANES, kRounds = (8 * NT + kAtOnce - 1) / kAtOnce;
+  const int G = p.groups, D = p.head_dim, sub = threadIdx.x % LANES;
+  int8_t* q8 = reinterpret_cast<int8_t*>(scratch);
+  int* off = reinterpret_cast<int*>(scratch + (size_t)8 * NT * G * kI4Group);
+  uint4 w[kRounds];
+#pragma unroll
+  for (int k = 0; k < kRounds; k++) {
+    const int m = k * kAtOnce + threadIdx.x / LANES;
+    w[k] = make_uint4(0, 0, 0, 0);
+    if (m < columns && sub * 8 < D) {
+      const int row = m / heads, head = m - row * heads;
+      w[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (int64_t)(row0 + row) * p.q_stride +
+                                                  (int64_t)(h * heads + head) * D) + sub);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kRounds; k++) {
+    const int m = k * kAtOnce + threadIdx.x / LANES;
+    const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+    float x[8], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = Elem<F16>::unpack(u[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      top = absmax_step(absmax_step(top, f.x), f.y);
+    }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) top = absmax_combine(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float scale = top == 0.0f ? 0.0f : __fdiv_rn(top, 127.0f), inv = top == 0.0f ? 0.0f : __fdiv_rn(1.0f, scale);
+    int sum = 0;
+    uint32_t b[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int c = top == 0.0f ? 0 : (int)quant_code(x[i], inv);
+      sum += c;
+      b[i >> 2] |= (uint32_t)(c & 255) << (8 * (i & 3));
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);  // four lanes hold a group
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if (m < 8 * NT && sub * 8 < G * kI4Group) {
+      *reinterpret_cast<uint2*>(q8 + (size_t)m * G * kI4Group + sub * 8) = make_uint2(b[0], b[1]);
+      if ((sub & 3) == 0) off[m * G + (sub >> 2)] = -8 * sum;
+      if (sub == 0) scales[m] = scale;
+    }
+  }
+  i4_fragments<NT>(G, q8, off, starts, ops);
+}
+
+template <bool F16, int NT>
+__global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, KbSelectShape shape) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ KthShared s_kth;
+  __shared__ float s_scale[8 * NT];
+  __shared__ int s_slot[32], s_len[32];
+  __shared__ uint32_t s_part[4 * kSelectWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, G = p.groups, D = p.head_dim;
+  const int heads = p.q_heads / p.kv_heads, quads = (G + 3) / 4;
+  const uint32_t rank = cluster_rank(), nranks = cluster_size();
+  const int row0 = (int)(blockIdx.x / nranks) * shape.rt, nrows = min(shape.rt, p.rows - row0);
+  int4* starts = reinterpret_cast<int4*>(smem);
+  uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
+  unsigned char* scratch = smem + i4_frag_bytes<NT>(G);
+  uint32_t* ord = reinterpret_cast<uint32_t*>(scratch + (((size_t)8 * NT * G * (kI4Group + 4) + 15) & ~(size_t)15));
+  pdl_launch_dependents();
+  if (nranks > 1) cluster_arrive();
+  if (tid < nrows) {
+    int slot;
+    s_len[tid] = kb_row_at(p, row0 + tid, &slot);
+    s_slot[tid] = slot;
+  }
+  if (D <= 128) kb_queries<F16, NT, 16>(p, row0, nrows * heads, heads, h, scratch, starts, ops, s_scale);
+  else kb_queries<F16, NT, 32>(p, row0, nrows * heads, heads, h, scratch, starts, ops, s_scale);
+  if (nranks > 1) cluster_wait();
+  auto blocks_of = [&](int r) { return (s_len[r] + p.block - 1) / p.block; };
+  if (shape.rt > 1) {  // several columns meet in one rank
+    for (int i = tid; i < nrows * shape.stride; i += kSelectThreads) ord[i] = 0;
+    __syncthreads();
+  }
+  starts += lane;
+  ops += lane;
+  // runs of rows that share a slot; rows that see no more blocks than they may take need no ranks
+  for (int r0 = 0; r0 < nrows;) {
+    const int slot = s_slot[r0];
+    int r1 = r0, most = 0;
+    for (; r1 < nrows && s_slot[r1] == slot; r1++)
+      if (blocks_of(r1) > p.select) most = max(most, blocks_of(r1));
+    const int tiles = (max(0, most - p.last) + kI4Tile - 1) / kI4Tile;
+    const I4Rows rows = kb_rows(p, (int64_t)slot * p.kv_heads + h);
+    for (int tile = (int)rank * kSelectWarps + warp; tile < tiles; tile += (int)nranks * kSelectWarps) {
+      int tot[2][NT][4];
+#pragma unroll
+      for (int a = 0; a < 2; a++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) tot[a][n][e] = 0;
+      float scale[4];
+#pragma unroll
+      for (int b = 0; b < 4; b++) scale[b] = __ldg(rows.scales + tile * kI4Tile + b * 8 + (lane >> 2));
+      const uint32_t* codes = rows.codes + (size_t)tile * G * 128;
+      const uint32_t* mults = rows.mults + (size_t)tile * quads * 32 + (lane >> 2);
+      for (int quad = 0; quad < quads; quad++) {
+        uint32_t w[4][4], mult[4];
+        const int depth = G - quad * 4;
+        const uint32_t* at = codes + quad * 512;
+#pragma unroll
+        for (int b = 0; b < 4; b++) mult[b] = __ldg(mults + quad * 32 + b * 8);
+        const int4* c = starts + quad * 4 * NT * 32;
+        const uint2* o = ops + quad * 4 * NT * 32;
+        if (depth >= 4) {
+#pragma unroll
+          for (int b = 0; b < 4; b++) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + b * 32 + lane);
+            w[b][0] = v.x, w[b][1] = v.y, w[b][2] = v.z, w[b][3] = v.w;
+          }
+          i4_multiply<NT, 4>(tot, w, mult, c, o);
+        } else {
+#pragma unroll
+          for (int b = 0; b < 4; b++)
+#pragma unroll
+            for (int j = 0; j < 3; j++) w[b][j] = j < depth ? __ldg(at + (b * depth + j) * 32 + lane) : 0u;
+          if (depth == 1) i4_multiply<NT, 1>(tot, w, mult, c, o);
+          else if (depth == 2) i4_multiply<NT, 2>(tot, w, mult, c, o);
+          else i4_multiply<NT, 3>(tot, w, mult, c, o);
+        }
+      }
+      // lane 4 r + t: blocks r, r + 8, r + 16, r + 24 of the tile, columns 2t and 2t + 1 of each eight
+      if (shape.rt == 1) {
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          float best = __uint_as_float(0x7FFFFFFFu);  // a NaN loses
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+              const int m = n * 8 + 2 * (lane & 3) + c;
+              const float s = kb_score(tot[b >> 1][n][(b & 1) * 2 + c], s_scale[m], scale[b]);
+              best = m < heads ? fmaxf(best, s) : best;
+            }
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+          const int i = tile * kI4Tile + b * 8 + (lane >> 2);
+          if ((lane & 3) == 0 && i < shape.stride) {
+            const uint32_t o = best == best ? score_to_ord(best) : 0u;
+            if (nranks > 1) st_cluster_u32(smem_u32(ord + i), 0, o);
+            else ord[i] = o;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const int m = n * 8 + 2 * (lane & 3), row = m / heads, next = (m + 1) / heads;
+#pragma unroll
+          for (int b = 0; b < 4; b++) {
+            const int i = tile * kI4Tile + b * 8 + (lane >> 2);
+            float s0 = kb_score(tot[b >> 1][n][(b & 1) * 2], s_scale[m], scale[b]);
+            const float s1 = kb_score(tot[b >> 1][n][(b & 1) * 2 + 1], s_scale[m + 1], scale[b]);
+            if (i >= shape.stride) continue;
+            if (next == row) s0 = fmaxf(s0, s1);
+            else if (next >= r0 && next < r1 && s1 == s1) atomicMax(ord + next * shape.stride + i, score_to_ord(s1));
+            if (row >= r0 && row < r1 && s0 == s0) atomicMax(ord + row * shape.stride + i, score_to_ord(s0));
+          }
+        }
+      }
+    }
+    r0 = r1;
+  }
+  if (nranks > 1) cluster_sync();
+  else __syncthreads();
+  if (rank != 0) return;
+
+  for (int r = 0; r < nrows; r++) {
+    const int nb = blocks_of(r), n = nb - p.first - p.last, need = p.select - p.first - p.last;
+    int32_t* sel = p.sel + ((int64_t)(row0 + r) * p.kv_heads + h) * p.select;
+    const uint32_t* o = ord + r * shape.stride + p.first;
+    if (nb <= p.select) {  // every visible block
+      if (r % kSelectWarps == warp)
+        for (int i = lane; i < p.select; i += 32) sel[i] = i < nb ? i : -1;
+    } else if (n <= kWarpPicks - 1) {
+      if (shape.rt == 1) {
+        kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_part);
+      } else if (r % kSelectWarps == warp) {
+        if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, nullptr);
+        else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, nullptr);
+      }
+    } else {
+      for (int i = tid; i < p.first; i += kSelectThreads) sel[i] = i;
+      for (int i = tid; i < p.last; i += kSelectThreads) sel[p.select - p.last + i] = nb - p.last + i;
+      if (need > 0) {
+        auto get = [&](int i) { return o[i]; };
+        const Kth kth = kth_rank(get, n, (uint32_t)need, (uint32_t)need, &s_kth);
+        kth_place(get, n, kth, &s_kth, [&](uint32_t at, int i) { sel[p.first + at] = p.first + i; });
+      }
+    }
   }
 }
 
@@ -343,7 +517,7 @@ __global__ void __launch_bounds__(kAttendThreads) kb_attend_kernel(KbParams p) {
   const int mrows = min(16, heads - m0);
   const int D = p.head_dim, chunks = D / 8, steps = D / 16;
   int slot;
-  const int len = kb_row(p, r, &slot);
+  const int len = kb_row_at(p, r, &slot);
   const int nb = (len + p.block - 1) / p.block;
   const int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
 
@@ -568,8 +742,6 @@ __global__ void __launch_bounds__(kAttendThreads) kb_attend_kernel(KbParams p) {
 template <int DP, bool F16>
 cudaError_t attend_launch(const KbParams& p, int32_t splits, cudaStream_t stream) {
   auto fn = kb_attend_kernel<DP, F16>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttendSmem<DP>::kBytes);
-  if (e != cudaSuccess) return e;
   const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -598,15 +770,75 @@ cudaError_t kb_update_launch(const KbParams& p, const int32_t* slot, const int32
   return cudaGetLastError();
 }
 
-cudaError_t kb_select_launch(const KbParams& p, cudaStream_t stream) {
+namespace {
+
+template <bool F16, int NT>
+cudaError_t select_launch(const KbParams& p, const KbSelectShape& shape, int cluster, size_t smem, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.rows + shape.rt - 1) / shape.rt * cluster), (unsigned)p.kv_heads);
+  cfg.blockDim = dim3(kSelectThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kb_select_kernel<F16, NT>, p, shape);
+}
+
+template <bool F16>
+cudaError_t select_nt(int nt, const KbParams& p, const KbSelectShape& shape, int cluster, size_t smem, cudaStream_t stream) {
+  switch (nt) {
+    case 1: return select_launch<F16, 1>(p, shape, cluster, smem, stream);
+    case 2: return select_launch<F16, 2>(p, shape, cluster, smem, stream);
+    case 4: return select_launch<F16, 4>(p, shape, cluster, smem, stream);
+    default: return select_launch<F16, 8>(p, shape, cluster, smem, stream);
+  }
+}
+
+}  // namespace
+
+cudaError_t kb_init() {
+  const int most = 227 * 1024 - 12 * 1024;  // beside the select kernels' static shared memory
+  const auto kind = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e = cudaSuccess;
+  auto set = [&](auto fn, int bytes) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, kind, bytes);
+  };
+  set(kb_select_kernel<false, 1>, most), set(kb_select_kernel<true, 1>, most);
+  set(kb_select_kernel<false, 2>, most), set(kb_select_kernel<true, 2>, most);
+  set(kb_select_kernel<false, 4>, most), set(kb_select_kernel<true, 4>, most);
+  set(kb_select_kernel<false, 8>, most), set(kb_select_kernel<true, 8>, most);
+  set(kb_attend_kernel<64, false>, (int)AttendSmem<64>::kBytes), set(kb_attend_kernel<64, true>, (int)AttendSmem<64>::kBytes);
+  set(kb_attend_kernel<128, false>, (int)AttendSmem<128>::kBytes), set(kb_attend_kernel<128, true>, (int)AttendSmem<128>::kBytes);
+  set(kb_attend_kernel<256, false>, (int)AttendSmem<256>::kBytes), set(kb_attend_kernel<256, true>, (int)AttendSmem<256>::kBytes);
+  return e;
+}
+
+cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream) {
   const int heads = p.q_heads / p.kv_heads;
   const int64_t blocks = (p.capacity + p.block - 1) / p.block;
-  const size_t smem = (size_t)heads * (p.groups * (kI4Group + 4) + 4) + (size_t)blocks * 4;
-  auto fn = p.f16 ? kb_select_kernel<true> : kb_select_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  fn<<<dim3((unsigned)p.rows, (unsigned)p.kv_heads), kSelectThreads, smem, stream>>>(p);
-  return cudaGetLastError();
+  KbSelectShape shape{1, (int)((blocks + 31) / 32 * 32)};
+  int nt = heads <= 8 ? 1 : heads <= 16 ? 2 : heads <= 32 ? 4 : 8, cluster = 1;
+  // Rows that can share slots (two or more a slot on average) and fill the GPU
+  // without it share a CTA: up to 32 query vectors and 96 KB of ranks.
+  if (heads <= 16 && p.rows >= 2 * p.slots && (int64_t)p.rows * p.kv_heads >= 8 * (int64_t)sm_count) {
+    const int64_t fit = 96 * 1024 / ((int64_t)shape.stride * 4);
+    const int rt = (int)(fit < 32 / heads ? fit : 32 / heads);
+    if (rt > 1) shape.rt = rt, nt = 4;
+  }
+  // Very many blocks and few rows: a cluster, while there are SMs for it and
+  // every warp has a tile.
+  if (shape.rt == 1)
+    while (cluster < 8 && (int64_t)p.rows * p.kv_heads * cluster * 2 <= 2 * (int64_t)sm_count &&
+           blocks >= (int64_t)cluster * 2 * kSelectWarps * kI4Tile)
+      cluster *= 2;
+  const size_t smem = (size_t)p.groups * nt * 32 * 24 + (((size_t)8 * nt * p.groups * (kI4Group + 4) + 15) & ~(size_t)15) +
+                      (size_t)shape.rt * shape.stride * 4;
+  return p.f16 ? select_nt<true>(nt, p, shape, cluster, smem, stream) : select_nt<false>(nt, p, shape, cluster, smem, stream);
 }
 
 cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream) {

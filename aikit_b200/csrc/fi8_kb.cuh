@@ -14,7 +14,7 @@ constexpr int32_t kKbMaxHeadDim = 256;
 constexpr int32_t kKbMaxBlock = 128;
 constexpr int32_t kKbMaxGroup = 64;       // query heads of a key/value head
 constexpr int32_t kKbMaxSelect = 1024;    // blocks a query row may read
-constexpr int32_t kKbMaxBlocks = 49152;   // blocks of a slot: their scores fit one CTA's shared memory
+constexpr int32_t kKbMaxBlocks = 36864;   // blocks of a slot: their ranks fit one CTA's shared memory
 constexpr int32_t kKbMaxRows = 65535;     // query rows of a call
 
 // Everything a launch needs. Strides in elements.
@@ -25,11 +25,11 @@ struct KbParams {
   int64_t capacity;
   int32_t slots, kv_heads, q_heads, head_dim, block, max_blocks;
   bool f16;
-  // one row a (slot, kv head, full block): [slots][kv_heads][max_blocks]
-  uint8_t* codes;
-  uint8_t* mults;
+  // FlatI4 rows, one a full block, a set of whole tiles a (slot, kv head)
+  uint32_t* codes;
+  uint32_t* mults;
   float* scales;
-  int32_t groups, mpitch;
+  int32_t groups, tiles;  // tiles of a set
   unsigned int* err;  // device error flags (kKbErrRow)
   // a call's query rows
   const void* q;
@@ -43,14 +43,26 @@ struct KbParams {
   float* lse;
 };
 
-// Bytes of a block row's multipliers: whole words.
-inline int32_t kb_mult_pitch(int32_t groups) { return (groups + 3) / 4 * 4; }
+// The rows of (slot, kv head) pair i.
+__host__ __device__ inline I4Rows kb_rows(const KbParams& p, int64_t i) {
+  I4Rows r;
+  r.codes = p.codes + i * p.tiles * p.groups * 128;
+  r.mults = p.mults + i * p.tiles * ((p.groups + 3) / 4) * 32;
+  r.scales = p.scales + i * p.tiles * kI4Tile;
+  r.n = p.max_blocks;
+  r.dim = p.head_dim;
+  r.groups = p.groups;
+  return r;
+}
 
 constexpr unsigned int kKbErrRow = 2u;  // a slot, length or range outside the cache
 
+// Once on each device, before the first launch on it.
+cudaError_t kb_init();
+
 cudaError_t kb_update_launch(const KbParams& p, const int32_t* slot, const int32_t* from, const int32_t* to,
                              int32_t count, int32_t max_tokens, cudaStream_t stream);
-cudaError_t kb_select_launch(const KbParams& p, cudaStream_t stream);
+cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream);
 cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream);
 
 }  // namespace fi8

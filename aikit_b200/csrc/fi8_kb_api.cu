@@ -15,7 +15,7 @@ struct fi8_kb {
   int device = 0, sm_count = 0;
   int32_t max_rows = 0, max_select = 0;
   KbParams p{};  // the cache and its block rows; a call fills in the rest
-  unsigned int* h_err = nullptr;
+  unsigned char* base = nullptr;
   std::mutex mu;
 };
 
@@ -23,11 +23,7 @@ namespace {
 
 void kb_free(fi8_kb* b) {
   DeviceGuard g(b->device);
-  cudaFree(b->p.codes);
-  cudaFree(b->p.mults);
-  cudaFree(b->p.scales);
-  cudaFree(b->p.err);
-  if (b->h_err) cudaFreeHost(b->h_err);
+  cudaFree(b->base);
   delete b;
 }
 
@@ -123,24 +119,27 @@ int fi8_kb_create(fi8_ctx* ctx, const fi8_kb_desc* desc, fi8_kb** out) {
   p.max_blocks = (int32_t)(d.capacity / d.block);
   p.f16 = d.dtype == FI8_F16;
   p.groups = i4_groups(d.head_dim);
-  p.mpitch = kb_mult_pitch(p.groups);
-  const size_t rows = (size_t)d.slots * d.kv_heads * p.max_blocks + 1;  // never an empty allocation
+  p.tiles = (int32_t)i4_tiles(p.max_blocks);
+  // one allocation: codes, multipliers, scales, the error word
+  const size_t sets = (size_t)d.slots * d.kv_heads;
+  const size_t codes = sets * p.tiles * p.groups * 512, mults = sets * p.tiles * ((p.groups + 3) / 4) * 128;
+  const size_t scales = sets * p.tiles * kI4Tile * sizeof(float), bytes = codes + mults + scales + 16;
   DeviceGuard g(b->device);
-  cudaError_t e = cudaMalloc(&p.codes, rows * p.groups * 16);
-  if (e == cudaSuccess) e = cudaMalloc(&p.mults, rows * p.mpitch);
-  if (e == cudaSuccess) e = cudaMalloc(&p.scales, rows * sizeof(float));
-  if (e == cudaSuccess) e = cudaMalloc(&p.err, sizeof(unsigned int));
-  if (e == cudaSuccess) e = cudaMallocHost(&b->h_err, sizeof(unsigned int));
-  if (e == cudaSuccess) e = cudaMemset(p.codes, 0, rows * p.groups * 16);
-  if (e == cudaSuccess) e = cudaMemset(p.mults, 0, rows * p.mpitch);
-  if (e == cudaSuccess) e = cudaMemset(p.scales, 0, rows * sizeof(float));
-  if (e == cudaSuccess) e = cudaMemset(p.err, 0, sizeof(unsigned int));
+  unsigned char* base = nullptr;
+  cudaError_t e = kb_init();
+  if (e == cudaSuccess) e = cudaMalloc(&base, bytes);
+  b->base = base;
+  if (e == cudaSuccess) e = cudaMemset(base, 0, bytes);
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   if (e != cudaSuccess) {
     const int rc = cuda_fail(e, "gpu: device allocation failed");
     kb_free(b);
     return rc;
   }
+  p.codes = reinterpret_cast<uint32_t*>(base);
+  p.mults = reinterpret_cast<uint32_t*>(base + codes);
+  p.scales = reinterpret_cast<float*>(base + codes + mults);
+  p.err = reinterpret_cast<unsigned int*>(base + codes + mults + scales);
   *out = b;
   return FI8_OK;
 }
@@ -178,7 +177,7 @@ int fi8_kb_select_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int
   if (rc == FI8_OK) rc = fill_select(who, first, last, &p);
   if (rc != FI8_OK) return rc;
   DeviceGuard g(kb->device);
-  FI8_CUDA(kb_select_launch(p, static_cast<cudaStream_t>(stream)), "kb_select_launch");
+  FI8_CUDA(kb_select_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_select_launch");
   return FI8_OK;
 }
 
@@ -211,7 +210,7 @@ int fi8_kb_query_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int3
   if (rc == FI8_OK) rc = fill_attend(who, scale, d_out, d_lse, &p);
   if (rc != FI8_OK) return rc;
   DeviceGuard g(kb->device);
-  FI8_CUDA(kb_select_launch(p, static_cast<cudaStream_t>(stream)), "kb_select_launch");
+  FI8_CUDA(kb_select_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_select_launch");
   FI8_CUDA(kb_attend_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
   return FI8_OK;
 }
@@ -222,14 +221,23 @@ int fi8_kb_read_rows(fi8_kb* kb, int32_t slot, uint8_t* codes, uint8_t* mults, f
   if (slot < 0 || slot >= p.slots) return fail(FI8_ERR_ARG, "fi8_kb_read_rows: slot %d of %d", slot, p.slots);
   std::lock_guard<std::mutex> lk(kb->mu);
   DeviceGuard g(kb->device);
-  const size_t rows = (size_t)p.kv_heads * p.max_blocks, at = (size_t)slot * rows;
   FI8_CUDA(cudaDeviceSynchronize(), "sync");
-  if (rows == 0) return FI8_OK;
-  FI8_CUDA(cudaMemcpy(codes, p.codes + at * p.groups * 16, rows * p.groups * 16, cudaMemcpyDeviceToHost),
-           "fi8_kb_read_rows");
-  FI8_CUDA(cudaMemcpy2D(mults, p.groups, p.mults + at * p.mpitch, p.mpitch, p.groups, rows, cudaMemcpyDeviceToHost),
-           "fi8_kb_read_rows");
-  FI8_CUDA(cudaMemcpy(scales, p.scales + at, rows * sizeof(float), cudaMemcpyDeviceToHost), "fi8_kb_read_rows");
+  const int64_t n = p.max_blocks;
+  if (n == 0) return FI8_OK;
+  const size_t cb = (size_t)p.groups * 16, mb = p.groups;
+  unsigned char* tmp = nullptr;
+  FI8_CUDA(cudaMalloc(&tmp, n * (cb + mb + 4)), "fi8_kb_read_rows");
+  cudaError_t e = cudaSuccess;
+  for (int32_t h = 0; e == cudaSuccess && h < p.kv_heads; h++) {
+    uint8_t* d_mults = tmp + n * (cb + 4);
+    float* d_scales = reinterpret_cast<float*>(tmp + n * cb);
+    e = i4_unpack_launch(kb_rows(p, (int64_t)slot * p.kv_heads + h), 0, n, tmp, d_mults, d_scales, nullptr);
+    if (e == cudaSuccess) e = cudaMemcpy(codes + h * n * cb, tmp, n * cb, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) e = cudaMemcpy(mults + h * n * mb, d_mults, n * mb, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) e = cudaMemcpy(scales + h * n, d_scales, n * 4, cudaMemcpyDeviceToHost);
+  }
+  cudaFree(tmp);
+  if (e != cudaSuccess) return cuda_fail(e, "fi8_kb_read_rows");
   return FI8_OK;
 }
 
@@ -238,8 +246,9 @@ int fi8_kb_sync(fi8_kb* kb) {
   std::lock_guard<std::mutex> lk(kb->mu);
   DeviceGuard g(kb->device);
   FI8_CUDA(cudaDeviceSynchronize(), "sync");
-  FI8_CUDA(cudaMemcpy(kb->h_err, kb->p.err, sizeof(unsigned int), cudaMemcpyDeviceToHost), "D2H err");
-  if (*kb->h_err == 0) return FI8_OK;
+  unsigned int err = 0;
+  FI8_CUDA(cudaMemcpy(&err, kb->p.err, sizeof(err), cudaMemcpyDeviceToHost), "D2H err");
+  if (err == 0) return FI8_OK;
   FI8_CUDA(cudaMemset(kb->p.err, 0, sizeof(unsigned int)), "clear err");
   return fail(FI8_ERR_DEVICE, "fi8_kb: a slot, length or token range lay outside the cache; its row saw nothing");
 }

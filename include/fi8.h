@@ -428,7 +428,7 @@ int fi8_i4_topk_async(fi8_i4* idx, const float* d_q, int32_t M, int32_t k, const
  * token_stride (in values; head_dim contiguous values follow), its value at the
  * same place of d_v. Addresses are 16-byte aligned, strides multiples of 8.
  * head_dim is a multiple of 16 up to 256, block 16, 32, 64 or 128, capacity at
- * most 49152 blocks, and a key/value head has at most 64 query heads.
+ * most 36864 blocks, and a key/value head has at most 64 query heads.
  *
  * A query row has q_heads * head_dim values of the cache's type (rows q_stride
  * values apart, 16-byte aligned), a slot, and the number len of its slot's

@@ -318,7 +318,7 @@ def test_refusals(backend):
               slot_stride=8192, head_stride=4096, token_stride=64)
     k = c.k.data_ptr()
     for change in (dict(slots=0), dict(capacity=0), dict(q_heads=3), dict(kv_heads=0), dict(head_dim=0), dict(head_dim=72),
-                   dict(head_dim=272), dict(block=48), dict(block=256), dict(capacity=49152 * 32 + 1), dict(max_rows=0),
+                   dict(head_dim=272), dict(block=48), dict(block=256), dict(capacity=36864 * 32 + 1), dict(max_rows=0),
                    dict(max_rows=65536), dict(max_select=0), dict(max_select=1025), dict(token_stride=56), dict(token_stride=68),
                    dict(head_stride=4), dict(slot_stride=-8), dict(q_heads=130)):
         with pytest.raises(Fi8Error):
