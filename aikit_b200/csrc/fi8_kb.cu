@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "fi8_cluster.cuh"
@@ -463,17 +464,21 @@ constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kPiece = 16;
 
-// Shared memory of a head dimension up to DP.
+// Shared memory of a head dimension up to DP: the warps' rings (each holds, at
+// the end, its warp's result; the CTA's joined result, 16 x DP f32, replaces the
+// first), the query tile, maxima and sums, the chosen blocks. Three CTAs an SM
+// up to 128.
 template <int DP>
 struct AttendSmem {
-  static constexpr int kStages = DP == 64 ? 4 : DP == 128 ? 3 : 2;
-  static constexpr size_t kStage = (size_t)2 * kPiece * DP * 2;  // a warp's stage: 16 keys, then 16 values
-  static constexpr size_t kRing = kAttendWarps * kStages * kStage;
-  // after the ring: the query tile, then the joined result (16 x DP f32) and its maxima and sums
-  static constexpr size_t kBytes = kRing + 16 * DP * 2 + 16 * DP * 4 + 2 * 16 * 4;
-  static_assert(kBytes <= 227 * 1024, "shared memory");
-  static_assert(kRing >= (size_t)kAttendWarps * 16 * (DP + 2) * 4, "the warps' partial results fit the ring");
+  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr uint32_t kStage = 2 * kPiece * DP * 2;  // 16 keys, then 16 values
+  static constexpr uint32_t kRing = kStages * kStage;      // of a warp
+  static constexpr uint32_t kQuery = kAttendWarps * kRing, kStats = kQuery + 16 * DP * 2;
+  static_assert(kRing >= 16 * DP * 4, "a warp's result fits its ring");
+  static constexpr uint32_t kSel = kStats + 2 * 16 * 4 + 2 * kAttendWarps * 16 * 4;
+  static size_t bytes(int select) { return kSel + (size_t)select * 4; }
 };
+static_assert(AttendSmem<256>::kSel + kKbMaxSelect * 4 <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -492,6 +497,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
 // Byte offset of 16-byte chunk c of row r in a tile of DP-element rows; the
 // chunk index is permuted by the row so that eight rows' equal chunks fall
 // into different banks.
@@ -500,262 +513,337 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return (uint32_t)(r * (DP * 2) + ((c ^ (r & 7)) << 4));
 }
 
-template <int DP, bool F16>
-__global__ void __launch_bounds__(kAttendThreads) kb_attend_kernel(KbParams p) {
+// The running state of 16 query rows over the tokens of a warp (log2 domain):
+// lane 4 r + t holds rows r and r + 8.
+template <int DP>
+struct AttendState {
+  float o[DP / 8][4];
+  float mx[2], sum[2];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    mx[0] = mx[1] = -INFINITY;
+    sum[0] = sum[1] = 0.0f;
+  }
+};
+
+// 16 tokens (keys at shared address kt, values at vt, `n` of them visible) into
+// the state. c2 >= 0 is the softmax scale times log2(e). koff and voff are the
+// lane's ldmatrix offsets: a step of 16 channels flips bits above them.
+template <int DP, bool F16, bool kQInRegs, bool FULL>
+__device__ __forceinline__ void attend_piece(AttendState<DP>& st, const uint32_t (&qf)[kQInRegs ? DP / 16 : 1][4], uint32_t qt,
+                                             uint32_t kt, uint32_t vt, uint32_t qoff, uint32_t koff, int n, float c2, int steps) {
+  using E = Elem<F16>;
+  const int lane = threadIdx.x & 31;
+  float sc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+  for (int t = 0; t < DP / 16; t++) {
+    if (!FULL && t >= steps) break;
+    uint32_t kf[4];
+    ldmatrix4(kf, kt + (koff ^ (t * 32)));
+    if (kQInRegs) {
+      E::mma(sc[0], qf[kQInRegs ? t : 0], kf[0], kf[1]);
+      E::mma(sc[1], qf[kQInRegs ? t : 0], kf[2], kf[3]);
+    } else {
+      uint32_t a[4];
+      ldmatrix4(a, qt + (qoff ^ (t * 32)));
+      E::mma(sc[0], a, kf[0], kf[1]);
+      E::mma(sc[1], a, kf[2], kf[3]);
+    }
+  }
+  if (n < kPiece) {
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (j * 8 + (lane & 3) * 2 + (e & 1) >= n) sc[j][e] = -INFINITY;
+  }
+  // the rows' maxima: the four lanes that share a row
+  float pm[2];
+#pragma unroll
+  for (int e = 0; e < 2; e++) {
+    pm[e] = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
+    pm[e] = fmaxf(pm[e], __shfl_xor_sync(0xffffffffu, pm[e], 1));
+    pm[e] = fmaxf(pm[e], __shfl_xor_sync(0xffffffffu, pm[e], 2));
+    // scaled after the maximum; a scale of 0 must not meet -inf
+    pm[e] = fmaxf(st.mx[e], pm[e] == -INFINITY ? -INFINITY : pm[e] * c2);
+  }
+  if (__any_sync(0xffffffffu, pm[0] != st.mx[0] || pm[1] != st.mx[1])) {
+    const float f0 = pm[0] == st.mx[0] ? 1.0f : exp2_fast(st.mx[0] - pm[0]);
+    const float f1 = pm[1] == st.mx[1] ? 1.0f : exp2_fast(st.mx[1] - pm[1]);
+#pragma unroll
+    for (int t = 0; t < DP / 8; t++) {
+      st.o[t][0] *= f0, st.o[t][1] *= f0;
+      st.o[t][2] *= f1, st.o[t][3] *= f1;
+    }
+    st.sum[0] *= f0, st.sum[1] *= f1;
+    st.mx[0] = pm[0], st.mx[1] = pm[1];
+  }
+  // a row that has seen nothing but -inf keeps weights of 0
+  const float base0 = st.mx[0] == -INFINITY ? 0.0f : -st.mx[0], base1 = st.mx[1] == -INFINITY ? 0.0f : -st.mx[1];
+  uint32_t pf[4];
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      w[e] = exp2_fast(fmaf(sc[j][e], c2, e < 2 ? base0 : base1));
+      if (n < kPiece && sc[j][e] == -INFINITY) w[e] = 0.0f;  // -inf times a scale of 0
+    }
+    st.sum[0] += w[0] + w[1];
+    st.sum[1] += w[2] + w[3];
+    // the weights enter the product in the cache's type (a relative 2^-9 or 2^-12 each; the sums stay 32 bits)
+    pf[2 * j] = E::pack(w[0], w[1]);
+    pf[2 * j + 1] = E::pack(w[2], w[3]);
+  }
+#pragma unroll
+  for (int t = 0; t < DP / 16; t++) {
+    if (!FULL && t >= steps) break;
+    uint32_t vf[4];
+    ldmatrix4_trans(vf, vt + (qoff ^ (t * 32)));
+    E::mma(st.o[2 * t], pf, vf[0], vf[1]);
+    E::mma(st.o[2 * t + 1], pf, vf[2], vf[3]);
+  }
+}
+
+// Two packed values of the query tile, negated when the scale is negative (the
+// rest then works with its absolute value).
+__device__ __forceinline__ uint4 flip_sign(uint4 w, bool flip) {
+  const uint32_t f = flip ? 0x80008000u : 0u;
+  return make_uint4(w.x ^ f, w.y ^ f, w.z ^ f, w.w ^ f);
+}
+
+// FULL: head_dim is DP itself.
+template <int DP, bool F16, bool FULL>
+__global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_kernel(KbParams p) {
   using E = Elem<F16>;
   using T = typename E::T;
-  constexpr int NS = AttendSmem<DP>::kStages;
-  constexpr int kChunks = DP / 8;       // 16-byte chunks of a padded row
-  constexpr int kSteps = DP / 16;
-  constexpr bool kQInRegs = DP <= 128;  // else the query fragments are read again for each piece
-  extern __shared__ __align__(128) unsigned char smem[];
+  using S = AttendSmem<DP>;
+  constexpr int NS = S::kStages;
+  constexpr int kChunks = DP / 8;             // 16-byte chunks of a padded row
+  constexpr int kRowStep = 32 / kChunks;      // rows that a warp copies at once
+  constexpr bool kQInRegs = DP <= 128;        // else the query fragments are read again for each piece
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), nsplit = cluster_size();
   const int r = blockIdx.x / nsplit;
   const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
   const int h = blockIdx.y / mtiles, m0 = (blockIdx.y % mtiles) * 16;
   const int mrows = min(16, heads - m0);
-  const int D = p.head_dim, chunks = D / 8, steps = D / 16;
-  int slot;
-  const int len = kb_row_at(p, r, &slot);
-  const int nb = (len + p.block - 1) / p.block;
-  const int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
-
-  unsigned char* s_q = smem + AttendSmem<DP>::kRing;
-  float* s_o = reinterpret_cast<float*>(s_q + 16 * DP * 2);
-  float* s_m = s_o + 16 * DP;
-  float* s_l = s_m + 16;
+  const int D = FULL ? DP : p.head_dim, chunks = D / 8, steps = D / 16;
+  const uint32_t base = smem_u32(smem);
+  float* s_o = reinterpret_cast<float*>(smem);  // each value replaces the first warp's, which the same thread has read
+  float* s_m = reinterpret_cast<float*>(smem + S::kStats);  // [16], then the sums [16]
+  float* w_m = s_m + 32;                                    // the warps' [warps][16], then their sums
+  float* w_l = w_m + kAttendWarps * 16;
+  int* s_sel = reinterpret_cast<int*>(smem + S::kSel);
 
   // the query tile: absent heads are zero rows
   const T* q = static_cast<const T*>(p.q) + (int64_t)r * p.q_stride + (int64_t)(h * heads + m0) * D;
-  for (int i = tid; i < 16 * kChunks; i += kAttendThreads) {
-    const int row = i / kChunks, c = i % kChunks;
+#pragma unroll
+  for (int i0 = 0; i0 < 16 * kChunks; i0 += kAttendThreads) {
+    const int i = i0 + tid, row = i / kChunks, c = i % kChunks;
     uint4 w = make_uint4(0, 0, 0, 0);
-    if (row < mrows && c < chunks) w = __ldg(reinterpret_cast<const uint4*>(q + (int64_t)row * D) + c);
-    *reinterpret_cast<uint4*>(s_q + tile_at<DP>(row, c)) = w;
+    if (row < mrows && c < chunks) w = flip_sign(__ldg(reinterpret_cast<const uint4*>(q + (int64_t)row * D) + c), p.scale < 0.0f);
+    *reinterpret_cast<uint4*>(smem + S::kQuery + tile_at<DP>(row, c)) = w;
   }
+  int slot;
+  const int len = kb_row_at(p, r, &slot);
+  const int nb = (len + p.block - 1) / p.block;
+  pdl_wait_prior();  // the chosen blocks may come from the kernel before
+  const int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
+  for (int i = tid; i < p.select; i += kAttendThreads) s_sel[i] = __ldcg(sel + i);
   __syncthreads();
-  const uint32_t q_base = smem_u32(s_q);
-  // ldmatrix lane addresses: rows 0-7 / 8-15 by lane bit 3, chunk +1 by bit 4
-  const int a_row = (lane & 7) + (lane & 8), a_chunk = lane >> 4;
-  // keys: rows by lane bit 4, chunk by bit 3
-  const int b_row = (lane & 7) + ((lane & 16) >> 1), b_chunk = (lane >> 3) & 1;
-  uint32_t qf[kQInRegs ? kSteps : 1][4];
+  // ldmatrix lane addresses. Query and values: rows 0-7 / 8-15 by lane bit 3, chunk + 1 by bit 4; keys: the other way round
+  const uint32_t qoff = tile_at<DP>(lane & 15, lane >> 4), koff = tile_at<DP>((lane & 7) + ((lane & 16) >> 1), (lane >> 3) & 1);
+  uint32_t qf[kQInRegs ? DP / 16 : 1][4];
   if (kQInRegs) {
 #pragma unroll
-    for (int s = 0; s < kSteps; s++)
-      if (s < steps) ldmatrix4(qf[s], q_base + tile_at<DP>(a_row, 2 * s + a_chunk));
+    for (int s = 0; s < DP / 16; s++)
+      if (FULL || s < steps) ldmatrix4(qf[kQInRegs ? s : 0], base + S::kQuery + (qoff ^ (s * 32)));
   }
 
-  const int per_block = p.block / kPiece, pieces = p.select * per_block;
+  const int shift = __ffs(p.block / kPiece) - 1, pieces = p.select << shift;
   const int stride = (int)nsplit * kAttendWarps;
-  const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + (int64_t)slot * p.slot_stride +
-                                                    (int64_t)h * p.head_stride);
-  const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + (int64_t)slot * p.slot_stride +
-                                                    (int64_t)h * p.head_stride);
   const int64_t pitch = p.token_stride * 2;
-  const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * NS * AttendSmem<DP>::kStage);
+  const int lane_row = lane / kChunks, lane_chunk = lane % kChunks;
+  const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + (int64_t)slot * p.slot_stride +
+                                                    (int64_t)h * p.head_stride) + lane_row * pitch + lane_chunk * 16;
+  const int64_t to_values = static_cast<const char*>(p.v) - static_cast<const char*>(p.k);
+  const uint32_t ring = base + warp * S::kRing;
+  const bool copies = FULL || lane_chunk < chunks;
+  const uint32_t to0 = tile_at<DP>(lane_row, lane_chunk);  // of a row further on by a multiple of kRowStep: chunk bits flipped
+  const int64_t row_step = kRowStep * pitch;
 
-  // tokens of piece i that the row sees (0: the piece is skipped), from token *t0
-  auto visible = [&](int i, int* t0) {
-    if (i >= pieces) return 0;
-    const int b = __ldg(sel + i / per_block);
-    if (b < 0 || b >= nb) return 0;
-    *t0 = b * p.block + (i % per_block) * kPiece;
-    return max(0, min(kPiece, len - *t0));
-  };
-  auto load = [&](int i, int stage) {
-    int t0 = 0;
-    const int n = visible(i, &t0);
-    if (n > 0) {
-      const uint32_t dst = ring + (uint32_t)(stage * AttendSmem<DP>::kStage);
-      for (int j = lane; j < kPiece * kChunks; j += 32) {
-        const int row = j / kChunks, c = j % kChunks;
-        if (c >= chunks) continue;
-        const bool ok = row < n;  // hidden tokens are zeros: 0 * their weight 0 stays 0
-        const int64_t at = (int64_t)(t0 + (ok ? row : 0)) * pitch + c * 16;
-        cp_async16(dst + tile_at<DP>(row, c), kbase + at, ok);
-        cp_async16(dst + kPiece * DP * 2 + tile_at<DP>(row, c), vbase + at, ok);
+  // starts the copies of piece i; the tokens of it that the row sees (0: skipped)
+  auto load = [&](int i, uint32_t dst) {
+    int n = 0;
+    const int b = i < pieces ? s_sel[i >> shift] : -1;
+    if (b >= 0 && b < nb) {
+      const int t0 = b * p.block + (i & ((1 << shift) - 1)) * kPiece;
+      n = max(0, min(kPiece, len - t0));
+      const char* from = kbase + t0 * pitch;
+      if (n == kPiece) {
+        if (copies)
+#pragma unroll
+          for (int row = 0; row < kPiece; row += kRowStep) {
+            const uint32_t at = dst + (to0 ^ ((row & 7) << 4)) + row * (DP * 2);
+            cp_async16(at, from, true);
+            cp_async16(at + kPiece * DP * 2, from + to_values, true);
+            from += row_step;
+          }
+      } else if (n > 0 && copies) {
+        for (int row = 0; row < kPiece; row += kRowStep) {
+          // hidden tokens are zeros: 0 * their weight 0 stays 0
+          const bool ok = row + lane_row < n;
+          const uint32_t at = dst + (to0 ^ ((row & 7) << 4)) + row * (DP * 2);
+          cp_async16(at, ok ? from : kbase, ok);
+          cp_async16(at + kPiece * DP * 2, (ok ? from : kbase) + to_values, ok);
+          from += row_step;
+        }
       }
     }
     cp_async_commit();
     return n;
   };
 
-  float o[kSteps * 2][4];
-#pragma unroll
-  for (int i = 0; i < kSteps * 2; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-  const float c2 = p.scale * 1.4426950408889634f;  // log2(e)
-
+  AttendState<DP> st;
+  st.clear();
+  const float c2 = fabsf(p.scale) * 1.4426950408889634f;  // log2(e)
   int i = (int)rank * kAttendWarps + warp;
   int have[NS];
 #pragma unroll
-  for (int s = 0; s < NS; s++) have[s] = 0;
-#pragma unroll
-  for (int s = 0; s < NS - 1; s++) have[s] = load(i + s * stride, s);
+  for (int s = 0; s < NS - 1; s++) have[s] = load(i + s * stride, ring + s * S::kStage);
   for (; i < pieces; i += NS * stride) {
 #pragma unroll
     for (int s = 0; s < NS; s++) {
       const int at = i + s * stride;
       if (at >= pieces) break;
-      have[(s + NS - 1) % NS] = load(at + (NS - 1) * stride, (s + NS - 1) % NS);
+      have[(s + NS - 1) % NS] = load(at + (NS - 1) * stride, ring + (s + NS - 1) % NS * S::kStage);
       cp_async_wait<NS - 1>();
       __syncwarp();
-      const int n = have[s];
-      if (n > 0) {
-        const uint32_t kt = ring + (uint32_t)(s * AttendSmem<DP>::kStage), vt = kt + kPiece * DP * 2;
-        float sc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-        for (int t = 0; t < kSteps; t++) {
-          if (t >= steps) break;
-          uint32_t kf[4];
-          ldmatrix4(kf, kt + tile_at<DP>(b_row, 2 * t + b_chunk));
-          if (kQInRegs) {
-            E::mma(sc[0], qf[kQInRegs ? t : 0], kf[0], kf[1]);
-            E::mma(sc[1], qf[kQInRegs ? t : 0], kf[2], kf[3]);
-          } else {
-            uint32_t a[4];
-            ldmatrix4(a, q_base + tile_at<DP>(a_row, 2 * t + a_chunk));
-            E::mma(sc[0], a, kf[0], kf[1]);
-            E::mma(sc[1], a, kf[2], kf[3]);
-          }
-        }
-        // hidden tokens out, then the maximum of the four lanes that share a row
-        float pm[2] = {mx[0], mx[1]};
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int token = j * 8 + (lane & 3) * 2 + (e & 1);
-            sc[j][e] = token < n ? sc[j][e] * c2 : -INFINITY;
-            pm[e >> 1] = fmaxf(pm[e >> 1], sc[j][e]);
-          }
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          pm[e] = fmaxf(pm[e], __shfl_xor_sync(0xffffffffu, pm[e], 1));
-          pm[e] = fmaxf(pm[e], __shfl_xor_sync(0xffffffffu, pm[e], 2));
-        }
-        if (__any_sync(0xffffffffu, pm[0] != mx[0] || pm[1] != mx[1])) {
-          const float f0 = pm[0] == mx[0] ? 1.0f : exp2_fast(mx[0] - pm[0]);
-          const float f1 = pm[1] == mx[1] ? 1.0f : exp2_fast(mx[1] - pm[1]);
-#pragma unroll
-          for (int t = 0; t < kSteps * 2; t++) {
-            o[t][0] *= f0, o[t][1] *= f0;
-            o[t][2] *= f1, o[t][3] *= f1;
-          }
-          sum[0] *= f0, sum[1] *= f1;
-          mx[0] = pm[0], mx[1] = pm[1];
-        }
-        // a row that has seen nothing but -inf keeps weights of 0
-        const float base0 = mx[0] == -INFINITY ? 0.0f : mx[0], base1 = mx[1] == -INFINITY ? 0.0f : mx[1];
-        uint32_t pf[4];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const float p0 = exp2_fast(sc[j][0] - base0), p1 = exp2_fast(sc[j][1] - base0);
-          const float p2 = exp2_fast(sc[j][2] - base1), p3 = exp2_fast(sc[j][3] - base1);
-          sum[0] += p0 + p1;
-          sum[1] += p2 + p3;
-          // the weights enter the product in the cache's type (a relative 2^-9 or 2^-12 each; the sums stay 32 bits)
-          pf[2 * j] = E::pack(p0, p1);
-          pf[2 * j + 1] = E::pack(p2, p3);
-        }
-#pragma unroll
-        for (int t = 0; t < kSteps; t++) {
-          if (t >= steps) break;
-          uint32_t vf[4];
-          ldmatrix4_trans(vf, vt + tile_at<DP>(a_row, 2 * t + a_chunk));
-          E::mma(o[2 * t], pf, vf[0], vf[1]);
-          E::mma(o[2 * t + 1], pf, vf[2], vf[3]);
-        }
-      }
+      const uint32_t kt = ring + s * S::kStage;
+      if (have[s] > 0)
+        attend_piece<DP, F16, kQInRegs, FULL>(st, qf, base + S::kQuery, kt, kt + kPiece * DP * 2, qoff, koff, have[s], c2, steps);
       __syncwarp();  // the stage may be filled again
     }
   }
   cp_async_wait<0>();
 #pragma unroll
   for (int e = 0; e < 2; e++) {
-    sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
-    sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+    st.sum[e] += __shfl_xor_sync(0xffffffffu, st.sum[e], 1);
+    st.sum[e] += __shfl_xor_sync(0xffffffffu, st.sum[e], 2);
   }
-  __syncthreads();  // every warp is done with the ring: it holds the warps' partial results now
-
-  float* w_o = reinterpret_cast<float*>(smem);             // [warps][16][DP]
-  float* w_m = w_o + (size_t)kAttendWarps * 16 * DP;       // [warps][16]
-  float* w_l = w_m + kAttendWarps * 16;
-  {
+  __syncwarp();
+  {  // the warp's result over its own ring
     const int row = lane >> 2, col = (lane & 3) * 2;
-    float* mine = w_o + (size_t)warp * 16 * DP;
+    float* mine = reinterpret_cast<float*>(smem + warp * S::kRing);
 #pragma unroll
-    for (int t = 0; t < kSteps * 2; t++) {
+    for (int t = 0; t < DP / 8; t++) {
       if (t * 8 >= D) break;
-      *reinterpret_cast<float2*>(mine + row * DP + t * 8 + col) = make_float2(o[t][0], o[t][1]);
-      *reinterpret_cast<float2*>(mine + (row + 8) * DP + t * 8 + col) = make_float2(o[t][2], o[t][3]);
+      if (row < mrows) *reinterpret_cast<float2*>(mine + row * DP + t * 8 + col) = make_float2(st.o[t][0], st.o[t][1]);
+      if (row + 8 < mrows) *reinterpret_cast<float2*>(mine + (row + 8) * DP + t * 8 + col) = make_float2(st.o[t][2], st.o[t][3]);
     }
     if ((lane & 3) == 0) {
-      w_m[warp * 16 + row] = mx[0], w_m[warp * 16 + row + 8] = mx[1];
-      w_l[warp * 16 + row] = sum[0], w_l[warp * 16 + row + 8] = sum[1];
+      w_m[warp * 16 + row] = st.mx[0], w_m[warp * 16 + row + 8] = st.mx[1];
+      w_l[warp * 16 + row] = st.sum[0], w_l[warp * 16 + row + 8] = st.sum[1];
     }
   }
   __syncthreads();
-  for (int j = tid; j < mrows * D; j += kAttendThreads) {
-    const int row = j / D, d = j % D;
+  T* out = static_cast<T*>(p.out) + ((int64_t)r * p.q_heads + h * heads + m0) * D;
+  float* lse = p.lse ? p.lse + (int64_t)r * p.q_heads + h * heads + m0 : nullptr;
+  // four channels of a row, of the whole softmax
+  auto finish = [&](int row, int d, float4 acc, float m, float l) {
+    const bool some = l > 0.0f || l != l;
+    const float f = some ? 1.0f / l : 0.0f;
+    *reinterpret_cast<uint2*>(out + (int64_t)row * D + d) = make_uint2(E::pack(acc.x * f, acc.y * f), E::pack(acc.z * f, acc.w * f));
+    if (lse && d == 0) lse[row] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  };
+  for (int j = tid; j < mrows * (DP / 4); j += kAttendThreads) {
+    const int row = j / (DP / 4), d = j % (DP / 4) * 4;
+    if (d >= D) continue;
     float m = w_m[row];
 #pragma unroll
     for (int w = 1; w < kAttendWarps; w++) m = fmaxf(m, w_m[w * 16 + row]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float acc = 0.0f, l = 0.0f;
+    const float zero = m == -INFINITY ? 0.0f : m;
+    float4 acc = make_float4(0, 0, 0, 0);
+    float l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kAttendWarps; w++) {
-      const float f = exp2_fast(w_m[w * 16 + row] - base);
-      acc += f * w_o[((size_t)w * 16 + row) * DP + d];
+      const float f = exp2_fast(w_m[w * 16 + row] - zero);
+      const float4 v = *reinterpret_cast<const float4*>(smem + w * S::kRing + (row * DP + d) * 4);
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
       l += f * w_l[w * 16 + row];
     }
-    s_o[row * DP + d] = acc;
-    if (d == 0) {
-      s_m[row] = m;
-      s_l[row] = l;
+    if (nsplit == 1) {
+      finish(row, d, acc, m, l);
+    } else {
+      *reinterpret_cast<float4*>(s_o + row * DP + d) = acc;
+      if (d == 0) s_m[row] = m, s_m[16 + row] = l;
     }
   }
-  __syncthreads();
-  if (nsplit > 1) cluster_sync();
-  // the cluster's CTAs share out the joined tile
-  T* out = static_cast<T*>(p.out) + ((int64_t)r * p.q_heads + h * heads + m0) * D;
-  float* lse = p.lse ? p.lse + (int64_t)r * p.q_heads + h * heads + m0 : nullptr;
-  const uint32_t o_at = smem_u32(s_o), m_at = smem_u32(s_m), l_at = smem_u32(s_l);
-  for (int j = (int)rank * kAttendThreads + tid; j < mrows * D; j += (int)nsplit * kAttendThreads) {
-    const int row = j / D, d = j % D;
-    float m = -INFINITY, acc = 0.0f, l = 0.0f;
-    for (uint32_t c = 0; c < nsplit; c++) m = fmaxf(m, ld_cluster(m_at + row * 4, c));
-    const float base = m == -INFINITY ? 0.0f : m;
+  if (nsplit == 1) return;
+  cluster_sync();
+  // the cluster's CTAs share out the channels of the joined tile
+  for (int j = tid * (int)nsplit + (int)rank; j < mrows * (DP / 4); j += kAttendThreads * (int)nsplit) {
+    const int row = j / (DP / 4), d = j % (DP / 4) * 4;
+    if (d >= D) continue;
+    const uint32_t at = base + S::kStats + row * 4;
+    float m = -INFINITY;
+    for (uint32_t c = 0; c < nsplit; c++) m = fmaxf(m, ld_cluster(at, c));
+    const float zero = m == -INFINITY ? 0.0f : m;
+    float4 acc = make_float4(0, 0, 0, 0);
+    float l = 0.0f;
     for (uint32_t c = 0; c < nsplit; c++) {
-      const float f = exp2_fast(ld_cluster(m_at + row * 4, c) - base);
-      acc += f * ld_cluster(o_at + (row * DP + d) * 4, c);
-      l += f * ld_cluster(l_at + row * 4, c);
+      const float f = exp2_fast(ld_cluster(at, c) - zero);
+      const float4 v = ld_cluster_v4(base + (row * DP + d) * 4, c);
+      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+      l += f * ld_cluster(at + 64, c);
     }
-    out[(int64_t)row * D + d] = T(l > 0.0f || l != l ? acc / l : 0.0f);
-    if (lse && d == 0) lse[row] = l > 0.0f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+    finish(row, d, acc, m, l);
   }
-  if (nsplit > 1) cluster_sync();  // the others' shared memory is read until here
+  cluster_sync();  // the others' shared memory is read until here
 }
 
-template <int DP, bool F16>
-cudaError_t attend_launch(const KbParams& p, int32_t splits, cudaStream_t stream) {
-  auto fn = kb_attend_kernel<DP, F16>;
+template <int DP, bool F16, bool FULL>
+cudaError_t attend_launch(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
   const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * splits), (unsigned)(p.kv_heads * mtiles));
   cfg.blockDim = dim3(kAttendThreads);
-  cfg.dynamicSmemBytes = AttendSmem<DP>::kBytes;
+  cfg.dynamicSmemBytes = AttendSmem<DP>::bytes(p.select);
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fn, p);
+  cfg.numAttrs = after_select ? 2 : 1;  // queries and lengths are read before the wait: they must not come from the kernel before
+  return cudaLaunchKernelEx(&cfg, kb_attend_kernel<DP, F16, FULL>, p);
+}
+
+template <int DP, bool F16>
+cudaError_t attend_full(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
+  return p.head_dim == DP ? attend_launch<DP, F16, true>(p, splits, after_select, stream)
+                          : attend_launch<DP, F16, false>(p, splits, after_select, stream);
+}
+
+template <bool F16>
+cudaError_t attend_any(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
+  return p.head_dim <= 64    ? attend_full<64, F16>(p, splits, after_select, stream)
+         : p.head_dim <= 128 ? attend_full<128, F16>(p, splits, after_select, stream)
+                             : attend_full<256, F16>(p, splits, after_select, stream);
+}
+
+template <int DP, bool F16, bool FULL>
+cudaError_t attend_init() {
+  auto fn = kb_attend_kernel<DP, F16, FULL>;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttendSmem<DP>::bytes(kKbMaxSelect));
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
 }
 
 }  // namespace
@@ -812,9 +900,11 @@ cudaError_t kb_init() {
   set(kb_select_kernel<false, 2>, most), set(kb_select_kernel<true, 2>, most);
   set(kb_select_kernel<false, 4>, most), set(kb_select_kernel<true, 4>, most);
   set(kb_select_kernel<false, 8>, most), set(kb_select_kernel<true, 8>, most);
-  set(kb_attend_kernel<64, false>, (int)AttendSmem<64>::kBytes), set(kb_attend_kernel<64, true>, (int)AttendSmem<64>::kBytes);
-  set(kb_attend_kernel<128, false>, (int)AttendSmem<128>::kBytes), set(kb_attend_kernel<128, true>, (int)AttendSmem<128>::kBytes);
-  set(kb_attend_kernel<256, false>, (int)AttendSmem<256>::kBytes), set(kb_attend_kernel<256, true>, (int)AttendSmem<256>::kBytes);
+  for (auto init : {attend_init<64, false, false>, attend_init<64, false, true>, attend_init<64, true, false>, attend_init<64, true, true>,
+                    attend_init<128, false, false>, attend_init<128, false, true>, attend_init<128, true, false>,
+                    attend_init<128, true, true>, attend_init<256, false, false>, attend_init<256, false, true>,
+                    attend_init<256, true, false>, attend_init<256, true, true>})
+    if (e == cudaSuccess) e = init();
   return e;
 }
 
@@ -841,19 +931,14 @@ cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t s
   return p.f16 ? select_nt<true>(nt, p, shape, cluster, smem, stream) : select_nt<false>(nt, p, shape, cluster, smem, stream);
 }
 
-cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream) {
-  // Splits of a (row, kv head): enough CTAs for two an SM, at least two pieces
-  // a warp, eight at most (the portable cluster size).
+cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, bool after_select, cudaStream_t stream) {
+  // Splits of a (row, kv head): as many as fill every SM once (three CTAs each
+  // up to 128 channels, one above), while every warp has a piece, 16 at most.
   const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
-  const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles;
+  const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles, fill = (int64_t)sm_count * (p.head_dim <= 128 ? 3 : 1);
   const int64_t pieces = (int64_t)p.select * (p.block / kPiece);
-  int32_t splits = 1;
-  while (splits < 8 && units * splits < 2 * (int64_t)sm_count && pieces >= (int64_t)splits * 2 * kAttendWarps * 2) splits *= 2;
-  const int d = p.head_dim;
-  if (p.f16) return d <= 64 ? attend_launch<64, true>(p, splits, stream)
-                  : d <= 128 ? attend_launch<128, true>(p, splits, stream) : attend_launch<256, true>(p, splits, stream);
-  return d <= 64 ? attend_launch<64, false>(p, splits, stream)
-         : d <= 128 ? attend_launch<128, false>(p, splits, stream) : attend_launch<256, false>(p, splits, stream);
+  const int32_t splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({16, fill / units, pieces / kAttendWarps}));
+  return p.f16 ? attend_any<true>(p, splits, after_select, stream) : attend_any<false>(p, splits, after_select, stream);
 }
 
 }  // namespace fi8

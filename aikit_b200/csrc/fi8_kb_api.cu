@@ -59,7 +59,7 @@ int fill_select(const char* who, int32_t first, int32_t last, KbParams* p) {
 }
 
 int fill_attend(const char* who, float scale, void* d_out, float* d_lse, KbParams* p) {
-  if (!d_out) return fail(FI8_ERR_ARG, "%s: null output", who);
+  if (!d_out || !aligned16(d_out)) return fail(FI8_ERR_ARG, "%s: the output must be a 16-byte aligned device address", who);
   if (!std::isfinite(scale)) return fail(FI8_ERR_ARG, "%s: scale is not finite", who);
   p->scale = scale;
   p->out = d_out;
@@ -193,7 +193,7 @@ int fi8_kb_attend_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int
   if (rc == FI8_OK) rc = fill_attend(who, scale, d_out, d_lse, &p);
   if (rc != FI8_OK) return rc;
   DeviceGuard g(kb->device);
-  FI8_CUDA(kb_attend_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
+  FI8_CUDA(kb_attend_launch(p, kb->sm_count, false, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
   return FI8_OK;
 }
 
@@ -211,7 +211,7 @@ int fi8_kb_query_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int3
   if (rc != FI8_OK) return rc;
   DeviceGuard g(kb->device);
   FI8_CUDA(kb_select_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_select_launch");
-  FI8_CUDA(kb_attend_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
+  FI8_CUDA(kb_attend_launch(p, kb->sm_count, true, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
   return FI8_OK;
 }
 

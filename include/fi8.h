@@ -485,7 +485,7 @@ int fi8_kb_select_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int
 
 /* Attention over chosen blocks (d_sel as above, in any order; numbers outside
  * the row's blocks are skipped, one that is repeated counts again):
- * d_out [rows][q_heads][head_dim] = softmax(scale * q.k) v over the tokens below
+ * d_out [rows][q_heads][head_dim] (16-byte aligned) = softmax(scale * q.k) v over the tokens below
  * len of those blocks, and d_lse [rows][q_heads] (or NULL) the natural log of
  * the softmax's sum. A row that sees nothing gets zeros and -inf. */
 int fi8_kb_attend_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int32_t* d_slot, const int32_t* d_len,
