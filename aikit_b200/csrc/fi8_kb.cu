@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kUpdateThreads) kb_update_kernel(KbParams p, c
 // ---------------------------------------------------------------------------
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
-constexpr int kWarpPicks = 1024;  // blocks that a warp picks from
+constexpr int kWarpPicks = 1024;  // a warp picks from fewer blocks
 
 struct KbSelectShape {
   int rt;      // query rows of a CTA
@@ -170,68 +170,127 @@ struct KbSelectShape {
 };
 
 // One row's picks by a warp (WARPS = 1) or by the CTA's WARPS warps: ranks ord
-// [0 .. n) of the inner blocks, n < 32 E WARPS and n <= kWarpPicks; `need` of
-// them, behind `first` and before `last` blocks that are always in. The
-// threshold is found from the top bit down, two bits a step, from three counts
-// of at most 1023 in one word; the ranks stay in registers, and leading bits
-// that all share are skipped.
+// [0 .. n) of the inner blocks, n <= 32 E WARPS and below 1024; `need` of them,
+// behind `first` and before `last` blocks that are always in. As kth_rank does,
+// with the ranks in registers: 256 bins of equal spans of the scores (hist),
+// then the ranks of the bin that holds the need-th one, found from the top bit
+// down, two bits a step, by three counts of at most 1023 in one word. Every
+// warp scans the bins for itself; part has 3 WARPS words.
 template <int E, int WARPS>
-__device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* s_part) {
+__device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* hist, uint32_t* part) {
   constexpr int kSpan = 32 * WARPS;
   const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5, tid = warp * 32 + lane;
+  auto sync = [] {
+    if (WARPS > 1) __syncthreads();
+    else __syncwarp();
+  };
   for (int i = tid; i < first; i += kSpan) sel[i] = i;
   for (int i = tid; i < last; i += kSpan) sel[first + need + i] = first + n + i;
   if (need == 0) return;
-  // a warp's ranks are neighbours, so that its picks are
-  const int base = warp * 32 * E;
+  const int base = warp * 32 * E;  // a warp's ranks are neighbours, so that its picks are
   uint32_t v[E], top = 0, low = 0xFFFFFFFFu;
+  for (int i = tid; i < 256; i += kSpan) hist[i] = 0;
 #pragma unroll
   for (int e = 0; e < E; e++) {
     const int i = base + e * 32 + lane;
-    v[e] = i < n ? ord[i] : 0u;
+    v[e] = i < n ? ord[i] : 0u;  // past n: 0, which no count below takes in
     top = max(top, v[e]);
-    low = i < n ? min(low, v[e]) : low;
+    low = min(low, v[e] - 1u);  // the smallest score that is one
   }
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_min_sync(0xffffffffu, low);
+  if (WARPS > 1 && lane == 0) part[warp] = top, part[WARPS + warp] = low;
+  sync();
   if (WARPS > 1) {
-    if (lane == 0) s_part[2 * WARPS + warp] = top, s_part[3 * WARPS + warp] = low;
-    __syncthreads();
-    top = __reduce_max_sync(0xffffffffu, lane < WARPS ? s_part[2 * WARPS + lane] : 0u);
-    low = __reduce_min_sync(0xffffffffu, lane < WARPS ? s_part[3 * WARPS + lane] : 0xFFFFFFFFu);
+    top = __reduce_max_sync(0xffffffffu, lane < WARPS ? part[lane] : 0u);
+    low = __reduce_min_sync(0xffffffffu, lane < WARPS ? part[WARPS + lane] : 0xFFFFFFFFu);
   }
-  int bits = 32 - __clz(top ^ low);
-  uint32_t t = bits == 32 ? 0u : top >> bits << bits, count = (uint32_t)n, above = 0;
-  for (int step = 0; bits > 0 && count > (uint32_t)need; step ^= 1) {
-    bits = max(0, bits - 2);  // an odd last bit: t + 2 and t + 3 count the ranks known to be above
-    const uint32_t t1 = t + (1u << bits), t2 = t + (2u << bits), t3 = t + (3u << bits);
-    uint32_t c = 0;
+  const ScoreBins bins(ord_to_score(low + 1u), ord_to_score(top), 256);
 #pragma unroll
-    for (int e = 0; e < E; e++) c += (v[e] >= t1 ? 1u : 0u) + (v[e] >= t2 ? 1u << 10 : 0u) + (v[e] >= t3 ? 1u << 20 : 0u);
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (WARPS > 1) {  // two sets of counts in turn: one barrier a step
-      if (lane == 0) s_part[step * WARPS + warp] = c;
-      __syncthreads();
-      c = __reduce_add_sync(0xffffffffu, lane < WARPS ? s_part[step * WARPS + lane] : 0u);
-    }
-    const uint32_t c1 = c & 1023u, c2 = (c >> 10) & 1023u, c3 = c >> 20;
-    if (c3 >= (uint32_t)need) t = t3, count = c3;
-    else if (c2 >= (uint32_t)need) t = t2, count = c2, above = c3;
-    else if (c1 >= (uint32_t)need) t = t1, count = c1, above = c2;
-    else above = c1;
+  for (int e = 0; e < E; e++)
+    if (base + e * 32 + lane < n) atomicAdd(hist + bins(v[e]), 1u);
+  sync();
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) mine += hist[255 - lane * 8 - i];
+  uint32_t before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += y;
   }
-  // the ranks from t on; of the equal ones the first, when they are too many
-  const uint32_t ties = count == (uint32_t)need ? 0xFFFFFFFFu : (uint32_t)need - above;
+  before -= mine;
+  const bool here = before < (uint32_t)need && before + mine >= (uint32_t)need;
+  uint32_t bin = 0, count = 0;
+  if (here) {
+    for (int i = 0; i < 8; i++) {
+      bin = (uint32_t)(255 - lane * 8 - i);
+      count = before + hist[bin];
+      if (count >= (uint32_t)need) break;
+      before = count;
+    }
+  }
+  const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  bin = __shfl_sync(0xffffffffu, bin, from);
+  count = __shfl_sync(0xffffffffu, count, from);               // ranks in that bin or above
+  const uint32_t above_bin = __shfl_sync(0xffffffffu, before, from);
+  // the bin's ranks stay, those above it become the largest, the others 0
+  uint32_t in_top = 0, in_low = 0xFFFFFFFFu;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int b = base + e * 32 + lane < n ? bins(v[e]) : -1;
+    if (b == (int)bin) in_top = max(in_top, v[e]), in_low = min(in_low, v[e]);
+    else v[e] = b > (int)bin ? 0xFFFFFFFFu : 0u;
+  }
+  uint32_t t = 0, above = above_bin, ties = 0xFFFFFFFFu;
+  const bool whole = count == (uint32_t)need;
+  // one barrier that every warp passes: the bins' counts and `part` are read
+  in_top = __reduce_max_sync(0xffffffffu, in_top);
+  in_low = __reduce_min_sync(0xffffffffu, in_low);
+  if (WARPS > 1) {
+    if (lane == 0) part[2 * WARPS + warp] = in_top;
+    sync();
+    if (lane == 0) part[warp] = in_low;
+    sync();
+    in_top = __reduce_max_sync(0xffffffffu, lane < WARPS ? part[2 * WARPS + lane] : 0u);
+    in_low = __reduce_min_sync(0xffffffffu, lane < WARPS ? part[lane] : 0xFFFFFFFFu);
+  }
+  if (whole) {
+    t = in_low;
+  } else {
+    int bits = 32 - __clz(in_top ^ in_low);
+    t = bits == 32 ? 0u : in_top >> bits << bits;
+    for (int step = 1; bits > 0 && count > (uint32_t)need; step = 3 - step) {
+      bits = max(0, bits - 2);  // an odd last bit: t + 2 and t + 3 count the ranks known to be above
+      const uint32_t t1 = t + (1u << bits), t2 = t + (2u << bits), t3 = t + (3u << bits);
+      uint32_t c = 0;
+#pragma unroll
+      for (int e = 0; e < E; e++) c += (v[e] >= t1 ? 1u : 0u) + (v[e] >= t2 ? 1u << 10 : 0u) + (v[e] >= t3 ? 1u << 20 : 0u);
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (WARPS > 1) {  // two sets of counts in turn: one barrier a step
+        if (lane == 0) part[step * WARPS + warp] = c;
+        sync();
+        c = __reduce_add_sync(0xffffffffu, lane < WARPS ? part[step * WARPS + lane] : 0u);
+      }
+      const uint32_t c1 = c & 1023u, c2 = (c >> 10) & 1023u, c3 = c >> 20;
+      if (c3 >= (uint32_t)need) t = t3, count = c3;
+      else if (c2 >= (uint32_t)need) t = t2, count = c2, above = c3;
+      else if (c1 >= (uint32_t)need) t = t1, count = c1, above = c2;
+      else above = c1;
+    }
+    // of the ranks equal to t the first, when they are too many
+    if (count != (uint32_t)need) ties = (uint32_t)need - above;
+  }
   uint32_t gt = 0, eq = 0;  // before this warp
   if (WARPS > 1) {
     uint32_t c = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) c += base + e * 32 + lane < n ? (v[e] > t ? 1u : 0u) + (v[e] == t ? 1u << 16 : 0u) : 0u;
     c = __reduce_add_sync(0xffffffffu, c);
-    __syncthreads();
-    if (lane == 0) s_part[warp] = c;
-    __syncthreads();
-    c = __reduce_add_sync(0xffffffffu, lane < warp ? s_part[lane] : 0u);
+    sync();
+    if (lane == 0) part[warp] = c;
+    sync();
+    c = __reduce_add_sync(0xffffffffu, lane < warp ? part[lane] : 0u);
     gt = c & 0xFFFFu, eq = c >> 16;
   }
 #pragma unroll
@@ -306,7 +365,6 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
   __shared__ KthShared s_kth;
   __shared__ float s_scale[8 * NT];
   __shared__ int s_slot[32], s_len[32];
-  __shared__ uint32_t s_part[4 * kSelectWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, G = p.groups, D = p.head_dim;
   const int heads = p.q_heads / p.kv_heads, quads = (G + 3) / 4;
   const uint32_t rank = cluster_rank(), nranks = cluster_size();
@@ -430,14 +488,16 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
     if (nb <= p.select) {  // every visible block
       if (r % kSelectWarps == warp)
         for (int i = lane; i < p.select; i += 32) sel[i] = i < nb ? i : -1;
-    } else if (n <= kWarpPicks - 1) {
-      if (shape.rt == 1) {
-        kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_part);
-      } else if (r % kSelectWarps == warp) {
-        if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, nullptr);
-        else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, nullptr);
+    } else if (shape.rt > 1 && n < kWarpPicks) {
+      if (r % kSelectWarps == warp) {
+        uint32_t* hist = s_kth.hist + warp * 256;
+        if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
+        else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
       }
+    } else if (n < kWarpPicks) {
+      kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_kth.hist, s_kth.list);
     } else {
+      __syncthreads();  // warps may be picking for rows before this one
       for (int i = tid; i < p.first; i += kSelectThreads) sel[i] = i;
       for (int i = tid; i < p.last; i += kSelectThreads) sel[p.select - p.last + i] = nb - p.last + i;
       if (need > 0) {
@@ -932,12 +992,15 @@ cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t s
 }
 
 cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, bool after_select, cudaStream_t stream) {
-  // Splits of a (row, kv head): as many as fill every SM once (three CTAs each
-  // up to 128 channels, one above), while every warp has a piece, 16 at most.
+  // Splits of a (row, kv head): as many as still fit on the SMs at once (three
+  // CTAs each up to 128 channels, one above), while every warp has a piece; 16
+  // at most, and a power of two: clusters of other sizes pack badly (16 rows x 8
+  // heads over 32k tokens: 37 us with 2, 47 with 3, 44 with 4, 47 with 8).
   const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
   const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles, fill = (int64_t)sm_count * (p.head_dim <= 128 ? 3 : 1);
   const int64_t pieces = (int64_t)p.select * (p.block / kPiece);
-  const int32_t splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({16, fill / units, pieces / kAttendWarps}));
+  int32_t splits = 1;
+  while (splits < 16 && units * splits * 2 <= fill && pieces >= (int64_t)splits * 2 * kAttendWarps) splits *= 2;
   return p.f16 ? attend_any<true>(p, splits, after_select, stream) : attend_any<false>(p, splits, after_select, stream);
 }
 

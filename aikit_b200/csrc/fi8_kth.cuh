@@ -1,11 +1,12 @@
-// fi8_kth.cuh -- the threshold of a top-k over 32-bit ranks by one CTA, and the
-// picks in index order.
+// fi8_kth.cuh -- the threshold of a top-k over ranks (order-preserving images
+// of float32 scores, 0 for none), and the picks in index order.
 //
-// A histogram of 2048 equal bins between the smallest and the largest rank (a
-// radix digit from the top would put scores of one size into one bin, where
-// their atomics queue), a scan from the top, and the same again inside the bin
-// that holds the need-th rank. A caller that takes a few picks more than it
-// needs is mostly done after the first one: the best ranks lie apart.
+// The scores are counted in equal bins between the smallest and the largest: a
+// digit of the rank would put scores of one size, or all those away from zero,
+// into a few bins, whose atomics queue and which decide nothing. The bins are
+// scanned from the top; the few ranks of the bin that holds the need-th one are
+// placed by counting, and a bin of many (equal scores, or infinite ones, which
+// all share one) is searched by the ranks themselves.
 #pragma once
 
 #include "fi8_device.cuh"
@@ -16,11 +17,31 @@ namespace fi8 {
 #ifdef __CUDACC__
 
 constexpr int kKthBins = 2048;
+constexpr int kKthList = 256;
 
 struct KthShared {
   uint32_t hist[kKthBins];
+  uint32_t list[kKthList];
   uint32_t warp_a[32], warp_b[32];
-  uint32_t bin, above, in_bin;
+  uint32_t bin, above, in_bin, listed;
+};
+
+// The score of a rank (0: a NaN).
+__device__ __forceinline__ float ord_to_score(uint32_t o) {
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
+
+// Scores to bins, monotone. Without a finite span all share bin 0.
+struct ScoreBins {
+  float low, scale;
+  int last;
+  __device__ __forceinline__ ScoreBins(float low_, float high, int bins) : low(low_), last(bins - 1) {
+    scale = (float)bins / (high - low);
+    if (!(high - low < 3.0e38f) || !(scale < 3.0e38f)) scale = 0.0f;
+  }
+  __device__ __forceinline__ int operator()(uint32_t o) const {
+    return min(max((int)((ord_to_score(o) - low) * scale), 0), last);  // a NaN converts to 0
+  }
 };
 
 struct Kth {
@@ -30,38 +51,44 @@ struct Kth {
 };
 
 // need in [1, n]: between need and limit picks, or, where no threshold gives
-// so many (ranks tie), need. All threads of the CTA (a multiple of 32 that
-// divides kKthBins) call it, behind a barrier after which get(0 .. n) is ready.
+// so many (ranks tie), need. All threads of the CTA (kKthList to kKthBins, a
+// power of two) call it, behind a barrier after which get(0 .. n) is ready.
 template <typename Get>
 __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared* s) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5, per = kKthBins / nt;
-  uint32_t top = 0, low = 0xFFFFFFFFu;
+  uint32_t top = 0, low = 0xFFFFFFFFu;  // the smallest score that is one
 #pragma unroll 4
   for (int i = tid; i < n; i += nt) {
     const uint32_t o = get(i);
     top = max(top, o);
-    low = min(low, o);
+    low = min(low, o - 1u);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_min_sync(0xffffffffu, low);
   if (lane == 0) s->warp_a[warp] = top, s->warp_b[warp] = low;
   for (int i = tid; i < kKthBins; i += nt) s->hist[i] = 0;
+  if (tid == 0) s->listed = 0;
   __syncthreads();
   top = __reduce_max_sync(0xffffffffu, lane < warps ? s->warp_a[lane] : 0u);
-  low = __reduce_min_sync(0xffffffffu, lane < warps ? s->warp_b[lane] : 0xFFFFFFFFu);
-  if ((uint32_t)n <= limit) return Kth{low, 0xFFFFFFFFu, (uint32_t)n};
-  uint32_t base = low, above = 0;  // ranks from base + 2^bits on: `above` of them, all picks
-  int bits = 32 - __clz(top - low);
+  low = __reduce_min_sync(0xffffffffu, lane < warps ? s->warp_b[lane] : 0xFFFFFFFFu) + 1u;
+  if ((uint32_t)n <= limit) return Kth{0u, 0xFFFFFFFFu, (uint32_t)n};
+  const ScoreBins bins(ord_to_score(low), ord_to_score(top), kKthBins);
+  int chosen = -1;  // the bin that the ranks are searched in; -1: none yet
+  uint32_t base = 0, above = 0;  // in the bin: ranks from base + 2^bits on are all picks, `above` in all
+  int bits = 32;
   for (;;) {
     const int shift = max(0, bits - 11);
 #pragma unroll 4
     for (int i = tid; i < n; i += nt) {
-      const uint32_t o = get(i) - base;  // below base: wraps to at least 2^bits
-      if ((o >> shift) < (uint32_t)kKthBins && (bits == 32 || (o >> bits) == 0)) atomicAdd(s->hist + (o >> shift), 1u);
+      const uint32_t o = get(i);
+      const int b = bins(o);
+      if (chosen < 0) atomicAdd(s->hist + b, 1u);
+      else if (b == chosen && o >= base && (bits == 32 || ((o - base) >> bits) == 0)) atomicAdd(s->hist + ((o - base) >> shift), 1u);
     }
     __syncthreads();
     // thread 0 holds the highest bins; counts run from the top
     uint32_t mine = 0;
+#pragma unroll 4
     for (int i = 0; i < per; i++) mine += s->hist[kKthBins - 1 - tid * per - i];
     uint32_t before = mine;
 #pragma unroll
@@ -85,15 +112,49 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
       }
     }
     __syncthreads();
-    const uint32_t t = base + (s->bin << shift);
+    const uint32_t bin = s->bin, in_bin = s->in_bin;
     above = s->above;
-    const uint32_t count = above + s->in_bin;
-    if (count <= limit || shift == 0) {
+    const uint32_t t = chosen < 0 ? 0u : base + (bin << shift);
+    if (chosen >= 0 && (above + in_bin <= limit || shift == 0)) {
       __syncthreads();  // the shared memory may be used again
-      return count <= limit ? Kth{t, 0xFFFFFFFFu, count} : Kth{t, need - above, need};
+      return above + in_bin <= limit ? Kth{t, 0xFFFFFFFFu, above + in_bin} : Kth{t, need - above, need};
     }
-    base = t;
-    bits = shift;
+    if (in_bin <= (uint32_t)kKthList) {
+#pragma unroll 4
+      for (int i = tid; i < n; i += nt) {
+        const uint32_t o = get(i);
+        if (chosen < 0 ? bins(o) == (int)bin : bins(o) == chosen && o >= t && ((o - t) >> shift) == 0)
+          s->list[atomicAdd(&s->listed, 1u)] = o;
+      }
+      __syncthreads();
+      if (tid < (int)in_bin) {
+        const uint32_t mine = s->list[tid];
+        uint32_t gt = above, eq = 0;
+#pragma unroll 4
+        for (int i = 0; i < (int)in_bin; i++) {
+          gt += s->list[i] > mine;
+          eq += s->list[i] == mine;
+        }
+        // the smallest rank of the bin, when the whole bin may be taken; else the need-th
+        const bool all = above + in_bin <= limit;
+        if (all ? gt + eq == above + in_bin : gt < need && gt + eq >= need) {  // equal ranks write the same
+          s->bin = mine;
+          s->above = gt;
+          s->in_bin = eq;
+        }
+      }
+      __syncthreads();
+      const uint32_t count = s->above + s->in_bin;
+      const Kth k = count <= limit ? Kth{s->bin, 0xFFFFFFFFu, count} : Kth{s->bin, need - s->above, need};
+      __syncthreads();
+      return k;
+    }
+    if (chosen < 0) {
+      chosen = (int)bin;
+    } else {
+      base = t;
+      bits = shift;
+    }
     for (int i = tid; i < kKthBins; i += nt) s->hist[i] = 0;
     __syncthreads();
   }
