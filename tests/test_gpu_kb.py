@@ -349,3 +349,75 @@ def test_refusals(backend):
     kb.update_async(0, 0, 0, 0, 0)
     kb.sync()
     kb.Close()
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,D,block,dtype,layout", SHAPES)
+@pytest.mark.parametrize("rows,k", [(64, 12), (150, 5)])
+def test_many_rows(backend, q_heads, kv_heads, D, block, dtype, layout, rows, k):
+    """A chunk of one sequence, rows of another one in between, some that see
+    nothing or one token."""
+    n = 7 * block + 5 + rows
+    c = Cache(backend, q_heads=q_heads, kv_heads=kv_heads, D=D, block=block, capacity=n, lens=[n, 2 * block + 7], dtype=dtype,
+              layout=layout, seed=rows, max_rows=rows, fill=float("nan"))
+    c.update_all()
+    slot = [0] * rows
+    length = list(range(n - rows + 1, n + 1))
+    for i, (s, m) in enumerate([(1, 2 * block + 7), (0, 0), (1, 1), (1, 0), (0, block), (0, 3 * block + 1)]):
+        slot[7 * i + 3], length[7 * i + 3] = s, m
+    c.check(c.queries(rows), slot, length, k, scale=-0.2 if k == 5 else None)
+    c.kb.Close()
+
+
+@pytest.mark.parametrize("D,block", [(64, 16), (128, 64), (96, 32)])
+def test_many_rows_and_hidden_values(backend, D, block):
+    """Infinite and NaN keys and values reach the rows that see them and no
+    others, in one call of 100 rows as in two of 50."""
+    import torch
+    rows, n, k = 100, 6 * block + 3, 6
+    c = Cache(backend, q_heads=4, kv_heads=2, D=D, block=block, capacity=n, lens=[n, n], seed=1, max_rows=rows)
+    c.update_all()
+    at = [block + 3, 4 * block + 2, 5 * block + 1]
+    c.v[0, 0, at[0], 3], c.v[0, 1, at[1], 1], c.k[1, 0, at[2], 0], c.v[1, 1, at[2] + 3, 5] = float("nan"), float("inf"), float("nan"), -float("inf")
+    rng = np.random.default_rng(2)
+    slot, length = c.ints(rng.integers(0, 2, rows)), c.ints(rng.integers(0, n + 1, rows))
+    q = c.queries(rows)
+    sel, out, lse = torch.zeros(rows, 2, k, dtype=torch.int32, device="cuda"), torch.zeros_like(q), torch.zeros(rows, 4, device="cuda")
+    c.kb.query_async(q.data_ptr(), slot.data_ptr(), length.data_ptr(), rows, k, 0.1, sel.data_ptr(), out.data_ptr(), lse.data_ptr())
+    sel2, out2, lse2 = torch.zeros_like(sel), torch.zeros_like(out), torch.zeros_like(lse)
+    for i in (0, 50):
+        c.kb.query_async(q[i:].data_ptr(), slot[i:].data_ptr(), length[i:].data_ptr(), 50, k, 0.1, sel2[i:].data_ptr(), out2[i:].data_ptr(),
+                         lse2[i:].data_ptr())
+    c.kb.sync()
+    assert torch.equal(sel, sel2)
+    for a, b, tol in ((out, out2, 2.0**-6), (lse, lse2, 1e-4)):  # each is within its own bound of the truth; these cover both
+        a, b = a.float(), b.float()
+        assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isinf(a), torch.isinf(b))
+        ok = torch.isfinite(a)
+        assert ((a - b)[ok].abs() <= tol * (1 + b[ok].abs())).all()
+    assert torch.isnan(out).any() and torch.isinf(out).any() and torch.isfinite(out).float().mean() > 0.5
+    c.kb.Close()
+
+
+def test_thousands_of_rows(backend):
+    """Every row of 5000 equals its own in a smaller call."""
+    import torch
+    rows, n, block, k = 5000, 900, 16, 40
+    c = Cache(backend, q_heads=8, kv_heads=8, D=32, block=block, capacity=n, lens=[n, n, n], seed=1, max_rows=rows, dtype="f16")
+    c.update_all()
+    rng = np.random.default_rng(5)
+    slot, length = c.ints(np.sort(rng.integers(0, 3, rows))), c.ints(rng.integers(0, n + 1, rows))
+    q = c.queries(rows)
+    sel, out, lse = torch.zeros(rows, 8, k, dtype=torch.int32, device="cuda"), torch.zeros_like(q), torch.zeros(rows, 8, device="cuda")
+    for _ in range(2):
+        c.kb.query_async(q.data_ptr(), slot.data_ptr(), length.data_ptr(), rows, k, 0.2, sel.data_ptr(), out.data_ptr(), lse.data_ptr())
+    sel2, out2, lse2 = torch.zeros_like(sel), torch.zeros_like(out), torch.zeros_like(lse)
+    for i in range(0, rows, 50):
+        c.kb.query_async(q[i:].data_ptr(), slot[i:].data_ptr(), length[i:].data_ptr(), 50, k, 0.2, sel2[i:].data_ptr(), out2[i:].data_ptr(),
+                         lse2[i:].data_ptr())
+    c.kb.sync()
+    assert torch.equal(sel, sel2)
+    # weights near 1 differ by a half step of f16 each, results once more
+    assert ((out.float() - out2.float()).abs() <= 4 * 2.0**-11 * (1 + out2.float().abs())).all()
+    seen = length > 0
+    assert torch.equal(torch.isinf(lse).all(1), ~seen) and (lse - lse2)[seen].abs().max() < 1e-5
+    c.kb.Close()
