@@ -546,11 +546,19 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+// With a constant offset, which costs no instruction.
+template <bool TRANS, int AT>
+__device__ __forceinline__ void ldmatrix4_at(uint32_t (&r)[4], uint32_t addr) {
+  if (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4 + %5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr), "n"(AT)
+                 : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4 + %5];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr), "n"(AT)
+                 : "memory");
 }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -587,30 +595,46 @@ struct AttendState {
   }
 };
 
-// 16 tokens (keys at shared address kt, values at vt, `n` of them visible) into
-// the state. c2 >= 0 is the softmax scale times log2(e). koff and voff are the
-// lane's ldmatrix offsets: a step of 16 channels flips bits above them.
-template <int DP, bool F16, bool kQInRegs, bool FULL>
-__device__ __forceinline__ void attend_piece(AttendState<DP>& st, const uint32_t (&qf)[kQInRegs ? DP / 16 : 1][4], uint32_t qt,
-                                             uint32_t kt, uint32_t vt, uint32_t qoff, uint32_t koff, int n, float c2, int steps) {
+// Steps t = 0 .. STEPS - 1 as compile-time constants: f(Int<t>{}).
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+template <int STEPS, int T = 0, typename F>
+__device__ __forceinline__ void for_steps(F f) {
+  if constexpr (T < STEPS) {
+    f(Int<T>{});
+    for_steps<STEPS, T + 1>(f);
+  }
+}
+
+// The 16 tokens of stage S (`n` of them visible) into the state. c2 >= 0 is the
+// softmax scale times log2(e). ka and va are the lane's ldmatrix addresses in
+// stage 0 for the steps 0 .. 3 of 16 channels, whose two bits are permuted by
+// the row; further steps and stages are constant offsets. q0: from a value
+// address to the same place of the query tile.
+template <int DP, bool F16, bool kQInRegs, bool FULL, int S>
+__device__ __forceinline__ void attend_piece(AttendState<DP>& st, const uint32_t (&qf)[kQInRegs ? DP / 16 : 1][4], uint32_t q0,
+                                             const uint32_t (&ka)[4], const uint32_t (&va)[4], int n, float c2, int steps) {
+  constexpr int kAt = S * (int)AttendSmem<DP>::kStage, kValues = kAt + kPiece * DP * 2;
   using E = Elem<F16>;
   const int lane = threadIdx.x & 31;
   float sc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-  for (int t = 0; t < DP / 16; t++) {
-    if (!FULL && t >= steps) break;
+  for_steps<DP / 16>([&](auto step) {
+    constexpr int t = decltype(step)::value;
+    if (!FULL && t >= steps) return;
     uint32_t kf[4];
-    ldmatrix4(kf, kt + (koff ^ (t * 32)));
-    if (kQInRegs) {
-      E::mma(sc[0], qf[kQInRegs ? t : 0], kf[0], kf[1]);
-      E::mma(sc[1], qf[kQInRegs ? t : 0], kf[2], kf[3]);
+    ldmatrix4_at<false, kAt + (t >> 2) * 128>(kf, ka[t & 3]);
+    if constexpr (kQInRegs) {
+      E::mma(sc[0], qf[t], kf[0], kf[1]);
+      E::mma(sc[1], qf[t], kf[2], kf[3]);
     } else {
       uint32_t a[4];
-      ldmatrix4(a, qt + (qoff ^ (t * 32)));
+      ldmatrix4_at<false, (t >> 2) * 128>(a, va[t & 3] + q0);
       E::mma(sc[0], a, kf[0], kf[1]);
       E::mma(sc[1], a, kf[2], kf[3]);
     }
-  }
+  });
   if (n < kPiece) {
 #pragma unroll
     for (int j = 0; j < 2; j++)
@@ -656,14 +680,14 @@ __device__ __forceinline__ void attend_piece(AttendState<DP>& st, const uint32_t
     pf[2 * j] = E::pack(w[0], w[1]);
     pf[2 * j + 1] = E::pack(w[2], w[3]);
   }
-#pragma unroll
-  for (int t = 0; t < DP / 16; t++) {
-    if (!FULL && t >= steps) break;
+  for_steps<DP / 16>([&](auto step) {
+    constexpr int t = decltype(step)::value;
+    if (!FULL && t >= steps) return;
     uint32_t vf[4];
-    ldmatrix4_trans(vf, vt + (qoff ^ (t * 32)));
+    ldmatrix4_at<true, kValues + (t >> 2) * 128>(vf, va[t & 3]);
     E::mma(st.o[2 * t], pf, vf[0], vf[1]);
     E::mma(st.o[2 * t + 1], pf, vf[2], vf[3]);
-  }
+  });
 }
 
 // Two packed values of the query tile, negated when the scale is negative (the
@@ -732,34 +756,43 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   const int64_t to_values = static_cast<const char*>(p.v) - static_cast<const char*>(p.k);
   const uint32_t ring = base + warp * S::kRing;
   const bool copies = FULL || lane_chunk < chunks;
-  const uint32_t to0 = tile_at<DP>(lane_row, lane_chunk);  // of a row further on by a multiple of kRowStep: chunk bits flipped
+  // where a warp's first rows go; rows further on by multiples of kRowStep flip chunk bits
+  uint32_t to[8 / kRowStep];
+#pragma unroll
+  for (int i = 0; i < 8 / kRowStep; i++) to[i] = ring + (tile_at<DP>(lane_row, lane_chunk) ^ ((i * kRowStep) << 4));
+  uint32_t ka[4], va[4];
+#pragma unroll
+  for (int t = 0; t < 4; t++) ka[t] = ring + (koff ^ (t * 32)), va[t] = ring + (qoff ^ (t * 32));
   const int64_t row_step = kRowStep * pitch;
 
-  // starts the copies of piece i; the tokens of it that the row sees (0: skipped)
-  auto load = [&](int i, uint32_t dst) {
+  // starts the copies of piece i into a stage; the tokens of it that the row sees (0: skipped)
+  auto load = [&](int i, auto stage) {
+    constexpr int kAt = decltype(stage)::value * (int)S::kStage;
     int n = 0;
     const int b = i < pieces ? s_sel[i >> shift] : -1;
     if (b >= 0 && b < nb) {
       const int t0 = b * p.block + (i & ((1 << shift) - 1)) * kPiece;
       n = max(0, min(kPiece, len - t0));
       const char* from = kbase + t0 * pitch;
-      if (n == kPiece) {
-        if (copies)
+      if (copies && n > 0) {
+        if (n == kPiece) {
 #pragma unroll
           for (int row = 0; row < kPiece; row += kRowStep) {
-            const uint32_t at = dst + (to0 ^ ((row & 7) << 4)) + row * (DP * 2);
+            const uint32_t at = to[(row & 7) / kRowStep] + kAt + row * (DP * 2);
             cp_async16(at, from, true);
             cp_async16(at + kPiece * DP * 2, from + to_values, true);
             from += row_step;
           }
-      } else if (n > 0 && copies) {
-        for (int row = 0; row < kPiece; row += kRowStep) {
-          // hidden tokens are zeros: 0 * their weight 0 stays 0
-          const bool ok = row + lane_row < n;
-          const uint32_t at = dst + (to0 ^ ((row & 7) << 4)) + row * (DP * 2);
-          cp_async16(at, ok ? from : kbase, ok);
-          cp_async16(at + kPiece * DP * 2, (ok ? from : kbase) + to_values, ok);
-          from += row_step;
+        } else {
+#pragma unroll 1
+          for (int row = 0; row < kPiece; row += kRowStep) {
+            // hidden tokens are zeros: 0 * their weight 0 stays 0
+            const bool ok = row + lane_row < n;
+            const uint32_t at = ring + (tile_at<DP>(lane_row, lane_chunk) ^ ((row & 7) << 4)) + kAt + row * (DP * 2);
+            cp_async16(at, ok ? from : kbase, ok);
+            cp_async16(at + kPiece * DP * 2, (ok ? from : kbase) + to_values, ok);
+            from += row_step;
+          }
         }
       }
     }
@@ -772,21 +805,19 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   const float c2 = fabsf(p.scale) * 1.4426950408889634f;  // log2(e)
   int i = (int)rank * kAttendWarps + warp;
   int have[NS];
-#pragma unroll
-  for (int s = 0; s < NS - 1; s++) have[s] = load(i + s * stride, ring + s * S::kStage);
+  for_steps<NS - 1>([&](auto s) { have[decltype(s)::value] = load(i + decltype(s)::value * stride, s); });
   for (; i < pieces; i += NS * stride) {
-#pragma unroll
-    for (int s = 0; s < NS; s++) {
+    for_steps<NS>([&](auto stage) {
+      constexpr int s = decltype(stage)::value, before = (s + NS - 1) % NS;
       const int at = i + s * stride;
-      if (at >= pieces) break;
-      have[(s + NS - 1) % NS] = load(at + (NS - 1) * stride, ring + (s + NS - 1) % NS * S::kStage);
+      if (at >= pieces) return;
+      have[before] = load(at + (NS - 1) * stride, Int<before>{});
       cp_async_wait<NS - 1>();
       __syncwarp();
-      const uint32_t kt = ring + s * S::kStage;
       if (have[s] > 0)
-        attend_piece<DP, F16, kQInRegs, FULL>(st, qf, base + S::kQuery, kt, kt + kPiece * DP * 2, qoff, koff, have[s], c2, steps);
+        attend_piece<DP, F16, kQInRegs, FULL, s>(st, qf, base + S::kQuery - ring, ka, va, have[s], c2, steps);
       __syncwarp();  // the stage may be filled again
-    }
+    });
   }
   cp_async_wait<0>();
 #pragma unroll
