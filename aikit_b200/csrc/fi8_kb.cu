@@ -512,33 +512,36 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
 // ---------------------------------------------------------------------------
 // Attention over the chosen blocks. One pass over the keys and values with the
 // running maximum and sum of the softmax (in the log2 domain). The query heads
-// that share a key/value head are the rows of one 16-row matrix product, so
-// each key and value is read once for all of them; bound by those bytes.
-// A cluster of CTAs per (query row, kv head, tile of 16 query heads); the
-// selected blocks are dealt in pieces of 16 tokens to the cluster's warps, and
-// each warp runs its own ring of asynchronous copies and its own softmax, so
-// nothing but the end synchronizes. The warps' partial results are joined in
-// shared memory, the CTAs' through the cluster's.
+// that share a key/value head share one read of each key and value; bound by
+// those bytes. They are the columns of the matrix products, eight or sixteen,
+// and the tokens and channels their rows: S' = K Q', O' = V' P'. (With the heads
+// as the rows a tile has sixteen of them whether they are there or not: twice
+// the products, results and exponentials for up to eight heads.)
+// A cluster of CTAs per (query row, kv head, tile of heads); the selected blocks
+// are dealt in pieces of 16 tokens to the cluster's warps, and each warp runs
+// its own ring of asynchronous copies and its own softmax, so nothing but the
+// end synchronizes. The warps' partial results are joined in shared memory, the
+// CTAs' through the cluster's.
 // ---------------------------------------------------------------------------
 constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kPiece = 16;
 
-// Shared memory of a head dimension up to DP: the warps' rings (each holds, at
-// the end, its warp's result; the CTA's joined result, 16 x DP f32, replaces the
-// first), the query tile, maxima and sums, the chosen blocks. Three CTAs an SM
-// up to 128.
-template <int DP>
+// Shared memory of a head dimension up to DP and 8 NT heads: the warps' rings
+// (each holds, at the end, its warp's result, rows of kRow floats; the CTA's
+// joined result replaces the first), the query tile, maxima and sums, the chosen
+// blocks. Three CTAs an SM up to 128.
+template <int DP, int NT>
 struct AttendSmem {
-  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr int kStages = DP == 64 ? 4 : 2, kHeads = 8 * NT;
   static constexpr uint32_t kStage = 2 * kPiece * DP * 2;  // 16 keys, then 16 values
   static constexpr uint32_t kRing = kStages * kStage;      // of a warp
-  static constexpr uint32_t kQuery = kAttendWarps * kRing, kStats = kQuery + 16 * DP * 2;
-  static_assert(kRing >= 16 * DP * 4, "a warp's result fits its ring");
-  static constexpr uint32_t kSel = kStats + 2 * 16 * 4 + 2 * kAttendWarps * 16 * 4;
+  static constexpr uint32_t kRow = DP + 4;                 // eight channels of four even heads fall into different banks
+  static constexpr uint32_t kQuery = kAttendWarps * kRing, kStats = kQuery + kHeads * DP * 2;
+  static_assert(kRing >= kHeads * kRow * 4, "a warp's result fits its ring");
+  static constexpr uint32_t kSel = kStats + (2 + 2 * kAttendWarps) * kHeads * 4;
   static size_t bytes(int select) { return kSel + (size_t)select * 4; }
 };
-static_assert(AttendSmem<256>::kSel + kKbMaxSelect * 4 <= 227 * 1024, "shared memory");
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -581,17 +584,21 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return (uint32_t)(r * (DP * 2) + ((c ^ (r & 7)) << 4));
 }
 
-// The running state of 16 query rows over the tokens of a warp (log2 domain):
-// lane 4 r + t holds rows r and r + 8.
-template <int DP>
+// The running state of 8 NT heads over the tokens of a warp (log2 domain): lane
+// 4 g + t holds channels 16 i + g and 16 i + g + 8 of heads 2t and 2t + 1 of each
+// eight; the lane's sums are those of its own tokens.
+template <int DP, int NT>
 struct AttendState {
-  float o[DP / 8][4];
-  float mx[2], sum[2];
+  float o[NT][DP / 16][4];
+  float mx[NT][2], sum[NT][2];
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < DP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    mx[0] = mx[1] = -INFINITY;
-    sum[0] = sum[1] = 0.0f;
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int i = 0; i < DP / 16; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+      mx[n][0] = mx[n][1] = -INFINITY;
+      sum[n][0] = sum[n][1] = 0.0f;
+    }
   }
 };
 
@@ -608,85 +615,96 @@ __device__ __forceinline__ void for_steps(F f) {
   }
 }
 
+// An 8 x 8 matrix of 16-bit values, transposed across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
 // The 16 tokens of stage S (`n` of them visible) into the state. c2 >= 0 is the
 // softmax scale times log2(e). ka and va are the lane's ldmatrix addresses in
 // stage 0 for the steps 0 .. 3 of 16 channels, whose two bits are permuted by
-// the row; further steps and stages are constant offsets. q0: from a value
-// address to the same place of the query tile.
-template <int DP, bool F16, bool kQInRegs, bool FULL, int S>
-__device__ __forceinline__ void attend_piece(AttendState<DP>& st, const uint32_t (&qf)[kQInRegs ? DP / 16 : 1][4], uint32_t q0,
-                                             const uint32_t (&ka)[4], const uint32_t (&va)[4], int n, float c2, int steps) {
-  constexpr int kAt = S * (int)AttendSmem<DP>::kStage, kValues = kAt + kPiece * DP * 2;
+// the row; further steps and stages are constant offsets.
+template <int DP, int NT, bool F16, bool FULL, int S>
+__device__ __forceinline__ void attend_piece(AttendState<DP, NT>& st, const uint32_t (&qf)[NT][DP / 16][2], const uint32_t (&ka)[4],
+                                             const uint32_t (&va)[4], int n, float c2, int steps) {
+  constexpr int kAt = S * (int)AttendSmem<DP, NT>::kStage, kValues = kAt + kPiece * DP * 2;
   using E = Elem<F16>;
   const int lane = threadIdx.x & 31;
-  float sc[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  // tokens g and g + 8 by heads 2t and 2t + 1
+  float sc[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; i++) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
   for_steps<DP / 16>([&](auto step) {
     constexpr int t = decltype(step)::value;
     if (!FULL && t >= steps) return;
     uint32_t kf[4];
     ldmatrix4_at<false, kAt + (t >> 2) * 128>(kf, ka[t & 3]);
-    if constexpr (kQInRegs) {
-      E::mma(sc[0], qf[t], kf[0], kf[1]);
-      E::mma(sc[1], qf[t], kf[2], kf[3]);
-    } else {
-      uint32_t a[4];
-      ldmatrix4_at<false, (t >> 2) * 128>(a, va[t & 3] + q0);
-      E::mma(sc[0], a, kf[0], kf[1]);
-      E::mma(sc[1], a, kf[2], kf[3]);
-    }
+#pragma unroll
+    for (int i = 0; i < NT; i++) E::mma(sc[i], kf, qf[i][t][0], qf[i][t][1]);
   });
   if (n < kPiece) {
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int i = 0; i < NT; i++)
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        if (j * 8 + (lane & 3) * 2 + (e & 1) >= n) sc[j][e] = -INFINITY;
+        if ((lane >> 2) + (e & 2) * 4 >= n) sc[i][e] = -INFINITY;
   }
-  // the rows' maxima: the four lanes that share a row
-  float pm[2];
+  // the heads' maxima: the eight lanes that share their columns
+  float pm[NT][2];
+  bool up = false;
 #pragma unroll
-  for (int e = 0; e < 2; e++) {
-    pm[e] = fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1]));
-    pm[e] = fmaxf(pm[e], __shfl_xor_sync(0xffffffffu, pm[e], 1));
-    pm[e] = fmaxf(pm[e], __shfl_xor_sync(0xffffffffu, pm[e], 2));
-    // scaled after the maximum; a scale of 0 must not meet -inf
-    pm[e] = fmaxf(st.mx[e], pm[e] == -INFINITY ? -INFINITY : pm[e] * c2);
-  }
-  if (__any_sync(0xffffffffu, pm[0] != st.mx[0] || pm[1] != st.mx[1])) {
-    const float f0 = pm[0] == st.mx[0] ? 1.0f : exp2_fast(st.mx[0] - pm[0]);
-    const float f1 = pm[1] == st.mx[1] ? 1.0f : exp2_fast(st.mx[1] - pm[1]);
+  for (int i = 0; i < NT; i++)
 #pragma unroll
-    for (int t = 0; t < DP / 8; t++) {
-      st.o[t][0] *= f0, st.o[t][1] *= f0;
-      st.o[t][2] *= f1, st.o[t][3] *= f1;
+    for (int e = 0; e < 2; e++) {
+      float m = fmaxf(sc[i][e], sc[i][e + 2]);
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+      // scaled after the maximum; a scale of 0 must not meet -inf
+      pm[i][e] = fmaxf(st.mx[i][e], m == -INFINITY ? -INFINITY : m * c2);
+      up |= pm[i][e] != st.mx[i][e];
     }
-    st.sum[0] *= f0, st.sum[1] *= f1;
-    st.mx[0] = pm[0], st.mx[1] = pm[1];
-  }
-  // a row that has seen nothing but -inf keeps weights of 0
-  const float base0 = st.mx[0] == -INFINITY ? 0.0f : -st.mx[0], base1 = st.mx[1] == -INFINITY ? 0.0f : -st.mx[1];
-  uint32_t pf[4];
+  if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
+    for (int i = 0; i < NT; i++) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        f[e] = pm[i][e] == st.mx[i][e] ? 1.0f : exp2_fast(st.mx[i][e] - pm[i][e]);
+        st.sum[i][e] *= f[e];
+        st.mx[i][e] = pm[i][e];
+      }
+#pragma unroll
+      for (int t = 0; t < DP / 16; t++) {
+        st.o[i][t][0] *= f[0], st.o[i][t][1] *= f[1];
+        st.o[i][t][2] *= f[0], st.o[i][t][3] *= f[1];
+      }
+    }
+  }
+  uint32_t pf[NT][2];
+#pragma unroll
+  for (int i = 0; i < NT; i++) {
     float w[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      w[e] = exp2_fast(fmaf(sc[j][e], c2, e < 2 ? base0 : base1));
-      if (n < kPiece && sc[j][e] == -INFINITY) w[e] = 0.0f;  // -inf times a scale of 0
+      // a head that has seen nothing but -inf keeps weights of 0
+      const float base = st.mx[i][e & 1] == -INFINITY ? 0.0f : -st.mx[i][e & 1];
+      w[e] = exp2_fast(fmaf(sc[i][e], c2, base));
+      if (n < kPiece && sc[i][e] == -INFINITY) w[e] = 0.0f;  // -inf times a scale of 0
+      st.sum[i][e & 1] += w[e];
     }
-    st.sum[0] += w[0] + w[1];
-    st.sum[1] += w[2] + w[3];
     // the weights enter the product in the cache's type (a relative 2^-9 or 2^-12 each; the sums stay 32 bits)
-    pf[2 * j] = E::pack(w[0], w[1]);
-    pf[2 * j + 1] = E::pack(w[2], w[3]);
+    pf[i][0] = transpose8(E::pack(w[0], w[1]));
+    pf[i][1] = transpose8(E::pack(w[2], w[3]));
   }
   for_steps<DP / 16>([&](auto step) {
     constexpr int t = decltype(step)::value;
     if (!FULL && t >= steps) return;
     uint32_t vf[4];
     ldmatrix4_at<true, kValues + (t >> 2) * 128>(vf, va[t & 3]);
-    E::mma(st.o[2 * t], pf, vf[0], vf[1]);
-    E::mma(st.o[2 * t + 1], pf, vf[2], vf[3]);
+#pragma unroll
+    for (int i = 0; i < NT; i++) E::mma(st.o[i][t], vf, pf[i][0], pf[i][1]);
   });
 }
 
@@ -698,35 +716,35 @@ __device__ __forceinline__ uint4 flip_sign(uint4 w, bool flip) {
 }
 
 // FULL: head_dim is DP itself.
-template <int DP, bool F16, bool FULL>
+template <int DP, int NT, bool F16, bool FULL>
 __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_kernel(KbParams p) {
   using E = Elem<F16>;
   using T = typename E::T;
-  using S = AttendSmem<DP>;
+  using S = AttendSmem<DP, NT>;
   constexpr int NS = S::kStages;
   constexpr int kChunks = DP / 8;             // 16-byte chunks of a padded row
   constexpr int kRowStep = 32 / kChunks;      // rows that a warp copies at once
-  constexpr bool kQInRegs = DP <= 128;        // else the query fragments are read again for each piece
   extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), nsplit = cluster_size();
   const int r = blockIdx.x / nsplit;
-  const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
-  const int h = blockIdx.y / mtiles, m0 = (blockIdx.y % mtiles) * 16;
-  const int mrows = min(16, heads - m0);
+  const int heads = p.q_heads / p.kv_heads, mtiles = (heads + S::kHeads - 1) / S::kHeads;
+  const int h = blockIdx.y / mtiles, m0 = (blockIdx.y % mtiles) * S::kHeads;
+  const int mrows = min(S::kHeads, heads - m0);
   const int D = FULL ? DP : p.head_dim, chunks = D / 8, steps = D / 16;
   const uint32_t base = smem_u32(smem);
   float* s_o = reinterpret_cast<float*>(smem);  // each value replaces the first warp's, which the same thread has read
-  float* s_m = reinterpret_cast<float*>(smem + S::kStats);  // [16], then the sums [16]
-  float* w_m = s_m + 32;                                    // the warps' [warps][16], then their sums
-  float* w_l = w_m + kAttendWarps * 16;
+  float* s_m = reinterpret_cast<float*>(smem + S::kStats);  // maxima, then the sums
+  float* w_m = s_m + 2 * S::kHeads;                         // the warps', then their sums
+  float* w_l = w_m + kAttendWarps * S::kHeads;
   int* s_sel = reinterpret_cast<int*>(smem + S::kSel);
 
   // the query tile: absent heads are zero rows
   const T* q = static_cast<const T*>(p.q) + (int64_t)r * p.q_stride + (int64_t)(h * heads + m0) * D;
 #pragma unroll
-  for (int i0 = 0; i0 < 16 * kChunks; i0 += kAttendThreads) {
+  for (int i0 = 0; i0 < S::kHeads * kChunks; i0 += kAttendThreads) {
     const int i = i0 + tid, row = i / kChunks, c = i % kChunks;
+    if (S::kHeads * kChunks < kAttendThreads && i >= S::kHeads * kChunks) break;
     uint4 w = make_uint4(0, 0, 0, 0);
     if (row < mrows && c < chunks) w = flip_sign(__ldg(reinterpret_cast<const uint4*>(q + (int64_t)row * D) + c), p.scale < 0.0f);
     *reinterpret_cast<uint4*>(smem + S::kQuery + tile_at<DP>(row, c)) = w;
@@ -738,14 +756,17 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   const int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
   for (int i = tid; i < p.select; i += kAttendThreads) s_sel[i] = __ldcg(sel + i);
   __syncthreads();
-  // ldmatrix lane addresses. Query and values: rows 0-7 / 8-15 by lane bit 3, chunk + 1 by bit 4; keys: the other way round
-  const uint32_t qoff = tile_at<DP>(lane & 15, lane >> 4), koff = tile_at<DP>((lane & 7) + ((lane & 16) >> 1), (lane >> 3) & 1);
-  uint32_t qf[kQInRegs ? DP / 16 : 1][4];
-  if (kQInRegs) {
+  // ldmatrix lane addresses. Keys: tokens 0-7 / 8-15 by lane bit 3, chunk + 1 by bit 4; values: the other way round
+  const uint32_t koff = tile_at<DP>(lane & 15, lane >> 4), voff = tile_at<DP>((lane & 7) + ((lane & 16) >> 1), (lane >> 3) & 1);
+  uint32_t qf[NT][DP / 16][2];
 #pragma unroll
-    for (int s = 0; s < DP / 16; s++)
-      if (FULL || s < steps) ldmatrix4(qf[kQInRegs ? s : 0], base + S::kQuery + (qoff ^ (s * 32)));
-  }
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int t = 0; t < DP / 16; t += 2) {
+      uint32_t f[4];
+      ldmatrix4(f, base + S::kQuery + tile_at<DP>(n * 8 + (lane & 7), 2 * t + (lane >> 3)));
+      qf[n][t][0] = f[0], qf[n][t][1] = f[1], qf[n][t + 1][0] = f[2], qf[n][t + 1][1] = f[3];
+    }
 
   const int shift = __ffs(p.block / kPiece) - 1, pieces = p.select << shift;
   const int stride = (int)nsplit * kAttendWarps;
@@ -762,7 +783,7 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   for (int i = 0; i < 8 / kRowStep; i++) to[i] = ring + (tile_at<DP>(lane_row, lane_chunk) ^ ((i * kRowStep) << 4));
   uint32_t ka[4], va[4];
 #pragma unroll
-  for (int t = 0; t < 4; t++) ka[t] = ring + (koff ^ (t * 32)), va[t] = ring + (qoff ^ (t * 32));
+  for (int t = 0; t < 4; t++) ka[t] = ring + (koff ^ (t * 32)), va[t] = ring + (voff ^ (t * 32));
   const int64_t row_step = kRowStep * pitch;
 
   // starts the copies of piece i into a stage; the tokens of it that the row sees (0: skipped)
@@ -800,7 +821,7 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
     return n;
   };
 
-  AttendState<DP> st;
+  AttendState<DP, NT> st;
   st.clear();
   const float c2 = fabsf(p.scale) * 1.4426950408889634f;  // log2(e)
   int i = (int)rank * kAttendWarps + warp;
@@ -815,30 +836,34 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
       cp_async_wait<NS - 1>();
       __syncwarp();
       if (have[s] > 0)
-        attend_piece<DP, F16, kQInRegs, FULL, s>(st, qf, base + S::kQuery - ring, ka, va, have[s], c2, steps);
+        attend_piece<DP, NT, F16, FULL, s>(st, qf, ka, va, have[s], c2, steps);
       __syncwarp();  // the stage may be filled again
     });
   }
   cp_async_wait<0>();
 #pragma unroll
-  for (int e = 0; e < 2; e++) {
-    st.sum[e] += __shfl_xor_sync(0xffffffffu, st.sum[e], 1);
-    st.sum[e] += __shfl_xor_sync(0xffffffffu, st.sum[e], 2);
-  }
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) st.sum[n][e] += __shfl_xor_sync(0xffffffffu, st.sum[n][e], x);
   __syncwarp();
   {  // the warp's result over its own ring
-    const int row = lane >> 2, col = (lane & 3) * 2;
     float* mine = reinterpret_cast<float*>(smem + warp * S::kRing);
 #pragma unroll
-    for (int t = 0; t < DP / 8; t++) {
-      if (t * 8 >= D) break;
-      if (row < mrows) *reinterpret_cast<float2*>(mine + row * DP + t * 8 + col) = make_float2(st.o[t][0], st.o[t][1]);
-      if (row + 8 < mrows) *reinterpret_cast<float2*>(mine + (row + 8) * DP + t * 8 + col) = make_float2(st.o[t][2], st.o[t][3]);
-    }
-    if ((lane & 3) == 0) {
-      w_m[warp * 16 + row] = st.mx[0], w_m[warp * 16 + row + 8] = st.mx[1];
-      w_l[warp * 16 + row] = st.sum[0], w_l[warp * 16 + row + 8] = st.sum[1];
-    }
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int head = n * 8 + (lane & 3) * 2 + e;
+        if (head >= mrows) continue;
+#pragma unroll
+        for (int t = 0; t < DP / 16; t++) {
+          if (!FULL && t >= steps) break;
+          mine[head * S::kRow + t * 16 + (lane >> 2)] = st.o[n][t][e];
+          mine[head * S::kRow + t * 16 + (lane >> 2) + 8] = st.o[n][t][e + 2];
+        }
+        if (lane < 4) w_m[warp * S::kHeads + head] = st.mx[n][e], w_l[warp * S::kHeads + head] = st.sum[n][e];
+      }
   }
   __syncthreads();
   T* out = static_cast<T*>(p.out) + ((int64_t)r * p.q_heads + h * heads + m0) * D;
@@ -855,22 +880,22 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
     if (d >= D) continue;
     float m = w_m[row];
 #pragma unroll
-    for (int w = 1; w < kAttendWarps; w++) m = fmaxf(m, w_m[w * 16 + row]);
+    for (int w = 1; w < kAttendWarps; w++) m = fmaxf(m, w_m[w * S::kHeads + row]);
     const float zero = m == -INFINITY ? 0.0f : m;
     float4 acc = make_float4(0, 0, 0, 0);
     float l = 0.0f;
 #pragma unroll
     for (int w = 0; w < kAttendWarps; w++) {
-      const float f = exp2_fast(w_m[w * 16 + row] - zero);
-      const float4 v = *reinterpret_cast<const float4*>(smem + w * S::kRing + (row * DP + d) * 4);
+      const float f = exp2_fast(w_m[w * S::kHeads + row] - zero);
+      const float4 v = *reinterpret_cast<const float4*>(smem + w * S::kRing + (row * S::kRow + d) * 4);
       acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-      l += f * w_l[w * 16 + row];
+      l += f * w_l[w * S::kHeads + row];
     }
     if (nsplit == 1) {
       finish(row, d, acc, m, l);
     } else {
-      *reinterpret_cast<float4*>(s_o + row * DP + d) = acc;
-      if (d == 0) s_m[row] = m, s_m[16 + row] = l;
+      *reinterpret_cast<float4*>(s_o + row * S::kRow + d) = acc;
+      if (d == 0) s_m[row] = m, s_m[S::kHeads + row] = l;
     }
   }
   if (nsplit == 1) return;
@@ -887,18 +912,18 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
     float l = 0.0f;
     for (uint32_t c = 0; c < nsplit; c++) {
       const float f = exp2_fast(ld_cluster(at, c) - zero);
-      const float4 v = ld_cluster_v4(base + (row * DP + d) * 4, c);
+      const float4 v = ld_cluster_v4(base + (row * S::kRow + d) * 4, c);
       acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-      l += f * ld_cluster(at + 64, c);
+      l += f * ld_cluster(at + S::kHeads * 4, c);
     }
     finish(row, d, acc, m, l);
   }
   cluster_sync();  // the others' shared memory is read until here
 }
 
-template <int DP, bool F16, bool FULL>
+template <int DP, int NT, bool F16, bool FULL>
 cudaError_t attend_launch(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
-  const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
+  const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 8 * NT - 1) / (8 * NT);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)splits;
@@ -909,31 +934,42 @@ cudaError_t attend_launch(const KbParams& p, int32_t splits, bool after_select, 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.rows * splits), (unsigned)(p.kv_heads * mtiles));
   cfg.blockDim = dim3(kAttendThreads);
-  cfg.dynamicSmemBytes = AttendSmem<DP>::bytes(p.select);
+  cfg.dynamicSmemBytes = AttendSmem<DP, NT>::bytes(p.select);
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = after_select ? 2 : 1;  // queries and lengths are read before the wait: they must not come from the kernel before
-  return cudaLaunchKernelEx(&cfg, kb_attend_kernel<DP, F16, FULL>, p);
+  return cudaLaunchKernelEx(&cfg, kb_attend_kernel<DP, NT, F16, FULL>, p);
 }
 
-template <int DP, bool F16>
+template <int DP, int NT, bool F16>
 cudaError_t attend_full(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
-  return p.head_dim == DP ? attend_launch<DP, F16, true>(p, splits, after_select, stream)
-                          : attend_launch<DP, F16, false>(p, splits, after_select, stream);
+  return p.head_dim == DP ? attend_launch<DP, NT, F16, true>(p, splits, after_select, stream)
+                          : attend_launch<DP, NT, F16, false>(p, splits, after_select, stream);
 }
 
-template <bool F16>
+template <bool F16, int NT>
 cudaError_t attend_any(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
-  return p.head_dim <= 64    ? attend_full<64, F16>(p, splits, after_select, stream)
-         : p.head_dim <= 128 ? attend_full<128, F16>(p, splits, after_select, stream)
-                             : attend_full<256, F16>(p, splits, after_select, stream);
+  return p.head_dim <= 64    ? attend_full<64, NT, F16>(p, splits, after_select, stream)
+         : p.head_dim <= 128 ? attend_full<128, NT, F16>(p, splits, after_select, stream)
+                             : attend_full<256, NT, F16>(p, splits, after_select, stream);
 }
 
-template <int DP, bool F16, bool FULL>
+template <int DP, int NT, bool F16, bool FULL>
 cudaError_t attend_init() {
-  auto fn = kb_attend_kernel<DP, F16, FULL>;
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttendSmem<DP>::bytes(kKbMaxSelect));
+  auto fn = kb_attend_kernel<DP, NT, F16, FULL>;
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttendSmem<DP, NT>::bytes(kKbMaxSelect));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  return e;
+}
+
+template <int NT>
+cudaError_t attend_init_all() {
+  cudaError_t e = cudaSuccess;
+  for (auto init : {attend_init<64, NT, false, false>, attend_init<64, NT, false, true>, attend_init<64, NT, true, false>,
+                    attend_init<64, NT, true, true>, attend_init<128, NT, false, false>, attend_init<128, NT, false, true>,
+                    attend_init<128, NT, true, false>, attend_init<128, NT, true, true>, attend_init<256, NT, false, false>,
+                    attend_init<256, NT, false, true>, attend_init<256, NT, true, false>, attend_init<256, NT, true, true>})
+    if (e == cudaSuccess) e = init();
   return e;
 }
 
@@ -991,11 +1027,8 @@ cudaError_t kb_init() {
   set(kb_select_kernel<false, 2>, most), set(kb_select_kernel<true, 2>, most);
   set(kb_select_kernel<false, 4>, most), set(kb_select_kernel<true, 4>, most);
   set(kb_select_kernel<false, 8>, most), set(kb_select_kernel<true, 8>, most);
-  for (auto init : {attend_init<64, false, false>, attend_init<64, false, true>, attend_init<64, true, false>, attend_init<64, true, true>,
-                    attend_init<128, false, false>, attend_init<128, false, true>, attend_init<128, true, false>,
-                    attend_init<128, true, true>, attend_init<256, false, false>, attend_init<256, false, true>,
-                    attend_init<256, true, false>, attend_init<256, true, true>})
-    if (e == cudaSuccess) e = init();
+  if (e == cudaSuccess) e = attend_init_all<1>();
+  if (e == cudaSuccess) e = attend_init_all<2>();
   return e;
 }
 
@@ -1027,12 +1060,14 @@ cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, bool after_sel
   // CTAs each up to 128 channels, one above), while every warp has a piece; 16
   // at most, and a power of two: clusters of other sizes pack badly (16 rows x 8
   // heads over 32k tokens: 37 us with 2, 47 with 3, 44 with 4, 47 with 8).
-  const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 15) / 16;
+  const int heads = p.q_heads / p.kv_heads, tile = heads <= 8 ? 8 : 16, mtiles = (heads + tile - 1) / tile;
   const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles, fill = (int64_t)sm_count * (p.head_dim <= 128 ? 3 : 1);
   const int64_t pieces = (int64_t)p.select * (p.block / kPiece);
   int32_t splits = 1;
   while (splits < 16 && units * splits * 2 <= fill && pieces >= (int64_t)splits * 2 * kAttendWarps) splits *= 2;
-  return p.f16 ? attend_any<true>(p, splits, after_select, stream) : attend_any<false>(p, splits, after_select, stream);
+  if (tile == 8)
+    return p.f16 ? attend_any<true, 1>(p, splits, after_select, stream) : attend_any<false, 1>(p, splits, after_select, stream);
+  return p.f16 ? attend_any<true, 2>(p, splits, after_select, stream) : attend_any<false, 2>(p, splits, after_select, stream);
 }
 
 }  // namespace fi8
