@@ -148,6 +148,7 @@ struct I4ScoreArgs {
   uint32_t id_base;
   const uint64_t* keep;
   int64_t keep_nbits;
+  uint32_t ring_at;  // byte offset of the rings in shared memory
 };
 
 template <int NT, bool TOPK>
@@ -158,11 +159,9 @@ __global__ void __launch_bounds__(kWarps * 32) i4_score_kernel(I4ScoreArgs p) {
   const int G = r.groups, quads = (G + 3) >> 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int4* starts = reinterpret_cast<int4*>(smem);
   uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
-  I4Stage* ring = reinterpret_cast<I4Stage*>(smem + i4_frag_bytes<NT>(G)) + warp * kStages;
-  if (TOPK) pdl_launch_dependents();
-  i4_queries<NT>(p.q, p.M, r.dim, G, smem + i4_frag_bytes<NT>(G), starts, ops, s_scale);
-  starts += lane;
-  ops += lane;
+  I4Stage* ring = reinterpret_cast<I4Stage*>(smem + p.ring_at) + warp * kStages;
+  pdl_wait_prior();           // queries and rows may come from the kernel before
+  pdl_launch_dependents();    // after the wait: what starts early now may read the queries
 
   // the copies run kStages - 1 quads ahead of the products, over the ends of tiles
   const int64_t step = (int64_t)gridDim.x * kWarps;
@@ -185,8 +184,17 @@ __global__ void __launch_bounds__(kWarps * 32) i4_score_kernel(I4ScoreArgs p) {
       cursor.mults += 32;
     }
   };
+  // the first copies travel while the queries are quantized, unless the rings lie over that work's scratch
+  const bool early = p.ring_at > i4_frag_bytes<NT>(G);
+  if (early)
 #pragma unroll
-  for (int i = 0; i < kStages - 1; i++) fetch();
+    for (int i = 0; i < kStages - 1; i++) fetch();
+  i4_queries<NT>(p.q, p.M, r.dim, G, smem + i4_frag_bytes<NT>(G), starts, ops, s_scale);
+  starts += lane;
+  ops += lane;
+  if (!early)
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) fetch();
   for (; tile < p.tiles; tile += step) {
     // lane 4 r + t ends with rows r, r + 8, r + 16, r + 24 of the tile, queries 2t and 2t + 1
     const int64_t row0 = tile * kI4Tile;
@@ -497,20 +505,18 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
   for (int i = tid; i < p.k; i += kTopThreads) out[i] = i < have ? keys[i] : kEmptyKey;
 }
 
-// Fragments, then the queries' scratch, over which the rings lie afterwards.
-template <int NT>
-size_t score_smem(int groups) {
-  const size_t ring = sizeof(I4Stage) * kStages * kWarps, scratch = i4_query_bytes(groups, NT);
-  return i4_frag_bytes<NT>(groups) + (ring > scratch ? ring : scratch);
-}
-
 template <int NT, bool TOPK>
-cudaError_t score_launch(const I4ScoreArgs& p, int32_t sm_count, cudaStream_t stream) {
-  const size_t smem = score_smem<NT>(p.r.groups);
+cudaError_t score_launch(I4ScoreArgs p, int32_t sm_count, cudaStream_t stream) {
+  // Fragments, the queries' scratch, the rings; over the scratch where two CTAs
+  // an SM would not fit otherwise.
+  const size_t frags = i4_frag_bytes<NT>(p.r.groups), scratch = i4_query_bytes(p.r.groups, NT), ring = sizeof(I4Stage) * kStages * kWarps;
+  const size_t apart = frags + (scratch + 15) / 16 * 16 + ring;
+  const bool early = apart + 1024 <= kSmemSm / kScoreCtas;
+  p.ring_at = (uint32_t)(early ? apart - ring : frags);
+  const size_t smem = early ? apart : frags + (ring > scratch ? ring : scratch);
   const int64_t fit = (int64_t)(kSmemSm / (smem + 1024)), ctas = fit < kScoreCtas ? fit : kScoreCtas;
   const int64_t need = (p.tiles + kWarps - 1) / kWarps, most = (int64_t)sm_count * ctas;
-  i4_score_kernel<NT, TOPK><<<(unsigned)(need < most ? need : most), kWarps * 32, smem, stream>>>(p);
-  return cudaGetLastError();
+  return launch_pdl(i4_score_kernel<NT, TOPK>, dim3((unsigned)(need < most ? need : most)), dim3(kWarps * 32), smem, stream, p);
 }
 
 size_t block_smem(int groups) { return (size_t)8 * groups * 16 + (size_t)8 * ((groups + 3) / 4) * 4; }

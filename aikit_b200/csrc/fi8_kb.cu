@@ -373,8 +373,9 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
   uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
   unsigned char* scratch = smem + i4_frag_bytes<NT>(G);
   uint32_t* ord = reinterpret_cast<uint32_t*>(scratch + (((size_t)8 * NT * G * (kI4Group + 4) + 15) & ~(size_t)15));
-  pdl_launch_dependents();
   if (nranks > 1) cluster_arrive();
+  pdl_wait_prior();         // queries, lengths and block rows may come from the kernel before
+  pdl_launch_dependents();  // after the wait: the attention reads queries and lengths as it starts
   if (tid < nrows) {
     int slot;
     s_len[tid] = kb_row_at(p, row0 + tid, &slot);
@@ -921,24 +922,32 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   cluster_sync();  // the others' shared memory is read until here
 }
 
-template <int DP, int NT, bool F16, bool FULL>
-cudaError_t attend_launch(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
-  const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 8 * NT - 1) / (8 * NT);
+// A launch in clusters, as a programmatic dependent of the one before if pdl.
+template <typename... Args>
+cudaError_t launch_cluster(void (*kernel)(Args...), dim3 grid, int threads, int cluster, bool pdl, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.rows * splits), (unsigned)(p.kv_heads * mtiles));
-  cfg.blockDim = dim3(kAttendThreads);
-  cfg.dynamicSmemBytes = AttendSmem<DP, NT>::bytes(p.select);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = after_select ? 2 : 1;  // queries and lengths are read before the wait: they must not come from the kernel before
-  return cudaLaunchKernelEx(&cfg, kb_attend_kernel<DP, NT, F16, FULL>, p);
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int DP, int NT, bool F16, bool FULL>
+cudaError_t attend_launch(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
+  const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 8 * NT - 1) / (8 * NT);
+  // Queries and lengths are read before the wait for the launch before: only after a select, which waits itself.
+  return launch_cluster(kb_attend_kernel<DP, NT, F16, FULL>, dim3((unsigned)(p.rows * splits), (unsigned)(p.kv_heads * mtiles)),
+                        kAttendThreads, splits, after_select, AttendSmem<DP, NT>::bytes(p.select), stream, p);
 }
 
 template <int DP, int NT, bool F16>
@@ -989,19 +998,8 @@ namespace {
 
 template <bool F16, int NT>
 cudaError_t select_launch(const KbParams& p, const KbSelectShape& shape, int cluster, size_t smem, cudaStream_t stream) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((p.rows + shape.rt - 1) / shape.rt * cluster), (unsigned)p.kv_heads);
-  cfg.blockDim = dim3(kSelectThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kb_select_kernel<F16, NT>, p, shape);
+  return launch_cluster(kb_select_kernel<F16, NT>, dim3((unsigned)((p.rows + shape.rt - 1) / shape.rt * cluster), (unsigned)p.kv_heads),
+                        kSelectThreads, cluster, true, smem, stream, p, shape);
 }
 
 template <bool F16>
