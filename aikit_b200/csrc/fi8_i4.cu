@@ -106,12 +106,18 @@ __global__ void __launch_bounds__(kWarps * 32) i4_unpack_kernel(I4Rows r, int64_
 // multipliers: a row's 16 bytes cost the same few instructions for one query
 // as for eight, and the rows' bytes bound the kernel. The queries' fragments
 // lie in shared memory, 16 bytes a lane and group. A warp's words pass through
-// a ring of its own, kStages quads (four groups) deep, filled by asynchronous
+// a ring of its own, a few quads (four groups) deep, filled by asynchronous
 // copies; nothing but the warp itself waits for it.
 // ---------------------------------------------------------------------------
-constexpr int kStages = 4;
-constexpr int kScoreCtas = 2;              // CTAs an SM at most
-constexpr size_t kSmemSm = 228 * 1024;     // an SM's shared memory; a CTA takes 1 KB more than it asks for
+// CTAs an SM at most, and quads of a warp's ring. Up to eight queries three CTAs
+// of two quads keep the memory busy; with sixteen the products' registers leave
+// room for two (measured, CTAs x quads: 8 queries 3 x 2 208 us, 3 x 3 220, 2 x 4
+// 212 over 2M x 1024; 16 queries 2 x 4 78 us, 3 x 2 86 over 1.5M x 256).
+template <int NT>
+constexpr int kScoreCtas = NT == 1 ? 3 : 2;
+template <int NT>
+constexpr int kScoreStages = NT == 1 ? 2 : 4;
+constexpr size_t kSmemSm = 228 * 1024;  // an SM's shared memory; a CTA takes 1 KB more than it asks for
 
 // One quad of a tile: the lanes' words of four blocks of 8 rows (a tile's last
 // quad may have fewer groups, [4 blocks][groups][32 lanes] words from the start
@@ -152,13 +158,14 @@ struct I4ScoreArgs {
 };
 
 template <int NT, bool TOPK>
-__global__ void __launch_bounds__(kWarps * 32) i4_score_kernel(I4ScoreArgs p) {
+__global__ void __launch_bounds__(kWarps * 32, kScoreCtas<NT>) i4_score_kernel(I4ScoreArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float s_scale[8 * NT];
   const I4Rows& r = p.r;
   const int G = r.groups, quads = (G + 3) >> 2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int4* starts = reinterpret_cast<int4*>(smem);
   uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
+  constexpr int kStages = kScoreStages<NT>;
   I4Stage* ring = reinterpret_cast<I4Stage*>(smem + p.ring_at) + warp * kStages;
   pdl_wait_prior();           // queries and rows may come from the kernel before
   pdl_launch_dependents();    // after the wait: what starts early now may read the queries
@@ -507,14 +514,14 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
 
 template <int NT, bool TOPK>
 cudaError_t score_launch(I4ScoreArgs p, int32_t sm_count, cudaStream_t stream) {
-  // Fragments, the queries' scratch, the rings; over the scratch where two CTAs
-  // an SM would not fit otherwise.
-  const size_t frags = i4_frag_bytes<NT>(p.r.groups), scratch = i4_query_bytes(p.r.groups, NT), ring = sizeof(I4Stage) * kStages * kWarps;
+  // Fragments, the queries' scratch, the rings; over the scratch where the CTAs
+  // would not fit otherwise.
+  const size_t frags = i4_frag_bytes<NT>(p.r.groups), scratch = i4_query_bytes(p.r.groups, NT), ring = sizeof(I4Stage) * kScoreStages<NT> * kWarps;
   const size_t apart = frags + (scratch + 15) / 16 * 16 + ring;
-  const bool early = apart + 1024 <= kSmemSm / kScoreCtas;
+  const bool early = apart + 1024 <= kSmemSm / kScoreCtas<NT>;
   p.ring_at = (uint32_t)(early ? apart - ring : frags);
   const size_t smem = early ? apart : frags + (ring > scratch ? ring : scratch);
-  const int64_t fit = (int64_t)(kSmemSm / (smem + 1024)), ctas = fit < kScoreCtas ? fit : kScoreCtas;
+  const int64_t fit = (int64_t)(kSmemSm / (smem + 1024)), ctas = std::min<int64_t>(fit, kScoreCtas<NT>);
   const int64_t need = (p.tiles + kWarps - 1) / kWarps, most = (int64_t)sm_count * ctas;
   return launch_pdl(i4_score_kernel<NT, TOPK>, dim3((unsigned)(need < most ? need : most)), dim3(kWarps * 32), smem, stream, p);
 }

@@ -305,6 +305,29 @@ __device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int las
   }
 }
 
+// One row's picks of a short list, n at most the CTA's threads: a rank's place
+// is the number of larger ones, and of equal ones before it. No search, one
+// barrier.
+__device__ void kb_count_picks(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* part) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < first; i += kSelectThreads) sel[i] = i;
+  for (int i = tid; i < last; i += kSelectThreads) sel[first + need + i] = first + n + i;
+  const uint32_t mine = tid < n ? ord[tid] : 0xFFFFFFFFu;
+  uint32_t place = 0;
+  if (warp * 32 < n) {
+#pragma unroll 8
+    for (int j = 0; j < warp * 32; j++) place += ord[j] >= mine;
+    for (int j = warp * 32; j < min(n, warp * 32 + 32); j++) place += ord[j] > mine || (ord[j] == mine && j < tid);
+#pragma unroll 8
+    for (int j = warp * 32 + 32; j < n; j++) place += ord[j] > mine;
+  }
+  const uint32_t mask = __ballot_sync(0xffffffffu, tid < n && place < (uint32_t)need);
+  if (lane == 0) part[warp] = __popc(mask);
+  __syncthreads();
+  const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? part[lane] : 0u);
+  if ((mask >> lane) & 1u) sel[first + before + __popc(mask & lanemask_lt())] = first + tid;
+}
+
 // Quantize the query vectors of `columns` (row, head) pairs (LANES lanes each,
 // eight values a lane, all loads in flight together) and lay out their
 // fragments. Columns without a pair are zero.
@@ -495,6 +518,8 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
         if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
         else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
       }
+    } else if (n <= kSelectThreads) {
+      kb_count_picks(o, n, need, p.first, p.last, sel, s_kth.list);
     } else if (n < kWarpPicks) {
       kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_kth.hist, s_kth.list);
     } else {

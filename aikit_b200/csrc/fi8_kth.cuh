@@ -42,6 +42,11 @@ struct ScoreBins {
   __device__ __forceinline__ int operator()(uint32_t o) const {
     return min(max((int)((ord_to_score(o) - low) * scale), 0), last);  // a NaN converts to 0
   }
+  // A rank that none of bin b is below: half a bin under its edge, far more than
+  // the roundings.
+  __device__ __forceinline__ uint32_t below(int b) const {
+    return b > 0 ? score_to_ord(low + ((float)b - 0.5f) / scale) : 0u;
+  }
 };
 
 struct Kth {
@@ -120,10 +125,12 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
       return above + in_bin <= limit ? Kth{t, 0xFFFFFFFFu, above + in_bin} : Kth{t, need - above, need};
     }
     if (in_bin <= (uint32_t)kKthList) {
+      // ranks well below the bin are passed over without their bins
+      const uint32_t edge = chosen < 0 ? bins.below((int)bin) : t;
 #pragma unroll 4
       for (int i = tid; i < n; i += nt) {
         const uint32_t o = get(i);
-        if (chosen < 0 ? bins(o) == (int)bin : bins(o) == chosen && o >= t && ((o - t) >> shift) == 0)
+        if (o >= edge && (chosen < 0 ? bins(o) == (int)bin : bins(o) == chosen && ((o - t) >> shift) == 0))
           s->list[atomicAdd(&s->listed, 1u)] = o;
       }
       __syncthreads();
