@@ -382,8 +382,9 @@ __device__ __forceinline__ void kb_queries(const KbParams& p, int row0, int colu
   i4_fragments<NT>(G, q8, off, starts, ops);
 }
 
-template <bool F16, int NT>
-__global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, KbSelectShape shape) {
+// SHARED: rows share the CTA (shape.rt > 1).
+template <bool F16, int NT, bool SHARED>
+__global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 4 : NT == 8 ? 1 : 2) kb_select_kernel(KbParams p, KbSelectShape shape) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ KthShared s_kth;
   __shared__ float s_scale[8 * NT];
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
   else kb_queries<F16, NT, 32>(p, row0, nrows * heads, heads, h, scratch, starts, ops, s_scale);
   if (nranks > 1) cluster_wait();
   auto blocks_of = [&](int r) { return (s_len[r] + p.block - 1) / p.block; };
-  if (shape.rt > 1) {  // several columns meet in one rank
+  if (SHARED) {  // several columns meet in one rank
     for (int i = tid; i < nrows * shape.stride; i += kSelectThreads) ord[i] = 0;
     __syncthreads();
   }
@@ -461,7 +462,7 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
         }
       }
       // lane 4 r + t: blocks r, r + 8, r + 16, r + 24 of the tile, columns 2t and 2t + 1 of each eight
-      if (shape.rt == 1) {
+      if (!SHARED) {
 #pragma unroll
         for (int b = 0; b < 4; b++) {
           float best = __uint_as_float(0x7FFFFFFFu);  // a NaN loses
@@ -512,16 +513,18 @@ __global__ void __launch_bounds__(kSelectThreads) kb_select_kernel(KbParams p, K
     if (nb <= p.select) {  // every visible block
       if (r % kSelectWarps == warp)
         for (int i = lane; i < p.select; i += 32) sel[i] = i < nb ? i : -1;
-    } else if (shape.rt > 1 && n < kWarpPicks) {
-      if (r % kSelectWarps == warp) {
-        uint32_t* hist = s_kth.hist + warp * 256;
-        if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
-        else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
+    } else if (SHARED ? n < kWarpPicks : n <= kSelectThreads) {
+      if constexpr (SHARED) {
+        if (r % kSelectWarps == warp) {
+          uint32_t* hist = s_kth.hist + warp * 256;
+          if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
+          else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
+        }
+      } else {
+        kb_count_picks(o, n, need, p.first, p.last, sel, s_kth.list);
       }
-    } else if (n <= kSelectThreads) {
-      kb_count_picks(o, n, need, p.first, p.last, sel, s_kth.list);
-    } else if (n < kWarpPicks) {
-      kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_kth.hist, s_kth.list);
+    } else if (!SHARED && n < kWarpPicks) {
+      if constexpr (!SHARED) kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_kth.hist, s_kth.list);
     } else {
       __syncthreads();  // warps may be picking for rows before this one
       for (int i = tid; i < p.first; i += kSelectThreads) sel[i] = i;
@@ -1021,9 +1024,9 @@ cudaError_t kb_update_launch(const KbParams& p, const int32_t* slot, const int32
 
 namespace {
 
-template <bool F16, int NT>
+template <bool F16, int NT, bool SHARED = false>
 cudaError_t select_launch(const KbParams& p, const KbSelectShape& shape, int cluster, size_t smem, cudaStream_t stream) {
-  return launch_cluster(kb_select_kernel<F16, NT>, dim3((unsigned)((p.rows + shape.rt - 1) / shape.rt * cluster), (unsigned)p.kv_heads),
+  return launch_cluster(kb_select_kernel<F16, NT, SHARED>, dim3((unsigned)((p.rows + shape.rt - 1) / shape.rt * cluster), (unsigned)p.kv_heads),
                         kSelectThreads, cluster, true, smem, stream, p, shape);
 }
 
@@ -1032,7 +1035,9 @@ cudaError_t select_nt(int nt, const KbParams& p, const KbSelectShape& shape, int
   switch (nt) {
     case 1: return select_launch<F16, 1>(p, shape, cluster, smem, stream);
     case 2: return select_launch<F16, 2>(p, shape, cluster, smem, stream);
-    case 4: return select_launch<F16, 4>(p, shape, cluster, smem, stream);
+    case 4:
+      return shape.rt > 1 ? select_launch<F16, 4, true>(p, shape, cluster, smem, stream)
+                          : select_launch<F16, 4>(p, shape, cluster, smem, stream);
     default: return select_launch<F16, 8>(p, shape, cluster, smem, stream);
   }
 }
@@ -1046,10 +1051,11 @@ cudaError_t kb_init() {
   auto set = [&](auto fn, int bytes) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, kind, bytes);
   };
-  set(kb_select_kernel<false, 1>, most), set(kb_select_kernel<true, 1>, most);
-  set(kb_select_kernel<false, 2>, most), set(kb_select_kernel<true, 2>, most);
-  set(kb_select_kernel<false, 4>, most), set(kb_select_kernel<true, 4>, most);
-  set(kb_select_kernel<false, 8>, most), set(kb_select_kernel<true, 8>, most);
+  set(kb_select_kernel<false, 1, false>, most), set(kb_select_kernel<true, 1, false>, most);
+  set(kb_select_kernel<false, 2, false>, most), set(kb_select_kernel<true, 2, false>, most);
+  set(kb_select_kernel<false, 4, false>, most), set(kb_select_kernel<true, 4, false>, most);
+  set(kb_select_kernel<false, 8, false>, most), set(kb_select_kernel<true, 8, false>, most);
+  set(kb_select_kernel<false, 4, true>, most), set(kb_select_kernel<true, 4, true>, most);
   if (e == cudaSuccess) e = attend_init_all<1>();
   if (e == cudaSuccess) e = attend_init_all<2>();
   return e;
@@ -1071,7 +1077,7 @@ cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t s
   // every warp has a tile.
   if (shape.rt == 1)
     while (cluster < 8 && (int64_t)p.rows * p.kv_heads * cluster * 2 <= 2 * (int64_t)sm_count &&
-           blocks >= (int64_t)cluster * 2 * kSelectWarps * kI4Tile)
+           blocks >= (int64_t)cluster * 4 * kSelectWarps * kI4Tile)
       cluster *= 2;
   const size_t smem = (size_t)p.groups * nt * 32 * 24 + (((size_t)8 * nt * p.groups * (kI4Group + 4) + 15) & ~(size_t)15) +
                       (size_t)shape.rt * shape.stride * 4;
