@@ -655,11 +655,7 @@ class I4Index:
             check(lib().fi8_i4_destroy(self._h))
             self._h = None
 
-    def _queries(self, queries) -> np.ndarray:
-        Q = _f32(queries).reshape(len(queries), -1) if len(queries) else np.empty((0, self.dim), np.float32)
-        if Q.shape[1] != self.dim:
-            raise Fi8Error(1, f"gpu: batch query dim {Q.shape[1]} != index dim {self.dim}")
-        return Q
+    _queries = I8Index._queries
 
     def __del__(self):
         try:

@@ -205,13 +205,15 @@ int fi8_ctx_create(int device, fi8_ctx** out) {
   FI8_CUDA(cudaGetDeviceCount(&ndev), "cudaGetDeviceCount");
   if (device < 0 || device >= ndev) return fail(FI8_ERR_ARG, "fi8_ctx_create: device %d of %d", device, ndev);
   DeviceGuard g(device);
-  cudaDeviceProp prop;
-  FI8_CUDA(cudaGetDeviceProperties(&prop, device), "cudaGetDeviceProperties");
-  if (prop.major != 10) return fail(FI8_ERR_DECLINED, "fi8: device %d is sm_%d%d, this build targets sm_100a", device, prop.major, prop.minor);
+  int major = 0, minor = 0, sm_count = 0;  // single attributes: the whole property record takes a millisecond
+  FI8_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device), "cudaDeviceGetAttribute");
+  FI8_CUDA(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device), "cudaDeviceGetAttribute");
+  FI8_CUDA(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device), "cudaDeviceGetAttribute");
+  if (major != 10) return fail(FI8_ERR_DECLINED, "fi8: device %d is sm_%d%d, this build targets sm_100a", device, major, minor);
   fi8_ctx* c = new (std::nothrow) fi8_ctx;
   if (!c) return fail(FI8_ERR_OOM, "fi8_ctx_create: host allocation");
   c->device = device;
-  c->sm_count = prop.multiProcessorCount;
+  c->sm_count = sm_count;
   *out = c;
   return FI8_OK;
 }

@@ -1086,14 +1086,16 @@ cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t s
 
 cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, bool after_select, cudaStream_t stream) {
   // Splits of a (row, kv head): as many as still fit on the SMs at once (three
-  // CTAs each up to 128 channels, one above), while every warp has a piece; 16
-  // at most, and a power of two: clusters of other sizes pack badly (16 rows x 8
+  // CTAs each up to 128 channels, one above), while every warp has a piece; at
+  // most 16 (8 with a CTA an SM: not every part of the chip has 16 SMs side by
+  // side), and a power of two: clusters of other sizes pack badly (16 rows x 8
   // heads over 32k tokens: 37 us with 2, 47 with 3, 44 with 4, 47 with 8).
   const int heads = p.q_heads / p.kv_heads, tile = heads <= 8 ? 8 : 16, mtiles = (heads + tile - 1) / tile;
   const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles, fill = (int64_t)sm_count * (p.head_dim <= 128 ? 3 : 1);
   const int64_t pieces = (int64_t)p.select * (p.block / kPiece);
   int32_t splits = 1;
-  while (splits < 16 && units * splits * 2 <= fill && pieces >= (int64_t)splits * 2 * kAttendWarps) splits *= 2;
+  const int32_t most = p.head_dim <= 128 ? 16 : 8;
+  while (splits < most && units * splits * 2 <= fill && pieces >= (int64_t)splits * 2 * kAttendWarps) splits *= 2;
   if (tile == 8)
     return p.f16 ? attend_any<true, 1>(p, splits, after_select, stream) : attend_any<false, 1>(p, splits, after_select, stream);
   return p.f16 ? attend_any<true, 2>(p, splits, after_select, stream) : attend_any<false, 2>(p, splits, after_select, stream);

@@ -124,6 +124,10 @@ int fi8_kb_create(fi8_ctx* ctx, const fi8_kb_desc* desc, fi8_kb** out) {
   const size_t sets = (size_t)d.slots * d.kv_heads;
   const size_t codes = sets * p.tiles * p.groups * 512, mults = sets * p.tiles * ((p.groups + 3) / 4) * 128;
   const size_t scales = sets * p.tiles * kI4Tile * sizeof(float), bytes = codes + mults + scales + 16;
+  if ((double)sets * p.tiles * (p.groups * 512.0 + (p.groups + 3) / 4 * 128 + kI4Tile * 4) > 1e14) {
+    kb_free(b);
+    return fail(FI8_ERR_OOM, "fi8_kb_create: block rows of %d slots x %d heads x %d blocks", d.slots, d.kv_heads, p.max_blocks);
+  }
   DeviceGuard g(b->device);
   unsigned char* base = nullptr;
   cudaError_t e = kb_init();

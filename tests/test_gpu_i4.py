@@ -44,6 +44,60 @@ def test_rows_and_scores(backend, n, dim):
     iy.Close()
 
 
+@pytest.mark.parametrize("dim,M", [(1537, 16), (3000, 16), (3100, 16), (2000, 9), (64, 16), (130, 12)])
+def test_wide_batches(backend, dim, M):
+    """Batches that share a pass at dimensions around its limits."""
+    n = 333
+    v, q = rows(n, dim, dim), rows(M, dim, 5)
+    ix = backend.NewI4IndexFromFloats(v)
+    dst = np.full(M * n, np.nan, np.float32)
+    ix.ScoreBatch(q, dst)
+    want = i4_util.scores(*i4_util.quantize(v), q)
+    same(dst.reshape(M, n), want)
+    wi, ws = i4_util.topk(want, 21)
+    idx, sc = ix.topk_arrays(q, 21)
+    np.testing.assert_array_equal(idx, wi)
+    same(sc, ws)
+    ix.Close()
+
+
+def test_set_rows_in_parts(backend):
+    """Rows set in pieces that start and end inside the device's groups of rows."""
+    import torch
+    n, dim = 117, 45
+    v = rows(n, dim, 9)
+    dv = torch.from_numpy(v).cuda()
+    ix = backend.NewI4IndexEmpty(n, dim)
+    for a, b in ((3, 4), (60, 117), (4, 41), (41, 60), (0, 3)):
+        ix.set_rows_async(a, dv[a:b].data_ptr(), b - a)
+    for got, want in zip(ix.read_rows(), i4_util.quantize(v)):
+        np.testing.assert_array_equal(got, want)
+    ix.set_rows_async(10, dv[50:].data_ptr(), 5)
+    v[10:15] = v[50:55]
+    for got, want in zip(ix.read_rows(), i4_util.quantize(v)):
+        np.testing.assert_array_equal(got, want)
+    ix.Close()
+
+
+@pytest.mark.parametrize("k", [1, 100, 2048])
+def test_infinite_and_few_scores(backend, k):
+    """Scores of both infinities, of two values, and of which nearly all are NaN."""
+    n = 70_000
+    codes, mults, _ = i4_util.quantize(np.ones((n, 32), np.float32))
+    q = np.ones((2, 32), np.float32)
+    q[1] = -1
+    rng = np.random.default_rng(k)
+    for scales in (np.where(rng.random(n) < 0.01, np.inf, rng.standard_normal(n)), np.where(rng.random(n) < 0.001, 2.0, -1.0),
+                   np.where(rng.random(n) < 0.999, np.nan, 1.0), np.full(n, np.nan), rng.standard_normal(n) * 1e-38):
+        scales = scales.astype(np.float32)
+        ix = backend.NewI4Index(codes, mults, scales, n, 32)
+        wi, ws = i4_util.topk(i4_util.scores(codes, mults, scales, q), k)
+        idx, sc = ix.topk_arrays(q, k)
+        np.testing.assert_array_equal(idx, wi)
+        same(sc, ws)
+        ix.Close()
+
+
 def test_odd_rows_and_queries(backend):
     """Zero, NaN, infinite, tiny and huge rows and queries; every nibble and multiplier."""
     v = rows(40, 70, 1)

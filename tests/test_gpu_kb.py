@@ -171,6 +171,17 @@ def test_many_blocks_and_ties(backend):
     c.kb.Close()
 
 
+@pytest.mark.parametrize("D,block,k", [(256, 128, 64), (128, 64, 128), (64, 16, 1024), (80, 128, 300)])
+def test_one_row_and_many_blocks(backend, D, block, k):
+    """One row's blocks split over as many CTAs as there can be."""
+    n = block * (k + 20) + 3
+    c = Cache(backend, q_heads=2, kv_heads=1, D=D, block=block, capacity=n, lens=[n], seed=D, max_select=1024)
+    c.update_all()
+    c.check(c.queries(1), [0], [n], k)
+    c.check(c.queries(1), [0], [n - block * 19], k)
+    c.kb.Close()
+
+
 def test_large_and_small_scores(backend):
     """Scores far apart (one token takes all the weight) and a scale of 0, a negative one."""
     c = Cache(backend, q_heads=8, kv_heads=2, D=128, block=64, capacity=700, lens=[700], seed=3)
