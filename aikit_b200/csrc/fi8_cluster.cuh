@@ -36,6 +36,12 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t rank, uin
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
+__device__ __forceinline__ uint32_t atom_cluster_add(uint32_t addr, uint32_t rank, uint32_t v) {
+  uint32_t a, old;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(a), "r"(v) : "memory");
+  return old;
+}
 __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
   return __uint_as_float(ld_cluster_u32(addr, rank));
 }

@@ -290,10 +290,16 @@ __global__ void __launch_bounds__(kWarps * 32, kScoreCtas<NT>) i4_score_kernel(I
 // The same holds for runs of tiles: the k best runs hold the k best tiles. So
 // a cluster per query reduces the tiles' ranks to runs (all its CTAs), the CTA
 // of rank 0 picks the runs and then the tiles, all CTAs score the tiles' rows,
-// and rank 0 sorts what is left. Few tiles need no runs.
+// and rank 0 sorts what is left. Few tiles need no runs; and where few of few
+// tiles are picked, a CTA alone does it all, without a cluster's meetings.
+// Bound by the latency of its dependent steps, not by bytes or operations: it
+// ends 7 us after the score pass over 100,384 rows of 384 values, k = 10 (a
+// cluster: 10 us), and 20 us to 30 us after it over 4M rows, k = 100.
 // ---------------------------------------------------------------------------
-constexpr int kTopThreads = 512;
+constexpr int kTopThreads = 512;  // of a CTA of a cluster
 constexpr int kTopCluster = 8;
+constexpr int kTopAlone = 1024;   // of a CTA that works alone: at most kTopDirect tiles, of which kTopAlonePicks are scored
+constexpr int kTopAlonePicks = 64;
 constexpr int kTopSort = 4096;        // keys that a sort takes: two lists of the largest k
 constexpr int kTopHeld = 48 * 1024;   // ranks that rank 0 can hold in shared memory (more are read again in each step)
 constexpr int kTopDirect = 8 * 1024;  // tiles that it picks from without runs
@@ -316,20 +322,26 @@ struct I4SelectArgs {
   int held;  // ranks held in shared memory
 };
 
-__global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) {
+template <int THREADS, bool CLUSTER>
+__global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ KthShared s_kth;
   __shared__ float s_scale;
   __shared__ uint32_t s_count, s_floor, s_picks;
+  __shared__ uint32_t s_list[CLUSTER ? 1 : kTopAlonePicks];
   const I4Rows& r = p.r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, y = blockIdx.y, G = r.groups;
-  const uint32_t rank = cluster_rank(), nranks = cluster_size();
+  const uint32_t rank = CLUSTER ? cluster_rank() : 0, nranks = CLUSTER ? cluster_size() : 1;
+  auto sync = [] {
+    if (CLUSTER) cluster_sync();
+    else __syncthreads();
+  };
   int8_t* q8 = reinterpret_cast<int8_t*>(smem);             // [G * 32]
   int* off = reinterpret_cast<int*>(q8 + G * kI4Group);     // [G], 16-byte aligned
   // the runs' or tiles' ranks, later the sort's keys
   uint32_t* held = reinterpret_cast<uint32_t*>(smem + ((G * (kI4Group + 4) + 15) & ~15));
   uint32_t* s_runs = held + p.held;  // [i4_picks(kI4MaxK)]
-  if (p.run) cluster_arrive();
+  if (CLUSTER && p.run) cluster_arrive();
   __syncwarp();
   if (warp == 0) {
     const float* q = p.q + (size_t)y * r.dim;
@@ -340,12 +352,12 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
   pdl_wait_prior();  // the tiles' ranks
   const uint32_t* best = p.best + (size_t)y * p.best_ld;
   const int runs = p.run ? (int)((p.tiles + p.run - 1) / p.run) : 0;
-  if (p.run) {
+  if (CLUSTER && p.run) {
     // a few lanes reduce a run; the first of them writes to rank 0
     cluster_wait();
     const int lanes = min(8, p.run >> 2), per = p.run / (4 * lanes), sub = tid & (lanes - 1);
-    const int step = (int)nranks * (kTopThreads / lanes);
-    for (int base = (int)rank * (kTopThreads / lanes) + tid / lanes; base - tid / lanes < runs; base += 4 * step) {
+    const int step = (int)nranks * (THREADS / lanes);
+    for (int base = (int)rank * (THREADS / lanes) + tid / lanes; base - tid / lanes < runs; base += 4 * step) {
       uint32_t top[4] = {0, 0, 0, 0};
       for (int i = 0; i < per; i++) {
         uint4 v[4];
@@ -367,13 +379,21 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
     cluster_sync();
   }
   const uint32_t need = (uint32_t)min((int64_t)p.k, p.tiles);
-  uint32_t* list = p.list + (size_t)y * i4_picks(kI4MaxK);
+  uint32_t* list = CLUSTER ? p.list + (size_t)y * i4_picks(kI4MaxK) : s_list;
   if (rank == 0) {
-    Kth kth;
-    if (p.run) {
-      const uint32_t picks = (uint32_t)min(p.k, runs);
+    uint32_t picks, t;
+    // in any order where no tie is left out
+    auto choose = [&](auto get, int n, auto put) {
+      const Kth kth = kth_rank(get, n, need, (uint32_t)i4_picks((int)need), &s_kth);
+      if (kth.unordered()) kth_list(get, n, kth, &s_kth, put);
+      else kth_place(get, n, kth, &s_kth, put);
+      picks = kth.count;
+      t = kth.t;
+    };
+    if (CLUSTER && p.run) {
+      const uint32_t best_runs = (uint32_t)min(p.k, runs);
       auto get_run = [&](int i) { return held[i]; };
-      kth = kth_rank(get_run, runs, picks, min((uint32_t)i4_picks((int)picks), (uint32_t)p.held / p.run), &s_kth);
+      const Kth kth = kth_rank(get_run, runs, best_runs, min((uint32_t)i4_picks((int)best_runs), (uint32_t)p.held / p.run), &s_kth);
       kth_place(get_run, runs, kth, &s_kth, [&](uint32_t at, int i) { s_runs[at] = (uint32_t)i; });
       const int n = (int)kth.count * p.run, shift = __ffs(p.run) - 1;
       auto tile_of = [&](int i) { return (int64_t)s_runs[i >> shift] * p.run + (i & (p.run - 1)); };
@@ -383,51 +403,50 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
       };
       const bool fits = n <= p.held;
       if (fits) {
-        for (int i0 = tid; i0 < n; i0 += 8 * kTopThreads) {  // eight loads in flight
+        for (int i0 = tid; i0 < n; i0 += 8 * THREADS) {  // eight loads in flight
           uint32_t v[8];
 #pragma unroll
-          for (int u = 0; u < 8; u++) v[u] = i0 + u * kTopThreads < n ? rank_of(i0 + u * kTopThreads) : 0u;
+          for (int u = 0; u < 8; u++) v[u] = i0 + u * THREADS < n ? rank_of(i0 + u * THREADS) : 0u;
 #pragma unroll
           for (int u = 0; u < 8; u++)
-            if (i0 + u * kTopThreads < n) held[i0 + u * kTopThreads] = v[u];
+            if (i0 + u * THREADS < n) held[i0 + u * THREADS] = v[u];
         }
         __syncthreads();
       }
       auto get = [&](int i) { return fits ? held[i] : rank_of(i); };
-      kth = kth_rank(get, n, need, (uint32_t)i4_picks((int)need), &s_kth);
-      kth_place(get, n, kth, &s_kth, [&](uint32_t at, int i) { list[at] = (uint32_t)tile_of(i); });
+      choose(get, n, [&](uint32_t at, int i) { list[at] = (uint32_t)tile_of(i); });
     } else {
       const int n = (int)p.tiles;
-      for (int i0 = tid * 4; i0 < n; i0 += 4 * kTopThreads * 4) {  // four loads in flight
+      for (int i0 = tid * 4; i0 < n; i0 += 4 * THREADS * 4) {  // four loads in flight
         uint4 v[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-          const int i = i0 + u * kTopThreads * 4;
+          const int i = i0 + u * THREADS * 4;
           v[u] = i < n ? __ldcg(reinterpret_cast<const uint4*>(best + i)) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int u = 0; u < 4; u++)
-          if (i0 + u * kTopThreads * 4 < n) *reinterpret_cast<uint4*>(held + i0 + u * kTopThreads * 4) = v[u];
+          if (i0 + u * THREADS * 4 < n) *reinterpret_cast<uint4*>(held + i0 + u * THREADS * 4) = v[u];
       }
       __syncthreads();
       auto get = [&](int i) { return held[i]; };
-      kth = kth_rank(get, n, need, (uint32_t)i4_picks((int)need), &s_kth);
-      kth_place(get, n, kth, &s_kth, [&](uint32_t at, int i) { list[at] = (uint32_t)i; });
+      choose(get, n, [&](uint32_t at, int i) { list[at] = (uint32_t)i; });
     }
     if (tid == 0) {
-      s_floor = need == (uint32_t)p.k ? kth.t : 0u;  // fewer tiles than k offer every row
-      s_picks = kth.count;
+      s_floor = need == (uint32_t)p.k ? t : 0u;  // fewer tiles than k offer every row
+      s_picks = picks;
     }
   }
-  cluster_sync();  // the list is complete
-  const uint32_t floor = ld_cluster_u32(smem_u32(&s_floor), 0), picks = ld_cluster_u32(smem_u32(&s_picks), 0);
+  sync();  // the list is complete
+  const uint32_t floor = CLUSTER ? ld_cluster_u32(smem_u32(&s_floor), 0) : s_floor;
+  const uint32_t picks = CLUSTER ? ld_cluster_u32(smem_u32(&s_picks), 0) : s_picks;
 
   // a warp per tile; lane 4 r + t has word t of rows r, r + 8, r + 16, r + 24
   const uint32_t count_at = smem_u32(&s_count);
   uint64_t* cand = p.cand + (size_t)y * p.cand_cap;
   const int quads = (G + 3) / 4, t = lane & 3;
-  for (uint32_t i = rank * (kTopThreads / 32) + warp; i < picks; i += nranks * (kTopThreads / 32)) {
-    const int64_t tile = __ldcg(list + i), row = tile * kI4Tile + t * 8 + (lane >> 2);
+  for (uint32_t i = rank * (THREADS / 32) + warp; i < picks; i += nranks * (THREADS / 32)) {
+    const int64_t tile = CLUSTER ? __ldcg(list + i) : list[i], row = tile * kI4Tile + t * 8 + (lane >> 2);
     if (tile >= p.tiles) continue;  // behind the last run's tiles, picked where nothing better was left
     const uint32_t* codes = r.codes + (size_t)tile * G * 128 + lane * 4;
     const uint32_t* mults = r.mults + (size_t)tile * quads * 32 + (lane >> 2);
@@ -470,21 +489,19 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
     if (mask) {
       uint32_t base = 0;
       if (lane == 0) {
-        uint32_t a;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(count_at));
-        asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(base) : "r"(a), "r"((uint32_t)__popc(mask)) : "memory");
+        base = CLUSTER ? atom_cluster_add(count_at, 0, (uint32_t)__popc(mask)) : atomicAdd(&s_count, (uint32_t)__popc(mask));
       }
       base = __shfl_sync(0xffffffffu, base, 0);
       if (ok) cand[base + __popc(mask & lanemask_lt())] = make_key(s, (uint32_t)id);
     }
   }
-  cluster_sync();  // the candidates are complete; no CTA reads another's shared memory after this
+  sync();  // the candidates are complete; no CTA reads another's shared memory after this
   if (rank != 0) return;
 
   uint64_t* keys = reinterpret_cast<uint64_t*>(held);
   uint64_t* out = p.out + (size_t)y * p.k;
   const int total = (int)s_count;
-  if (total <= kTopThreads) {
+  if (total <= THREADS) {
     // one key a thread: its place is the number of larger keys
     const uint64_t mine = tid < total ? __ldcg(cand + tid) : kEmptyKey;
     keys[tid] = mine;
@@ -493,7 +510,7 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
 #pragma unroll 8
     for (int i = 0; i < total; i++) place += keys[i] > mine;
     if (tid < total && place < p.k) out[place] = mine;
-    for (int i = total + tid; i < p.k; i += kTopThreads) out[i] = kEmptyKey;
+    for (int i = total + tid; i < p.k; i += THREADS) out[i] = kEmptyKey;
     return;
   }
   // sort what there is, at most kTopSort keys at a time behind the best k so far
@@ -502,14 +519,14 @@ __global__ void __launch_bounds__(kTopThreads) i4_select_kernel(I4SelectArgs p) 
     const int take = min(total - at, kTopSort - have);
     int n2 = 2;
     while (n2 < have + take) n2 <<= 1;
-    for (int i = tid; i < n2 - have; i += kTopThreads) keys[have + i] = i < take ? __ldcg(cand + at + i) : kEmptyKey;
+    for (int i = tid; i < n2 - have; i += THREADS) keys[have + i] = i < take ? __ldcg(cand + at + i) : kEmptyKey;
     __syncthreads();
     bitonic_sort_desc(keys, n2);
     at += take;
     have = min(have + take, p.k);
     if (at >= total) break;
   }
-  for (int i = tid; i < p.k; i += kTopThreads) out[i] = i < have ? keys[i] : kEmptyKey;
+  for (int i = tid; i < p.k; i += THREADS) out[i] = i < have ? keys[i] : kEmptyKey;
 }
 
 template <int NT, bool TOPK>
@@ -538,7 +555,10 @@ cudaError_t i4_init() {
   if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<2, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_score_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 12 * 1024);
+  const int beside = 227 * 1024 - 12 * 1024;  // beside the select kernels' static shared memory
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(i4_select_kernel<kTopThreads, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, beside);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(i4_select_kernel<kTopAlone, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, beside);
   return e;
 }
 
@@ -618,6 +638,10 @@ cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, c
   if (s.run) held = std::max<int64_t>(held, std::min<int64_t>((int64_t)i4_picks(p.k) * s.run, kTopHeld));
   s.held = (int)std::max<int64_t>(held, kTopSort * 2);
   const size_t smem = (((size_t)r.groups * (kI4Group + 4) + 15) & ~(size_t)15) + ((size_t)s.held + (s.run ? i4_picks(p.k) : 0)) * 4;
+  if (!s.run && i4_picks(p.k) <= kTopAlonePicks) {
+    // few tiles to look at: their rows are scored before a cluster would have met
+    return launch_pdl(i4_select_kernel<kTopAlone, false>, dim3(1, (unsigned)p.M), dim3(kTopAlone), smem, stream, s);
+  }
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = kTopCluster;
@@ -632,7 +656,7 @@ cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, c
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, i4_select_kernel, s);
+  return cudaLaunchKernelEx(&cfg, i4_select_kernel<kTopThreads, true>, s);
 }
 
 }  // namespace fi8

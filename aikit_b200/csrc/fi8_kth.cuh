@@ -49,10 +49,17 @@ struct ScoreBins {
   }
 };
 
+// The picks: ranks in bin `bin` or above, or, with bin < 0, the ranks above t and
+// the first `ties` ranks equal to t.
 struct Kth {
-  uint32_t t;      // picks are the ranks above t and the first `ties` ranks equal to t
+  uint32_t t;  // with a bin, a rank that no pick is below
   uint32_t ties;
   uint32_t count;  // picks
+  int bin;
+  ScoreBins bins;
+  __device__ __forceinline__ bool above(uint32_t o) const { return bin < 0 ? o > t : o >= t && bins(o) >= bin; }
+  __device__ __forceinline__ bool equal(uint32_t o) const { return bin < 0 && o == t; }
+  __device__ __forceinline__ bool unordered() const { return bin >= 0 || ties == 0xFFFFFFFFu; }  // no tie is left out
 };
 
 // need in [1, n]: between need and limit picks, or, where no threshold gives
@@ -76,8 +83,8 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
   __syncthreads();
   top = __reduce_max_sync(0xffffffffu, lane < warps ? s->warp_a[lane] : 0u);
   low = __reduce_min_sync(0xffffffffu, lane < warps ? s->warp_b[lane] : 0xFFFFFFFFu) + 1u;
-  if ((uint32_t)n <= limit) return Kth{0u, 0xFFFFFFFFu, (uint32_t)n};
   const ScoreBins bins(ord_to_score(low), ord_to_score(top), kKthBins);
+  if ((uint32_t)n <= limit) return Kth{0u, 0xFFFFFFFFu, (uint32_t)n, -1, bins};
   int chosen = -1;  // the bin that the ranks are searched in; -1: none yet
   uint32_t base = 0, above = 0;  // in the bin: ranks from base + 2^bits on are all picks, `above` in all
   int bits = 32;
@@ -120,9 +127,10 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
     const uint32_t bin = s->bin, in_bin = s->in_bin;
     above = s->above;
     const uint32_t t = chosen < 0 ? 0u : base + (bin << shift);
-    if (chosen >= 0 && (above + in_bin <= limit || shift == 0)) {
+    if (above + in_bin <= limit || (chosen >= 0 && shift == 0)) {
       __syncthreads();  // the shared memory may be used again
-      return above + in_bin <= limit ? Kth{t, 0xFFFFFFFFu, above + in_bin} : Kth{t, need - above, need};
+      if (chosen < 0) return Kth{bins.below((int)bin), 0xFFFFFFFFu, above + in_bin, (int)bin, bins};
+      return above + in_bin <= limit ? Kth{t, 0xFFFFFFFFu, above + in_bin, -1, bins} : Kth{t, need - above, need, -1, bins};
     }
     if (in_bin <= (uint32_t)kKthList) {
       // ranks well below the bin are passed over without their bins
@@ -142,9 +150,7 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
           gt += s->list[i] > mine;
           eq += s->list[i] == mine;
         }
-        // the smallest rank of the bin, when the whole bin may be taken; else the need-th
-        const bool all = above + in_bin <= limit;
-        if (all ? gt + eq == above + in_bin : gt < need && gt + eq >= need) {  // equal ranks write the same
+        if (gt < need && gt + eq >= need) {  // equal ranks write the same
           s->bin = mine;
           s->above = gt;
           s->in_bin = eq;
@@ -152,7 +158,7 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
       }
       __syncthreads();
       const uint32_t count = s->above + s->in_bin;
-      const Kth k = count <= limit ? Kth{s->bin, 0xFFFFFFFFu, count} : Kth{s->bin, need - s->above, need};
+      const Kth k = count <= limit ? Kth{s->bin, 0xFFFFFFFFu, count, -1, bins} : Kth{s->bin, need - s->above, need, -1, bins};
       __syncthreads();
       return k;
     }
@@ -167,18 +173,17 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
   }
 }
 
-// Calls put(position, i) for the picks, in index order. With all ties taken, t
-// is a lower bound: the picks are the ranks from t on.
+// Calls put(position, i) for the picks, in index order.
 template <typename Get, typename Put>
 __device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int seg = (n + warps * 32 - 1) / (warps * 32) * 32, i0 = min(n, warp * seg), i1 = min(n, i0 + seg);
   uint32_t gt = 0, eq = 0;
-#pragma unroll 8
+#pragma unroll 4
   for (int i = i0 + lane; i < i1; i += 32) {
     const uint32_t o = get(i);
-    gt += o > k.t;
-    eq += o == k.t;
+    gt += k.above(o);
+    eq += k.equal(o);
   }
   gt = __reduce_add_sync(0xffffffffu, gt);
   eq = __reduce_add_sync(0xffffffffu, eq);
@@ -188,20 +193,36 @@ __device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
   gt = __reduce_add_sync(0xffffffffu, lane < warp ? s->warp_a[lane] : 0u);
   eq = __reduce_add_sync(0xffffffffu, lane < warp ? s->warp_b[lane] : 0u);
   for (int base = any ? i0 : i1; base < i1; base += 128) {
-    uint32_t o[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) o[u] = base + 32 * u + lane < i1 ? get(base + 32 * u + lane) : 0u;
+    bool is_gt[4], is_eq[4];
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       const int i = base + 32 * u + lane;
-      const bool is_gt = i < i1 && o[u] > k.t, is_eq = i < i1 && o[u] == k.t;
-      const uint32_t mgt = __ballot_sync(0xffffffffu, is_gt), meq = __ballot_sync(0xffffffffu, is_eq);
-      if ((mgt | meq) == 0) continue;
+      const uint32_t o = i < i1 ? get(i) : 0u;
+      is_gt[u] = i < i1 && k.above(o);
+      is_eq[u] = i < i1 && k.equal(o);
+    }
+    if (!__any_sync(0xffffffffu, is_gt[0] || is_eq[0] || is_gt[1] || is_eq[1] || is_gt[2] || is_eq[2] || is_gt[3] || is_eq[3])) continue;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const uint32_t mgt = __ballot_sync(0xffffffffu, is_gt[u]), meq = __ballot_sync(0xffffffffu, is_eq[u]);
       const uint32_t my_gt = gt + __popc(mgt & lanemask_lt()), my_eq = eq + __popc(meq & lanemask_lt());
-      if (is_gt || (is_eq && my_eq < k.ties)) put(my_gt + min(my_eq, k.ties), i);
+      if (is_gt[u] || (is_eq[u] && my_eq < k.ties)) put(my_gt + min(my_eq, k.ties), base + 32 * u + lane);
       gt += __popc(mgt);
       eq += __popc(meq);
     }
+  }
+  __syncthreads();
+}
+
+// The same in any order, where no tie is left out.
+template <typename Get, typename Put>
+__device__ void kth_list(Get get, int n, const Kth& k, KthShared* s, Put put) {
+  if (threadIdx.x == 0) s->listed = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const uint32_t o = get(i);
+    if (k.above(o) || k.equal(o)) put(atomicAdd(&s->listed, 1u), i);
   }
   __syncthreads();
 }

@@ -98,6 +98,26 @@ def test_infinite_and_few_scores(backend, k):
         ix.Close()
 
 
+@pytest.mark.parametrize("n", [262_144, 262_145])
+@pytest.mark.parametrize("k", [1, 50, 51])
+def test_close_scores(backend, n, k):
+    """Scores some roundings apart, equal but for a few, and tied at the last place, at the sizes where the selection changes its form."""
+    codes, mults, _ = i4_util.quantize(np.ones((n, 64), np.float32))
+    q = np.ones((1, 64), np.float32)
+    rng = np.random.default_rng(n + k)
+    some = rng.permutation(n)[: k + 40]
+    few = np.ones(n)
+    few[some] = 1 + np.arange(k + 40) // 2 * 2.0**-20
+    for scales in (1 + rng.integers(0, 64, n) * 2.0**-23, -1 - rng.integers(0, 9000, n) * 2.0**-23, few, np.where(few > 1, 5.0, -few)):
+        scales = scales.astype(np.float32)
+        ix = backend.NewI4Index(codes, mults, scales, n, 64)
+        wi, ws = i4_util.topk(i4_util.scores(codes, mults, scales, q), k)
+        idx, sc = ix.topk_arrays(q, k)
+        np.testing.assert_array_equal(idx, wi)
+        same(sc, ws)
+        ix.Close()
+
+
 def test_odd_rows_and_queries(backend):
     """Zero, NaN, infinite, tiny and huge rows and queries; every nibble and multiplier."""
     v = rows(40, 70, 1)
