@@ -77,9 +77,10 @@ __device__ __forceinline__ float kb_score(int dot, float qscale, float rowscale)
 // Block rows. The mean of a full block's keys, per channel. The sum is taken
 // in 64 bits: the values have at most 11 significant bits, so it is exact in
 // any order (f16 always; bf16 unless values of one channel differ by 2^38),
-// and the row has one value. Bound by the keys' bytes.
-// A CTA per (block, head, entry); a thread holds 8 channels of one token in a
-// few.
+// and the row has one value. A CTA per (block, head, entry); a thread adds 8
+// channels of one token in a few. 17 us for the 256 new blocks of a 16,384-token
+// prompt, 8 heads of 128 (33 MB, 2 TB/s): bound by the latency of a CTA's few
+// loads and barriers, beside the keys' bytes.
 // ---------------------------------------------------------------------------
 constexpr int kUpdateThreads = 256;
 
@@ -159,6 +160,9 @@ __global__ void __launch_bounds__(kUpdateThreads) kb_update_kernel(KbParams p, c
 // once. The ranks lie in shared memory. Up to 1023 blocks are picked from registers,
 // by a warp a row or by the CTA for its one row; more by the CTA. With one row a CTA
 // and very many blocks, a cluster scores them and its rank 0 picks.
+// Bound by the latency of its steps: 5 us for one row over 64 blocks a head (two
+// thirds of it launch and quantization), 9 us for sixteen rows over 512, 19 us for two over
+// 7,813, 90 us for 2,048 rows over 256 (there by the warps' picks and the rank's updates).
 // ---------------------------------------------------------------------------
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
