@@ -307,6 +307,7 @@ constexpr int kTopAlonePicks = 64;
 constexpr int kTopSort = 4096;        // keys that a sort takes: two lists of the largest k
 constexpr int kTopHeld = 48 * 1024;   // ranks that rank 0 can hold in shared memory (more are read again in each step)
 constexpr int kTopDirect = 8 * 1024;  // tiles that it picks from without runs
+static_assert(kTopAlonePicks * kI4Tile <= kTopSort, "one sort, in place, of a lone CTA's candidates");
 
 struct I4SelectArgs {
   I4Rows r;
@@ -447,7 +448,8 @@ __global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
 
   // a warp per tile; lane 4 r + t has word t of rows r, r + 8, r + 16, r + 24
   const uint32_t count_at = smem_u32(&s_count);
-  uint64_t* cand = p.cand + (size_t)y * p.cand_cap;
+  // a CTA alone keeps its candidates where the ranks were
+  uint64_t* cand = CLUSTER ? p.cand + (size_t)y * p.cand_cap : reinterpret_cast<uint64_t*>(held);
   const int quads = (G + 3) / 4, t = lane & 3;
   for (uint32_t i = rank * (THREADS / 32) + warp; i < picks; i += nranks * (THREADS / 32)) {
     const int64_t tile = CLUSTER ? __ldcg(list + i) : list[i], row = tile * kI4Tile + t * 8 + (lane >> 2);
@@ -507,9 +509,11 @@ __global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
   const int total = (int)s_count;
   if (total <= THREADS) {
     // one key a thread: its place is the number of larger keys
-    const uint64_t mine = tid < total ? __ldcg(cand + tid) : kEmptyKey;
-    keys[tid] = mine;
-    __syncthreads();
+    const uint64_t mine = tid < total ? CLUSTER ? __ldcg(cand + tid) : cand[tid] : kEmptyKey;
+    if (CLUSTER) {
+      keys[tid] = mine;
+      __syncthreads();
+    }
     int place = 0;
 #pragma unroll 8
     for (int i = 0; i < total; i++) place += keys[i] > mine;
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
     const int take = min(total - at, kTopSort - have);
     int n2 = 2;
     while (n2 < have + take) n2 <<= 1;
-    for (int i = tid; i < n2 - have; i += THREADS) keys[have + i] = i < take ? __ldcg(cand + at + i) : kEmptyKey;
+    for (int i = tid; i < n2 - have; i += THREADS) keys[have + i] = i < take ? CLUSTER ? __ldcg(cand + at + i) : cand[at + i] : kEmptyKey;
     __syncthreads();
     bitonic_sort_desc(keys, n2);
     at += take;
