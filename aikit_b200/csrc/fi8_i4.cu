@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
     // in any order where no tie is left out
     auto choose = [&](auto get, int n, auto put) {
       const Kth kth = kth_rank(get, n, need, (uint32_t)i4_picks((int)need), &s_kth);
-      if (kth.unordered()) kth_list(get, n, kth, &s_kth, put);
+      if (kth.ties == 0xFFFFFFFFu) kth_list(get, n, kth, &s_kth, put);
       else kth_place(get, n, kth, &s_kth, put);
       picks = kth.count;
       t = kth.t;

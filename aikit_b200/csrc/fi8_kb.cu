@@ -168,11 +168,6 @@ constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kWarpPicks = 1024;  // a warp picks from fewer blocks
 
-struct KbSelectShape {
-  int rt;      // query rows of a CTA
-  int stride;  // ranks held for a row
-};
-
 // One row's picks by a warp (WARPS = 1) or by the CTA's WARPS warps: ranks ord
 // [0 .. n) of the inner blocks, n <= 32 E WARPS and below 1024; `need` of them,
 // behind `first` and before `last` blocks that are always in. As kth_rank does,
@@ -214,9 +209,12 @@ __device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int las
   for (int e = 0; e < E; e++)
     if (base + e * 32 + lane < n) atomicAdd(hist + bins(v[e]), 1u);
   sync();
-  uint32_t mine = 0;
+  uint32_t c8[8], mine = 0;  // the highest first
+  const uint4* at = reinterpret_cast<const uint4*>(hist + 248 - lane * 8);
+  const uint4 lo = at[0], hi = at[1];
+  c8[0] = hi.w, c8[1] = hi.z, c8[2] = hi.y, c8[3] = hi.x, c8[4] = lo.w, c8[5] = lo.z, c8[6] = lo.y, c8[7] = lo.x;
 #pragma unroll
-  for (int i = 0; i < 8; i++) mine += hist[255 - lane * 8 - i];
+  for (int i = 0; i < 8; i++) mine += c8[i];
   uint32_t before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -227,11 +225,15 @@ __device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int las
   const bool here = before < (uint32_t)need && before + mine >= (uint32_t)need;
   uint32_t bin = 0, count = 0;
   if (here) {
+    bool found = false;
+#pragma unroll
     for (int i = 0; i < 8; i++) {
-      bin = (uint32_t)(255 - lane * 8 - i);
-      count = before + hist[bin];
-      if (count >= (uint32_t)need) break;
-      before = count;
+      if (!found) {
+        bin = (uint32_t)(255 - lane * 8 - i);
+        count = before + c8[i];
+        found = count >= (uint32_t)need;
+        if (!found) before = count;
+      }
     }
   }
   const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
@@ -311,33 +313,54 @@ __device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int las
 
 // One row's picks of a short list, n at most the CTA's threads: a rank's place
 // is the number of larger ones, and of equal ones before it. No search, one
-// barrier.
+// barrier. ord is 16-byte aligned and 0 from n to a multiple of 32. (Eight wide
+// loads at a time: rolled loops over single ranks took four times as long.)
 __device__ void kb_count_picks(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* part) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < first; i += kSelectThreads) sel[i] = i;
-  for (int i = tid; i < last; i += kSelectThreads) sel[first + need + i] = first + n + i;
-  const uint32_t mine = tid < n ? ord[tid] : 0xFFFFFFFFu;
   uint32_t place = 0;
   if (warp * 32 < n) {
-#pragma unroll 8
-    for (int j = 0; j < warp * 32; j++) place += ord[j] >= mine;
-    for (int j = warp * 32; j < min(n, warp * 32 + 32); j++) place += ord[j] > mine || (ord[j] == mine && j < tid);
-#pragma unroll 8
-    for (int j = warp * 32 + 32; j < n; j++) place += ord[j] > mine;
+    const uint32_t mine = ord[tid];
+#pragma unroll 1
+    for (int b = 0; b * 32 < n; b++) {
+      uint4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = reinterpret_cast<const uint4*>(ord + b * 32)[j];
+      if (b == warp) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          place += (v[j].x >= mine + (4 * j >= lane)) + (v[j].y >= mine + (4 * j + 1 >= lane)) + (v[j].z >= mine + (4 * j + 2 >= lane)) +
+                   (v[j].w >= mine + (4 * j + 3 >= lane));
+      } else {
+        const uint32_t least = mine + (b > warp);  // a rank is never the largest 32-bit number
+#pragma unroll
+        for (int j = 0; j < 8; j++) place += (v[j].x >= least) + (v[j].y >= least) + (v[j].z >= least) + (v[j].w >= least);
+      }
+    }
   }
   const uint32_t mask = __ballot_sync(0xffffffffu, tid < n && place < (uint32_t)need);
   if (lane == 0) part[warp] = __popc(mask);
   __syncthreads();
   const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? part[lane] : 0u);
   if ((mask >> lane) & 1u) sel[first + before + __popc(mask & lanemask_lt())] = first + tid;
+  for (int i = tid; i < first + last; i += kSelectThreads) sel[i < first ? i : need + i] = i < first ? i : n + i;
+}
+
+// One row's picks of a long list, by the CTA.
+__device__ void kb_pick_many(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, KthShared* s) {
+  for (int i = threadIdx.x; i < first + last; i += kSelectThreads) sel[i < first ? i : need + i] = i < first ? i : n + i;
+  if (need == 0) return;
+  auto get = [&](int i) { return ord[i]; };
+  const Kth kth = kth_rank(get, n, (uint32_t)need, (uint32_t)need, s);
+  kth_place(get, n, kth, s, [&](uint32_t at, int i) { sel[first + at] = first + i; });
 }
 
 // Quantize the query vectors of `columns` (row, head) pairs (LANES lanes each,
 // eight values a lane, all loads in flight together) and lay out their
-// fragments. Columns without a pair are zero.
-template <bool F16, int NT, int LANES>
+// fragments. Columns without a pair are zero and have a scale that makes their
+// scores NaN, which lose. between() runs while the loads travel.
+template <bool F16, int NT, int LANES, bool SHARED, typename Between>
 __device__ __forceinline__ void kb_queries(const KbParams& p, int row0, int columns, int heads, int h, unsigned char* scratch, int4* starts,
-                                           uint2* ops, float* scales) {
+                                           uint2* ops, float* scales, Between between) {
   constexpr int kAtOnce = kSelectThreads / LANES, kRounds = (8 * NT + kAtOnce - 1) / kAtOnce;
   const int G = p.groups, D = p.head_dim, sub = threadIdx.x % LANES;
   int8_t* q8 = reinterpret_cast<int8_t*>(scratch);
@@ -348,11 +371,12 @@ __device__ __forceinline__ void kb_queries(const KbParams& p, int row0, int colu
     const int m = k * kAtOnce + threadIdx.x / LANES;
     w[k] = make_uint4(0, 0, 0, 0);
     if (m < columns && sub * 8 < D) {
-      const int row = m / heads, head = m - row * heads;
+      const int row = SHARED ? m / heads : 0, head = m - row * heads;
       w[k] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + (int64_t)(row0 + row) * p.q_stride +
                                                   (int64_t)(h * heads + head) * D) + sub);
     }
   }
+  between();
 #pragma unroll
   for (int k = 0; k < kRounds; k++) {
     const int m = k * kAtOnce + threadIdx.x / LANES;
@@ -380,43 +404,180 @@ __device__ __forceinline__ void kb_queries(const KbParams& p, int row0, int colu
     if (m < 8 * NT && sub * 8 < G * kI4Group) {
       *reinterpret_cast<uint2*>(q8 + (size_t)m * G * kI4Group + sub * 8) = make_uint2(b[0], b[1]);
       if ((sub & 3) == 0) off[m * G + (sub >> 2)] = -8 * sum;
-      if (sub == 0) scales[m] = scale;
+      if (sub == 0) scales[m] = m < columns ? scale : __uint_as_float(0x7FFFFFFFu);
     }
   }
   i4_fragments<NT>(G, q8, off, starts, ops);
 }
 
-// SHARED: rows share the CTA (shape.rt > 1).
-template <bool F16, int NT, bool SHARED>
-__global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 4 : NT == 8 ? 1 : 2) kb_select_kernel(KbParams p, KbSelectShape shape) {
+// The words, multipliers and scales of a quad (four groups) of a tile.
+struct KbQuad {
+  uint32_t w[4][4], mult[4];
+  float scale[4];
+};
+
+__device__ __forceinline__ void kb_load(KbQuad& d, const I4Rows& rows, int tile, int quad, int lane) {
+  const int G = rows.groups, quads = (G + 3) / 4, depth = G - quad * 4;
+  const uint32_t* at = rows.codes + (size_t)tile * G * 128 + quad * 512;
+  const uint32_t* mults = rows.mults + ((size_t)tile * quads + quad) * 32 + (lane >> 2);
+#pragma unroll
+  for (int b = 0; b < 4; b++) d.mult[b] = __ldg(mults + b * 8);
+#pragma unroll
+  for (int b = 0; b < 4; b++) d.scale[b] = __ldg(rows.scales + tile * kI4Tile + b * 8 + (lane >> 2));
+  if (depth >= 4) {
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + b * 32 + lane);
+      d.w[b][0] = v.x, d.w[b][1] = v.y, d.w[b][2] = v.z, d.w[b][3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < 4; b++)
+#pragma unroll
+      for (int j = 0; j < 3; j++) d.w[b][j] = j < depth ? __ldg(at + (b * depth + j) * 32 + lane) : 0u;
+  }
+}
+
+template <int NT>
+__device__ __forceinline__ void kb_multiply(int (&tot)[2][NT][4], const KbQuad& d, int quad, int groups, const int4* starts, const uint2* ops) {
+  const int depth = groups - quad * 4;
+  const int4* c = starts + quad * 4 * NT * 32;
+  const uint2* o = ops + quad * 4 * NT * 32;
+  if (depth >= 4) i4_multiply<NT, 4>(tot, d.w, d.mult, c, o);
+  else if (depth == 1) i4_multiply<NT, 1>(tot, d.w, d.mult, c, o);
+  else if (depth == 2) i4_multiply<NT, 2>(tot, d.w, d.mult, c, o);
+  else i4_multiply<NT, 3>(tot, d.w, d.mult, c, o);
+}
+
+// A query row a CTA or cluster (grid: rows * cluster size, kv heads). Its first
+// tile's words travel while the queries are quantized, the next ones during the
+// products where registers allow.
+template <bool F16, int NT>
+__global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 3 : NT == 8 ? 1 : 2) kb_select_kernel(KbParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ KthShared s_kth;
+  __shared__ float s_scale[8 * NT];
+  constexpr bool kAhead = NT <= 2;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, G = p.groups;
+  const int heads = p.q_heads / p.kv_heads, quads = (G + 3) / 4;
+  const uint32_t rank = cluster_rank(), nranks = cluster_size();
+  const int row = (int)(blockIdx.x / nranks), step = (int)nranks * kSelectWarps;
+  int4* starts = reinterpret_cast<int4*>(smem);
+  uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
+  unsigned char* scratch = smem + i4_frag_bytes<NT>(G);
+  // the ranks; the first that is chosen from is 16-byte aligned
+  uint32_t* ord = reinterpret_cast<uint32_t*>(scratch + (((size_t)8 * NT * G * (kI4Group + 4) + 15) & ~(size_t)15)) + ((-p.first) & 3);
+  if (nranks > 1) cluster_arrive();
+  pdl_wait_prior();         // queries, lengths and block rows may come from the kernel before
+  pdl_launch_dependents();  // after the wait: the attention reads queries and lengths as it starts
+  int nb = 0, tiles = 0, tile = (int)rank * kSelectWarps + warp;
+  I4Rows rows;
+  KbQuad now, next;
+  auto start = [&] {
+    int slot;
+    nb = (kb_row_at(p, row, &slot) + p.block - 1) >> p.block_shift;
+    rows = kb_rows(p, (int64_t)slot * p.kv_heads + h);
+    // a row that sees no more blocks than it may take needs no ranks
+    tiles = nb > p.select ? (nb - p.last + kI4Tile - 1) / kI4Tile : 0;
+    if (tile < tiles) kb_load(next, rows, tile, 0, lane);
+    if (nb > p.select && rank == 0 && tid < 32) ord[nb - p.last + tid] = 0;
+  };
+  if (p.head_dim <= 128) kb_queries<F16, NT, 16, false>(p, row, heads, heads, h, scratch, starts, ops, s_scale, start);
+  else kb_queries<F16, NT, 32, false>(p, row, heads, heads, h, scratch, starts, ops, s_scale, start);
+  if (nranks > 1) cluster_wait();
+  starts += lane;
+  ops += lane;
+  float qscale[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; n++)
+#pragma unroll
+    for (int c = 0; c < 2; c++) qscale[n][c] = s_scale[n * 8 + 2 * (lane & 3) + c];
+  for (bool first = true; tile < tiles; tile += step, first = false) {
+    int tot[2][NT][4];
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) tot[a][n][e] = 0;
+    for (int quad = 0; quad < quads; quad++) {
+      if (kAhead || (first && quad == 0)) now = next;
+      else kb_load(now, rows, tile, quad, lane);
+      if (kAhead) {
+        if (quad + 1 < quads) kb_load(next, rows, tile, quad + 1, lane);
+        else if (tile + step < tiles) kb_load(next, rows, tile + step, 0, lane);
+      }
+      kb_multiply<NT>(tot, now, quad, G, starts, ops);
+    }
+    // lane 4 r + t: blocks r, r + 8, r + 16, r + 24 of the tile, columns 2t and 2t + 1 of each eight
+    float best[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      best[b] = __uint_as_float(0x7FFFFFFFu);  // a NaN loses
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) best[b] = fmaxf(best[b], kb_score(tot[b >> 1][n][(b & 1) * 2 + c], qscale[n][c], now.scale[b]));
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+      for (int b = 0; b < 4; b++) best[b] = fmaxf(best[b], __shfl_xor_sync(0xffffffffu, best[b], o));
+    // lane 4 r + t stores block 8 t + r
+    const float mine = (lane & 2) ? (lane & 1) ? best[3] : best[2] : (lane & 1) ? best[1] : best[0];
+    const int i = tile * kI4Tile + (lane & 3) * 8 + (lane >> 2);
+    if (i < nb - p.last) {
+      const uint32_t o = mine == mine ? score_to_ord(mine) : 0u;
+      if (nranks > 1) st_cluster_u32(smem_u32(ord + i), 0, o);
+      else ord[i] = o;
+    }
+  }
+  if (nranks > 1) cluster_sync();
+  else __syncthreads();
+  if (rank != 0) return;
+
+  const int n = nb - p.first - p.last, need = p.select - p.first - p.last;
+  int32_t* sel = p.sel + ((int64_t)row * p.kv_heads + h) * p.select;
+  const uint32_t* o = ord + p.first;
+  if (nb <= p.select) {  // every visible block
+    for (int i = tid; i < p.select; i += kSelectThreads) sel[i] = i < nb ? i : -1;
+  } else if (n <= kSelectThreads) {
+    kb_count_picks(o, n, need, p.first, p.last, sel, s_kth.list);
+  } else if (n < kWarpPicks) {
+    kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_kth.hist, s_kth.list);
+  } else {
+    kb_pick_many(o, n, need, p.first, p.last, sel, &s_kth);
+  }
+}
+
+// Rows share a CTA: rt of them, of which those of one slot share the scoring of
+// its block rows.
+template <bool F16, int NT>
+__global__ void __launch_bounds__(kSelectThreads, 2) kb_select_shared_kernel(KbParams p, int rt, int stride) {
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ KthShared s_kth;
   __shared__ float s_scale[8 * NT];
   __shared__ int s_slot[32], s_len[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, G = p.groups, D = p.head_dim;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, G = p.groups;
   const int heads = p.q_heads / p.kv_heads, quads = (G + 3) / 4;
-  const uint32_t rank = cluster_rank(), nranks = cluster_size();
-  const int row0 = (int)(blockIdx.x / nranks) * shape.rt, nrows = min(shape.rt, p.rows - row0);
+  const int row0 = (int)blockIdx.x * rt, nrows = min(rt, p.rows - row0);
   int4* starts = reinterpret_cast<int4*>(smem);
   uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
   unsigned char* scratch = smem + i4_frag_bytes<NT>(G);
   uint32_t* ord = reinterpret_cast<uint32_t*>(scratch + (((size_t)8 * NT * G * (kI4Group + 4) + 15) & ~(size_t)15));
-  if (nranks > 1) cluster_arrive();
   pdl_wait_prior();         // queries, lengths and block rows may come from the kernel before
   pdl_launch_dependents();  // after the wait: the attention reads queries and lengths as it starts
-  if (tid < nrows) {
-    int slot;
-    s_len[tid] = kb_row_at(p, row0 + tid, &slot);
-    s_slot[tid] = slot;
-  }
-  if (D <= 128) kb_queries<F16, NT, 16>(p, row0, nrows * heads, heads, h, scratch, starts, ops, s_scale);
-  else kb_queries<F16, NT, 32>(p, row0, nrows * heads, heads, h, scratch, starts, ops, s_scale);
-  if (nranks > 1) cluster_wait();
-  auto blocks_of = [&](int r) { return (s_len[r] + p.block - 1) / p.block; };
-  if (SHARED) {  // several columns meet in one rank
-    for (int i = tid; i < nrows * shape.stride; i += kSelectThreads) ord[i] = 0;
-    __syncthreads();
-  }
+  auto start = [&] {
+    if (tid < nrows) {
+      int slot;
+      s_len[tid] = kb_row_at(p, row0 + tid, &slot);
+      s_slot[tid] = slot;
+    }
+    for (int i = tid; i < nrows * stride; i += kSelectThreads) ord[i] = 0;  // several columns meet in one rank
+  };
+  if (p.head_dim <= 128) kb_queries<F16, NT, 16, true>(p, row0, nrows * heads, heads, h, scratch, starts, ops, s_scale, start);
+  else kb_queries<F16, NT, 32, true>(p, row0, nrows * heads, heads, h, scratch, starts, ops, s_scale, start);
+  auto blocks_of = [&](int r) { return (s_len[r] + p.block - 1) >> p.block_shift; };
   starts += lane;
   ops += lane;
   // runs of rows that share a slot; rows that see no more blocks than they may take need no ranks
@@ -427,7 +588,7 @@ __global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 4 : NT == 8 ? 1 : 2)
       if (blocks_of(r1) > p.select) most = max(most, blocks_of(r1));
     const int tiles = (max(0, most - p.last) + kI4Tile - 1) / kI4Tile;
     const I4Rows rows = kb_rows(p, (int64_t)slot * p.kv_heads + h);
-    for (int tile = (int)rank * kSelectWarps + warp; tile < tiles; tile += (int)nranks * kSelectWarps) {
+    for (int tile = warp; tile < tiles; tile += kSelectWarps) {
       int tot[2][NT][4];
 #pragma unroll
       for (int a = 0; a < 2; a++)
@@ -435,109 +596,48 @@ __global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 4 : NT == 8 ? 1 : 2)
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int e = 0; e < 4; e++) tot[a][n][e] = 0;
-      float scale[4];
-#pragma unroll
-      for (int b = 0; b < 4; b++) scale[b] = __ldg(rows.scales + tile * kI4Tile + b * 8 + (lane >> 2));
-      const uint32_t* codes = rows.codes + (size_t)tile * G * 128;
-      const uint32_t* mults = rows.mults + (size_t)tile * quads * 32 + (lane >> 2);
+      KbQuad d;
       for (int quad = 0; quad < quads; quad++) {
-        uint32_t w[4][4], mult[4];
-        const int depth = G - quad * 4;
-        const uint32_t* at = codes + quad * 512;
-#pragma unroll
-        for (int b = 0; b < 4; b++) mult[b] = __ldg(mults + quad * 32 + b * 8);
-        const int4* c = starts + quad * 4 * NT * 32;
-        const uint2* o = ops + quad * 4 * NT * 32;
-        if (depth >= 4) {
-#pragma unroll
-          for (int b = 0; b < 4; b++) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + b * 32 + lane);
-            w[b][0] = v.x, w[b][1] = v.y, w[b][2] = v.z, w[b][3] = v.w;
-          }
-          i4_multiply<NT, 4>(tot, w, mult, c, o);
-        } else {
-#pragma unroll
-          for (int b = 0; b < 4; b++)
-#pragma unroll
-            for (int j = 0; j < 3; j++) w[b][j] = j < depth ? __ldg(at + (b * depth + j) * 32 + lane) : 0u;
-          if (depth == 1) i4_multiply<NT, 1>(tot, w, mult, c, o);
-          else if (depth == 2) i4_multiply<NT, 2>(tot, w, mult, c, o);
-          else i4_multiply<NT, 3>(tot, w, mult, c, o);
-        }
+        kb_load(d, rows, tile, quad, lane);
+        kb_multiply<NT>(tot, d, quad, G, starts, ops);
       }
       // lane 4 r + t: blocks r, r + 8, r + 16, r + 24 of the tile, columns 2t and 2t + 1 of each eight
-      if (!SHARED) {
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const int m = n * 8 + 2 * (lane & 3), row = m / heads, next = (m + 1) / heads;
+        const float qs0 = s_scale[m], qs1 = s_scale[m + 1];
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-          float best = __uint_as_float(0x7FFFFFFFu);  // a NaN loses
-#pragma unroll
-          for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-              const int m = n * 8 + 2 * (lane & 3) + c;
-              const float s = kb_score(tot[b >> 1][n][(b & 1) * 2 + c], s_scale[m], scale[b]);
-              best = m < heads ? fmaxf(best, s) : best;
-            }
-          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
           const int i = tile * kI4Tile + b * 8 + (lane >> 2);
-          if ((lane & 3) == 0 && i < shape.stride) {
-            const uint32_t o = best == best ? score_to_ord(best) : 0u;
-            if (nranks > 1) st_cluster_u32(smem_u32(ord + i), 0, o);
-            else ord[i] = o;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const int m = n * 8 + 2 * (lane & 3), row = m / heads, next = (m + 1) / heads;
-#pragma unroll
-          for (int b = 0; b < 4; b++) {
-            const int i = tile * kI4Tile + b * 8 + (lane >> 2);
-            float s0 = kb_score(tot[b >> 1][n][(b & 1) * 2], s_scale[m], scale[b]);
-            const float s1 = kb_score(tot[b >> 1][n][(b & 1) * 2 + 1], s_scale[m + 1], scale[b]);
-            if (i >= shape.stride) continue;
-            if (next == row) s0 = fmaxf(s0, s1);
-            else if (next >= r0 && next < r1 && s1 == s1) atomicMax(ord + next * shape.stride + i, score_to_ord(s1));
-            if (row >= r0 && row < r1 && s0 == s0) atomicMax(ord + row * shape.stride + i, score_to_ord(s0));
-          }
+          float s0 = kb_score(tot[b >> 1][n][(b & 1) * 2], qs0, d.scale[b]);
+          const float s1 = kb_score(tot[b >> 1][n][(b & 1) * 2 + 1], qs1, d.scale[b]);
+          if (i >= stride) continue;
+          if (next == row) s0 = fmaxf(s0, s1);
+          else if (next >= r0 && next < r1 && s1 == s1) atomicMax(ord + next * stride + i, score_to_ord(s1));
+          if (row >= r0 && row < r1 && s0 == s0) atomicMax(ord + row * stride + i, score_to_ord(s0));
         }
       }
     }
     r0 = r1;
   }
-  if (nranks > 1) cluster_sync();
-  else __syncthreads();
-  if (rank != 0) return;
+  __syncthreads();
 
   for (int r = 0; r < nrows; r++) {
     const int nb = blocks_of(r), n = nb - p.first - p.last, need = p.select - p.first - p.last;
     int32_t* sel = p.sel + ((int64_t)(row0 + r) * p.kv_heads + h) * p.select;
-    const uint32_t* o = ord + r * shape.stride + p.first;
+    const uint32_t* o = ord + r * stride + p.first;
     if (nb <= p.select) {  // every visible block
       if (r % kSelectWarps == warp)
         for (int i = lane; i < p.select; i += 32) sel[i] = i < nb ? i : -1;
-    } else if (SHARED ? n < kWarpPicks : n <= kSelectThreads) {
-      if constexpr (SHARED) {
-        if (r % kSelectWarps == warp) {
-          uint32_t* hist = s_kth.hist + warp * 256;
-          if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
-          else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
-        }
-      } else {
-        kb_count_picks(o, n, need, p.first, p.last, sel, s_kth.list);
+    } else if (n < kWarpPicks) {
+      if (r % kSelectWarps == warp) {
+        uint32_t* hist = s_kth.hist + warp * 256;
+        if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
+        else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
       }
-    } else if (!SHARED && n < kWarpPicks) {
-      if constexpr (!SHARED) kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_kth.hist, s_kth.list);
     } else {
       __syncthreads();  // warps may be picking for rows before this one
-      for (int i = tid; i < p.first; i += kSelectThreads) sel[i] = i;
-      for (int i = tid; i < p.last; i += kSelectThreads) sel[p.select - p.last + i] = nb - p.last + i;
-      if (need > 0) {
-        auto get = [&](int i) { return o[i]; };
-        const Kth kth = kth_rank(get, n, (uint32_t)need, (uint32_t)need, &s_kth);
-        kth_place(get, n, kth, &s_kth, [&](uint32_t at, int i) { sel[p.first + at] = p.first + i; });
-      }
+      kb_pick_many(o, n, need, p.first, p.last, sel, &s_kth);
     }
   }
 }
@@ -784,7 +884,7 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   }
   int slot;
   const int len = kb_row_at(p, r, &slot);
-  const int nb = (len + p.block - 1) / p.block;
+  const int nb = (len + p.block - 1) >> p.block_shift;
   pdl_wait_prior();  // the chosen blocks may come from the kernel before
   const int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
   for (int i = tid; i < p.select; i += kAttendThreads) s_sel[i] = __ldcg(sel + i);
@@ -801,7 +901,7 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
       qf[n][t][0] = f[0], qf[n][t][1] = f[1], qf[n][t + 1][0] = f[2], qf[n][t + 1][1] = f[3];
     }
 
-  const int shift = __ffs(p.block / kPiece) - 1, pieces = p.select << shift;
+  const int shift = p.block_shift - 4, pieces = p.select << shift;
   const int stride = (int)nsplit * kAttendWarps;
   const int64_t pitch = p.token_stride * 2;
   const int lane_row = lane / kChunks, lane_chunk = lane % kChunks;
@@ -1028,22 +1128,13 @@ cudaError_t kb_update_launch(const KbParams& p, const int32_t* slot, const int32
 
 namespace {
 
-template <bool F16, int NT, bool SHARED = false>
-cudaError_t select_launch(const KbParams& p, const KbSelectShape& shape, int cluster, size_t smem, cudaStream_t stream) {
-  return launch_cluster(kb_select_kernel<F16, NT, SHARED>, dim3((unsigned)((p.rows + shape.rt - 1) / shape.rt * cluster), (unsigned)p.kv_heads),
-                        kSelectThreads, cluster, true, smem, stream, p, shape);
-}
-
 template <bool F16>
-cudaError_t select_nt(int nt, const KbParams& p, const KbSelectShape& shape, int cluster, size_t smem, cudaStream_t stream) {
-  switch (nt) {
-    case 1: return select_launch<F16, 1>(p, shape, cluster, smem, stream);
-    case 2: return select_launch<F16, 2>(p, shape, cluster, smem, stream);
-    case 4:
-      return shape.rt > 1 ? select_launch<F16, 4, true>(p, shape, cluster, smem, stream)
-                          : select_launch<F16, 4>(p, shape, cluster, smem, stream);
-    default: return select_launch<F16, 8>(p, shape, cluster, smem, stream);
-  }
+cudaError_t select_any(int nt, int rt, int stride, int cluster, const KbParams& p, size_t smem, cudaStream_t stream) {
+  if (rt > 1)
+    return launch_cluster(kb_select_shared_kernel<F16, 4>, dim3((unsigned)((p.rows + rt - 1) / rt), (unsigned)p.kv_heads), kSelectThreads, 1,
+                          true, smem, stream, p, rt, stride);
+  const auto fn = nt == 1 ? kb_select_kernel<F16, 1> : nt == 2 ? kb_select_kernel<F16, 2> : nt == 4 ? kb_select_kernel<F16, 4> : kb_select_kernel<F16, 8>;
+  return launch_cluster(fn, dim3((unsigned)(p.rows * cluster), (unsigned)p.kv_heads), kSelectThreads, cluster, true, smem, stream, p);
 }
 
 }  // namespace
@@ -1055,11 +1146,11 @@ cudaError_t kb_init() {
   auto set = [&](auto fn, int bytes) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, kind, bytes);
   };
-  set(kb_select_kernel<false, 1, false>, most), set(kb_select_kernel<true, 1, false>, most);
-  set(kb_select_kernel<false, 2, false>, most), set(kb_select_kernel<true, 2, false>, most);
-  set(kb_select_kernel<false, 4, false>, most), set(kb_select_kernel<true, 4, false>, most);
-  set(kb_select_kernel<false, 8, false>, most), set(kb_select_kernel<true, 8, false>, most);
-  set(kb_select_kernel<false, 4, true>, most), set(kb_select_kernel<true, 4, true>, most);
+  set(kb_select_kernel<false, 1>, most), set(kb_select_kernel<true, 1>, most);
+  set(kb_select_kernel<false, 2>, most), set(kb_select_kernel<true, 2>, most);
+  set(kb_select_kernel<false, 4>, most), set(kb_select_kernel<true, 4>, most);
+  set(kb_select_kernel<false, 8>, most), set(kb_select_kernel<true, 8>, most);
+  set(kb_select_shared_kernel<false, 4>, most), set(kb_select_shared_kernel<true, 4>, most);
   if (e == cudaSuccess) e = attend_init_all<1>();
   if (e == cudaSuccess) e = attend_init_all<2>();
   return e;
@@ -1068,24 +1159,25 @@ cudaError_t kb_init() {
 cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream) {
   const int heads = p.q_heads / p.kv_heads;
   const int64_t blocks = (p.capacity + p.block - 1) / p.block;
-  KbSelectShape shape{1, (int)((blocks + 31) / 32 * 32)};
+  const int stride = (int)((blocks + 31) / 32 * 32);  // ranks held for a row
+  int rt = 1;  // query rows of a CTA
   int nt = heads <= 8 ? 1 : heads <= 16 ? 2 : heads <= 32 ? 4 : 8, cluster = 1;
   // Rows that can share slots (two or more a slot on average) and fill the GPU
   // without it share a CTA: up to 32 query vectors and 96 KB of ranks.
   if (heads <= 16 && p.rows >= 2 * p.slots && (int64_t)p.rows * p.kv_heads >= 8 * (int64_t)sm_count) {
-    const int64_t fit = 96 * 1024 / ((int64_t)shape.stride * 4);
-    const int rt = (int)(fit < 32 / heads ? fit : 32 / heads);
-    if (rt > 1) shape.rt = rt, nt = 4;
+    const int64_t fit = 96 * 1024 / ((int64_t)stride * 4);
+    rt = std::max(1, (int)std::min<int64_t>(fit, 32 / heads));
+    if (rt > 1) nt = 4;
   }
   // Very many blocks and few rows: a cluster, while there are SMs for it and
   // every warp has a tile.
-  if (shape.rt == 1)
+  if (rt == 1)
     while (cluster < 8 && (int64_t)p.rows * p.kv_heads * cluster * 2 <= 2 * (int64_t)sm_count &&
            blocks >= (int64_t)cluster * 4 * kSelectWarps * kI4Tile)
       cluster *= 2;
   const size_t smem = (size_t)p.groups * nt * 32 * 24 + (((size_t)8 * nt * p.groups * (kI4Group + 4) + 15) & ~(size_t)15) +
-                      (size_t)shape.rt * shape.stride * 4;
-  return p.f16 ? select_nt<true>(nt, p, shape, cluster, smem, stream) : select_nt<false>(nt, p, shape, cluster, smem, stream);
+                      ((size_t)rt * stride + 36) * 4;  // zeros behind a row's ranks, and their alignment
+  return p.f16 ? select_any<true>(nt, rt, stride, cluster, p, smem, stream) : select_any<false>(nt, rt, stride, cluster, p, smem, stream);
 }
 
 cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, bool after_select, cudaStream_t stream) {

@@ -24,6 +24,7 @@ struct KbParams {
   int64_t slot_stride, head_stride, token_stride;
   int64_t capacity;
   int32_t slots, kv_heads, q_heads, head_dim, block, max_blocks;
+  int32_t block_shift;  // block = 1 << block_shift
   bool f16;
   // FlatI4 rows, one a full block, a set of whole tiles a (slot, kv head)
   uint32_t* codes;

@@ -116,6 +116,7 @@ int fi8_kb_create(fi8_ctx* ctx, const fi8_kb_desc* desc, fi8_kb** out) {
   p.q_heads = d.q_heads;
   p.head_dim = d.head_dim;
   p.block = d.block;
+  while ((1 << p.block_shift) < d.block) p.block_shift++;
   p.max_blocks = (int32_t)(d.capacity / d.block);
   p.f16 = d.dtype == FI8_F16;
   p.groups = i4_groups(d.head_dim);

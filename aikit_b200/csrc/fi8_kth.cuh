@@ -20,7 +20,7 @@ constexpr int kKthBins = 2048;
 constexpr int kKthList = 256;
 
 struct KthShared {
-  uint32_t hist[kKthBins];
+  alignas(16) uint32_t hist[kKthBins];
   uint32_t list[kKthList];
   uint32_t warp_a[32], warp_b[32];
   uint32_t bin, above, in_bin, listed;
@@ -36,7 +36,7 @@ struct ScoreBins {
   float low, scale;
   int last;
   __device__ __forceinline__ ScoreBins(float low_, float high, int bins) : low(low_), last(bins - 1) {
-    scale = (float)bins / (high - low);
+    scale = __fdividef((float)bins, high - low);  // 0 for the widest spans; any scale is monotone
     if (!(high - low < 3.0e38f) || !(scale < 3.0e38f)) scale = 0.0f;
   }
   __device__ __forceinline__ int operator()(uint32_t o) const {
@@ -49,36 +49,46 @@ struct ScoreBins {
   }
 };
 
-// The picks: ranks in bin `bin` or above, or, with bin < 0, the ranks above t and
-// the first `ties` ranks equal to t.
+// The picks: ranks in bin `bin` or above (all of them at least t), or, with bin < 0,
+// the ranks above t and the first `ties` ranks equal to t (0xFFFFFFFF: all).
 struct Kth {
-  uint32_t t;  // with a bin, a rank that no pick is below
+  uint32_t t;
   uint32_t ties;
   uint32_t count;  // picks
   int bin;
   ScoreBins bins;
-  __device__ __forceinline__ bool above(uint32_t o) const { return bin < 0 ? o > t : o >= t && bins(o) >= bin; }
-  __device__ __forceinline__ bool equal(uint32_t o) const { return bin < 0 && o == t; }
-  __device__ __forceinline__ bool unordered() const { return bin >= 0 || ties == 0xFFFFFFFFu; }  // no tie is left out
 };
 
+// f(rank) for the thread's share of get(0 .. n), four loads in flight.
+template <typename Get, typename F>
+__device__ __forceinline__ void kth_each(Get get, int n, F f) {
+  const int nt = blockDim.x;
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < n; i0 += 4 * nt) {
+    uint32_t o[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) o[u] = i0 + u * nt < n ? get(i0 + u * nt) : 0u;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (i0 + u * nt < n) f(o[u]);
+  }
+}
+
 // need in [1, n]: between need and limit picks, or, where no threshold gives
-// so many (ranks tie), need. All threads of the CTA (kKthList to kKthBins, a
-// power of two) call it, behind a barrier after which get(0 .. n) is ready.
+// so many (ranks tie), need. All threads of the CTA (kKthList to 1024, a power
+// of two) call it, behind a barrier after which get(0 .. n) is ready.
 template <typename Get>
 __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared* s) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5, per = kKthBins / nt;
   uint32_t top = 0, low = 0xFFFFFFFFu;  // the smallest score that is one
-#pragma unroll 4
-  for (int i = tid; i < n; i += nt) {
-    const uint32_t o = get(i);
+  kth_each(get, n, [&](uint32_t o) {
     top = max(top, o);
     low = min(low, o - 1u);
-  }
+  });
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_min_sync(0xffffffffu, low);
   if (lane == 0) s->warp_a[warp] = top, s->warp_b[warp] = low;
-  for (int i = tid; i < kKthBins; i += nt) s->hist[i] = 0;
+  for (int i = tid; i < kKthBins / 4; i += nt) reinterpret_cast<uint4*>(s->hist)[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) s->listed = 0;
   __syncthreads();
   top = __reduce_max_sync(0xffffffffu, lane < warps ? s->warp_a[lane] : 0u);
@@ -90,18 +100,25 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
   int bits = 32;
   for (;;) {
     const int shift = max(0, bits - 11);
-#pragma unroll 4
-    for (int i = tid; i < n; i += nt) {
-      const uint32_t o = get(i);
-      const int b = bins(o);
-      if (chosen < 0) atomicAdd(s->hist + b, 1u);
-      else if (b == chosen && o >= base && (bits == 32 || ((o - base) >> bits) == 0)) atomicAdd(s->hist + ((o - base) >> shift), 1u);
-    }
+    if (chosen < 0)
+      kth_each(get, n, [&](uint32_t o) { atomicAdd(s->hist + bins(o), 1u); });
+    else
+      kth_each(get, n, [&](uint32_t o) {
+        if (bins(o) == chosen && o >= base && (bits == 32 || ((o - base) >> bits) == 0)) atomicAdd(s->hist + ((o - base) >> shift), 1u);
+      });
     __syncthreads();
-    // thread 0 holds the highest bins; counts run from the top
-    uint32_t mine = 0;
-#pragma unroll 4
-    for (int i = 0; i < per; i++) mine += s->hist[kKthBins - 1 - tid * per - i];
+    // thread 0 holds the highest bins, c[0] the highest of them; counts run from the top
+    uint32_t c[8], mine = 0;
+    const uint32_t* at = s->hist + kKthBins - (tid + 1) * per;
+    if (per == 8) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(at), hi = *reinterpret_cast<const uint4*>(at + 4);
+      c[0] = hi.w, c[1] = hi.z, c[2] = hi.y, c[3] = hi.x, c[4] = lo.w, c[5] = lo.z, c[6] = lo.y, c[7] = lo.x;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) c[i] = i < per ? at[per - 1 - i] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) mine += c[i];
     uint32_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -112,15 +129,16 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
     __syncthreads();
     before += above - mine + __reduce_add_sync(0xffffffffu, lane < warp ? s->warp_a[lane] : 0u);
     if (before < need && before + mine >= need) {
-      for (int i = 0; i < per; i++) {
-        const uint32_t c = s->hist[kKthBins - 1 - tid * per - i];
-        if (before + c >= need) {
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (!found && before + c[i] >= need) {
+          found = true;
           s->bin = (uint32_t)(kKthBins - 1 - tid * per - i);
           s->above = before;
-          s->in_bin = c;
-          break;
+          s->in_bin = c[i];
         }
-        before += c;
+        before += c[i];
       }
     }
     __syncthreads();
@@ -135,17 +153,15 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
     if (in_bin <= (uint32_t)kKthList) {
       // ranks well below the bin are passed over without their bins
       const uint32_t edge = chosen < 0 ? bins.below((int)bin) : t;
-#pragma unroll 4
-      for (int i = tid; i < n; i += nt) {
-        const uint32_t o = get(i);
+      kth_each(get, n, [&](uint32_t o) {
         if (o >= edge && (chosen < 0 ? bins(o) == (int)bin : bins(o) == chosen && ((o - t) >> shift) == 0))
           s->list[atomicAdd(&s->listed, 1u)] = o;
-      }
+      });
       __syncthreads();
       if (tid < (int)in_bin) {
         const uint32_t mine = s->list[tid];
         uint32_t gt = above, eq = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < (int)in_bin; i++) {
           gt += s->list[i] > mine;
           eq += s->list[i] == mine;
@@ -173,17 +189,43 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
   }
 }
 
-// Calls put(position, i) for the picks, in index order.
+// Calls put(position, i) for the picks, in index order. A warp takes a run of
+// ranks, 1024 at a time: a lane's picks and ties among its 32 of them are bits.
 template <typename Get, typename Put>
 __device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int seg = (n + warps * 32 - 1) / (warps * 32) * 32, i0 = min(n, warp * seg), i1 = min(n, i0 + seg);
+  const bool all = k.ties == 0xFFFFFFFFu;
+  uint32_t picks = 0, ties = 0;
+  auto look = [&](int base) {
+    picks = ties = 0;
+    const int steps = min(32, (i1 - base + 31) >> 5);
+#pragma unroll 1
+    for (int e0 = 0; e0 < steps; e0 += 8) {
+      uint32_t o[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int i = base + (e0 + u) * 32 + lane;
+        o[u] = i < i1 ? get(i) : 0u;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const bool in = base + (e0 + u) * 32 + lane < i1;
+        picks |= (in && (o[u] > k.t || (all && o[u] == k.t)) ? 1u : 0u) << (e0 + u);
+        ties |= (in && !all && o[u] == k.t ? 1u : 0u) << (e0 + u);
+      }
+    }
+    if (k.bin >= 0)  // t lies a little under the bin
+      for (uint32_t m = picks; m; m &= m - 1) {
+        const int e = __ffs(m) - 1;
+        if (k.bins(get(base + e * 32 + lane)) < k.bin) picks &= ~(1u << e);
+      }
+  };
   uint32_t gt = 0, eq = 0;
-#pragma unroll 4
-  for (int i = i0 + lane; i < i1; i += 32) {
-    const uint32_t o = get(i);
-    gt += k.above(o);
-    eq += k.equal(o);
+  for (int base = i0; base < i1; base += 1024) {
+    look(base);
+    gt += __popc(picks);
+    eq += __popc(ties);
   }
   gt = __reduce_add_sync(0xffffffffu, gt);
   eq = __reduce_add_sync(0xffffffffu, eq);
@@ -192,21 +234,14 @@ __device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
   __syncthreads();
   gt = __reduce_add_sync(0xffffffffu, lane < warp ? s->warp_a[lane] : 0u);
   eq = __reduce_add_sync(0xffffffffu, lane < warp ? s->warp_b[lane] : 0u);
-  for (int base = any ? i0 : i1; base < i1; base += 128) {
-    bool is_gt[4], is_eq[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const int i = base + 32 * u + lane;
-      const uint32_t o = i < i1 ? get(i) : 0u;
-      is_gt[u] = i < i1 && k.above(o);
-      is_eq[u] = i < i1 && k.equal(o);
-    }
-    if (!__any_sync(0xffffffffu, is_gt[0] || is_eq[0] || is_gt[1] || is_eq[1] || is_gt[2] || is_eq[2] || is_gt[3] || is_eq[3])) continue;
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const uint32_t mgt = __ballot_sync(0xffffffffu, is_gt[u]), meq = __ballot_sync(0xffffffffu, is_eq[u]);
+  for (int base = any ? i0 : i1; base < i1; base += 1024) {
+    if (seg > 1024) look(base);
+    for (uint32_t m = __reduce_or_sync(0xffffffffu, picks | ties); m; m &= m - 1) {
+      const int e = __ffs(m) - 1;
+      const bool is_gt = (picks >> e) & 1u, is_eq = (ties >> e) & 1u;
+      const uint32_t mgt = __ballot_sync(0xffffffffu, is_gt), meq = __ballot_sync(0xffffffffu, is_eq);
       const uint32_t my_gt = gt + __popc(mgt & lanemask_lt()), my_eq = eq + __popc(meq & lanemask_lt());
-      if (is_gt[u] || (is_eq[u] && my_eq < k.ties)) put(my_gt + min(my_eq, k.ties), base + 32 * u + lane);
+      if (is_gt || (is_eq && my_eq < k.ties)) put(my_gt + min(my_eq, k.ties), base + e * 32 + lane);
       gt += __popc(mgt);
       eq += __popc(meq);
     }
@@ -217,12 +252,17 @@ __device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
 // The same in any order, where no tie is left out.
 template <typename Get, typename Put>
 __device__ void kth_list(Get get, int n, const Kth& k, KthShared* s, Put put) {
+  const int nt = blockDim.x;
   if (threadIdx.x == 0) s->listed = 0;
   __syncthreads();
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const uint32_t o = get(i);
-    if (k.above(o) || k.equal(o)) put(atomicAdd(&s->listed, 1u), i);
+#pragma unroll 1
+  for (int i0 = threadIdx.x; i0 < n; i0 += 4 * nt) {
+    uint32_t o[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) o[u] = i0 + u * nt < n ? get(i0 + u * nt) : 0u;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (i0 + u * nt < n && o[u] >= k.t && (k.bin < 0 || k.bins(o[u]) >= k.bin)) put(atomicAdd(&s->listed, 1u), i0 + u * nt);
   }
   __syncthreads();
 }
