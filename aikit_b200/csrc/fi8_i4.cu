@@ -389,7 +389,17 @@ __global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
     uint32_t picks, t;
     // in any order where no tie is left out
     auto choose = [&](auto get, int n, auto put) {
-      const Kth kth = kth_rank(get, n, need, (uint32_t)i4_picks((int)need), &s_kth);
+      const uint32_t limit = (uint32_t)i4_picks((int)need);
+      if (need <= kKthFew / 2 && n > kKthList) {
+        t = kth_floor(get, n, need, &s_kth);
+        const Kth kth{t, 0xFFFFFFFFu, 0, -1, ScoreBins(0.0f, 0.0f, 1)};
+        picks = kth_list(get, n, kth, &s_kth, [&](uint32_t at, int i) {
+          if (at < limit) put(at, i);
+        });
+        if (picks <= limit) return;
+        __syncthreads();  // more ranks reach the floor than may be picked
+      }
+      const Kth kth = kth_rank(get, n, need, limit, &s_kth);
       if (kth.ties == 0xFFFFFFFFu) kth_list(get, n, kth, &s_kth, put);
       else kth_place(get, n, kth, &s_kth, put);
       picks = kth.count;

@@ -168,47 +168,35 @@ constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kWarpPicks = 1024;  // a warp picks from fewer blocks
 
-// One row's picks by a warp (WARPS = 1) or by the CTA's WARPS warps: ranks ord
-// [0 .. n) of the inner blocks, n <= 32 E WARPS and below 1024; `need` of them,
-// behind `first` and before `last` blocks that are always in. As kth_rank does,
-// with the ranks in registers: 256 bins of equal spans of the scores (hist),
-// then the ranks of the bin that holds the need-th one, found from the top bit
-// down, two bits a step, by three counts of at most 1023 in one word. Every
-// warp scans the bins for itself; part has 3 WARPS words.
-template <int E, int WARPS>
-__device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* hist, uint32_t* part) {
-  constexpr int kSpan = 32 * WARPS;
-  const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5, tid = warp * 32 + lane;
-  auto sync = [] {
-    if (WARPS > 1) __syncthreads();
-    else __syncwarp();
-  };
-  for (int i = tid; i < first; i += kSpan) sel[i] = i;
-  for (int i = tid; i < last; i += kSpan) sel[first + need + i] = first + n + i;
+// One row's picks by a warp: ranks ord[0 .. n) of the inner blocks, n <= 32 E
+// and below 1024; `need` of them, behind `first` and before `last` blocks that are
+// always in. As kth_rank does, with the ranks in registers: 256 bins of equal
+// spans of the scores (hist), then the ranks of the bin that holds the need-th
+// one, found from the top bit down, two bits a step, by three counts of at most
+// 1023 in one word.
+template <int E>
+__device__ void kb_warp_picks(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* hist) {
+  const int lane = threadIdx.x & 31;
+  for (int i = lane; i < first; i += 32) sel[i] = i;
+  for (int i = lane; i < last; i += 32) sel[first + need + i] = first + n + i;
   if (need == 0) return;
-  const int base = warp * 32 * E;  // a warp's ranks are neighbours, so that its picks are
   uint32_t v[E], top = 0, low = 0xFFFFFFFFu;
-  for (int i = tid; i < 256; i += kSpan) hist[i] = 0;
+  for (int i = lane; i < 256; i += 32) hist[i] = 0;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const int i = base + e * 32 + lane;
+    const int i = e * 32 + lane;
     v[e] = i < n ? ord[i] : 0u;  // past n: 0, which no count below takes in
     top = max(top, v[e]);
     low = min(low, v[e] - 1u);  // the smallest score that is one
   }
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_min_sync(0xffffffffu, low);
-  if (WARPS > 1 && lane == 0) part[warp] = top, part[WARPS + warp] = low;
-  sync();
-  if (WARPS > 1) {
-    top = __reduce_max_sync(0xffffffffu, lane < WARPS ? part[lane] : 0u);
-    low = __reduce_min_sync(0xffffffffu, lane < WARPS ? part[WARPS + lane] : 0xFFFFFFFFu);
-  }
+  __syncwarp();
   const ScoreBins bins(ord_to_score(low + 1u), ord_to_score(top), 256);
 #pragma unroll
   for (int e = 0; e < E; e++)
-    if (base + e * 32 + lane < n) atomicAdd(hist + bins(v[e]), 1u);
-  sync();
+    if (e * 32 + lane < n) atomicAdd(hist + bins(v[e]), 1u);
+  __syncwarp();
   uint32_t c8[8], mine = 0;  // the highest first
   const uint4* at = reinterpret_cast<const uint4*>(hist + 248 - lane * 8);
   const uint4 lo = at[0], hi = at[1];
@@ -239,45 +227,28 @@ __device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int las
   const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
   bin = __shfl_sync(0xffffffffu, bin, from);
   count = __shfl_sync(0xffffffffu, count, from);               // ranks in that bin or above
-  const uint32_t above_bin = __shfl_sync(0xffffffffu, before, from);
+  uint32_t above = __shfl_sync(0xffffffffu, before, from);
   // the bin's ranks stay, those above it become the largest, the others 0
   uint32_t in_top = 0, in_low = 0xFFFFFFFFu;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const int b = base + e * 32 + lane < n ? bins(v[e]) : -1;
+    const int b = e * 32 + lane < n ? bins(v[e]) : -1;
     if (b == (int)bin) in_top = max(in_top, v[e]), in_low = min(in_low, v[e]);
     else v[e] = b > (int)bin ? 0xFFFFFFFFu : 0u;
   }
-  uint32_t t = 0, above = above_bin, ties = 0xFFFFFFFFu;
-  const bool whole = count == (uint32_t)need;
-  // one barrier that every warp passes: the bins' counts and `part` are read
   in_top = __reduce_max_sync(0xffffffffu, in_top);
   in_low = __reduce_min_sync(0xffffffffu, in_low);
-  if (WARPS > 1) {
-    if (lane == 0) part[2 * WARPS + warp] = in_top;
-    sync();
-    if (lane == 0) part[warp] = in_low;
-    sync();
-    in_top = __reduce_max_sync(0xffffffffu, lane < WARPS ? part[2 * WARPS + lane] : 0u);
-    in_low = __reduce_min_sync(0xffffffffu, lane < WARPS ? part[lane] : 0xFFFFFFFFu);
-  }
-  if (whole) {
-    t = in_low;
-  } else {
+  uint32_t t = in_low, ties = 0xFFFFFFFFu;
+  if (count != (uint32_t)need) {
     int bits = 32 - __clz(in_top ^ in_low);
     t = bits == 32 ? 0u : in_top >> bits << bits;
-    for (int step = 1; bits > 0 && count > (uint32_t)need; step = 3 - step) {
+    while (bits > 0 && count > (uint32_t)need) {
       bits = max(0, bits - 2);  // an odd last bit: t + 2 and t + 3 count the ranks known to be above
       const uint32_t t1 = t + (1u << bits), t2 = t + (2u << bits), t3 = t + (3u << bits);
       uint32_t c = 0;
 #pragma unroll
       for (int e = 0; e < E; e++) c += (v[e] >= t1 ? 1u : 0u) + (v[e] >= t2 ? 1u << 10 : 0u) + (v[e] >= t3 ? 1u << 20 : 0u);
       c = __reduce_add_sync(0xffffffffu, c);
-      if (WARPS > 1) {  // two sets of counts in turn: one barrier a step
-        if (lane == 0) part[step * WARPS + warp] = c;
-        sync();
-        c = __reduce_add_sync(0xffffffffu, lane < WARPS ? part[step * WARPS + lane] : 0u);
-      }
       const uint32_t c1 = c & 1023u, c2 = (c >> 10) & 1023u, c3 = c >> 20;
       if (c3 >= (uint32_t)need) t = t3, count = c3;
       else if (c2 >= (uint32_t)need) t = t2, count = c2, above = c3;
@@ -287,21 +258,10 @@ __device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int las
     // of the ranks equal to t the first, when they are too many
     if (count != (uint32_t)need) ties = (uint32_t)need - above;
   }
-  uint32_t gt = 0, eq = 0;  // before this warp
-  if (WARPS > 1) {
-    uint32_t c = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) c += base + e * 32 + lane < n ? (v[e] > t ? 1u : 0u) + (v[e] == t ? 1u << 16 : 0u) : 0u;
-    c = __reduce_add_sync(0xffffffffu, c);
-    sync();
-    if (lane == 0) part[warp] = c;
-    sync();
-    c = __reduce_add_sync(0xffffffffu, lane < warp ? part[lane] : 0u);
-    gt = c & 0xFFFFu, eq = c >> 16;
-  }
+  uint32_t gt = 0, eq = 0;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    const int i = base + e * 32 + lane;
+    const int i = e * 32 + lane;
     const bool is_gt = i < n && v[e] > t, is_eq = i < n && v[e] == t;
     const uint32_t mgt = __ballot_sync(0xffffffffu, is_gt), meq = __ballot_sync(0xffffffffu, is_eq);
     const uint32_t my_gt = gt + __popc(mgt & lanemask_lt()), my_eq = eq + __popc(meq & lanemask_lt());
@@ -315,7 +275,9 @@ __device__ void kb_pick(const uint32_t* ord, int n, int need, int first, int las
 // is the number of larger ones, and of equal ones before it. No search, one
 // barrier. ord is 16-byte aligned and 0 from n to a multiple of 32. (Eight wide
 // loads at a time: rolled loops over single ranks took four times as long.)
-__device__ void kb_count_picks(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, uint32_t* part) {
+// pick(place, i) takes the picks.
+template <typename Pick>
+__device__ __forceinline__ void kb_count_picks(const uint32_t* ord, int n, int need, uint32_t* part, Pick pick) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t place = 0;
   if (warp * 32 < n) {
@@ -341,15 +303,33 @@ __device__ void kb_count_picks(const uint32_t* ord, int n, int need, int first, 
   if (lane == 0) part[warp] = __popc(mask);
   __syncthreads();
   const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? part[lane] : 0u);
-  if ((mask >> lane) & 1u) sel[first + before + __popc(mask & lanemask_lt())] = first + tid;
-  for (int i = tid; i < first + last; i += kSelectThreads) sel[i < first ? i : need + i] = i < first ? i : n + i;
+  if ((mask >> lane) & 1u) pick(before + __popc(mask & lanemask_lt()), tid);
 }
 
-// One row's picks of a long list, by the CTA.
-__device__ void kb_pick_many(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, KthShared* s) {
+// One row's picks, by the CTA. Of a long list the few ranks that reach a floor
+// are gathered first, in order; where they are many, the ranks are searched.
+__device__ void kb_pick_row(const uint32_t* ord, int n, int need, int first, int last, int32_t* sel, KthShared* s) {
   for (int i = threadIdx.x; i < first + last; i += kSelectThreads) sel[i < first ? i : need + i] = i < first ? i : n + i;
   if (need == 0) return;
+  if (n <= kSelectThreads) {
+    kb_count_picks(ord, n, need, s->warp_a, [&](uint32_t at, int i) { sel[first + at] = first + i; });
+    return;
+  }
   auto get = [&](int i) { return ord[i]; };
+  if (need <= kKthFew) {
+    uint32_t* few = s->hist;  // ranks, zeros behind them, then where they stood
+    int* where = reinterpret_cast<int*>(s->hist + kSelectThreads + 32);
+    const Kth floor{kth_floor(get, n, (uint32_t)need, s), 0xFFFFFFFFu, 0, -1, ScoreBins(0.0f, 0.0f, 1)};
+    const uint32_t found = kth_place(get, n, floor, s, [&](uint32_t at, int i) {
+      if (at < kSelectThreads) few[at] = ord[i], where[at] = i;
+    });
+    if (found <= kSelectThreads) {
+      if (threadIdx.x < 32) few[found + threadIdx.x] = 0;
+      __syncthreads();
+      kb_count_picks(few, (int)found, need, s->warp_a, [&](uint32_t at, int i) { sel[first + at] = first + where[i]; });
+      return;
+    }
+  }
   const Kth kth = kth_rank(get, n, (uint32_t)need, (uint32_t)need, s);
   kth_place(get, n, kth, s, [&](uint32_t at, int i) { sel[first + at] = first + i; });
 }
@@ -541,12 +521,8 @@ __global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 3 : NT == 8 ? 1 : 2)
   const uint32_t* o = ord + p.first;
   if (nb <= p.select) {  // every visible block
     for (int i = tid; i < p.select; i += kSelectThreads) sel[i] = i < nb ? i : -1;
-  } else if (n <= kSelectThreads) {
-    kb_count_picks(o, n, need, p.first, p.last, sel, s_kth.list);
-  } else if (n < kWarpPicks) {
-    kb_pick<4, kSelectWarps>(o, n, need, p.first, p.last, sel, s_kth.hist, s_kth.list);
   } else {
-    kb_pick_many(o, n, need, p.first, p.last, sel, &s_kth);
+    kb_pick_row(o, n, need, p.first, p.last, sel, &s_kth);
   }
 }
 
@@ -632,12 +608,13 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kb_select_shared_kernel(KbP
     } else if (n < kWarpPicks) {
       if (r % kSelectWarps == warp) {
         uint32_t* hist = s_kth.hist + warp * 256;
-        if (n <= 256) kb_pick<8, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
-        else kb_pick<32, 1>(o, n, need, p.first, p.last, sel, hist, nullptr);
+        if (n <= 256) kb_warp_picks<8>(o, n, need, p.first, p.last, sel, hist);
+        else kb_warp_picks<32>(o, n, need, p.first, p.last, sel, hist);
       }
     } else {
       __syncthreads();  // warps may be picking for rows before this one
-      kb_pick_many(o, n, need, p.first, p.last, sel, &s_kth);
+      kb_pick_row(o, n, need, p.first, p.last, sel, &s_kth);
+      __syncthreads();
     }
   }
 }

@@ -18,10 +18,12 @@ namespace fi8 {
 
 constexpr int kKthBins = 2048;
 constexpr int kKthList = 256;
+constexpr int kKthGroups = 128;
+constexpr int kKthFew = 64;  // what kth_floor is asked for at most
 
 struct KthShared {
   alignas(16) uint32_t hist[kKthBins];
-  uint32_t list[kKthList];
+  alignas(16) uint32_t list[kKthList];
   uint32_t warp_a[32], warp_b[32];
   uint32_t bin, above, in_bin, listed;
 };
@@ -189,31 +191,67 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
   }
 }
 
-// Calls put(position, i) for the picks, in index order. A warp takes a run of
-// ranks, 1024 at a time: a lane's picks and ties among its 32 of them are bits.
+// A rank that at least need (at most kKthFew) of get(0 .. n) reach, n > 256, and
+// few more than need where the ranks lie in no order: the need-th largest of the
+// maxima of 128 groups, in which few of the largest ranks fall together. (-ln(1 -
+// need / 128) * 128 ranks reach it on average: 34 for 30, 84 for 62.) All threads
+// of a CTA of 256 to 1024 call it, behind a barrier after which get is ready.
+template <typename Get>
+__device__ uint32_t kth_floor(Get get, int n, uint32_t need, KthShared* s) {
+  const int tid = threadIdx.x, lane = tid & 31, per = blockDim.x / kKthGroups;
+  uint32_t top = 0;
+  kth_each(get, n, [&](uint32_t o) { top = max(top, o); });
+  for (int o = 1; o < per; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane % per == 0) s->list[tid / per] = top;
+  if (tid == 0) s->bin = 0;
+  __syncthreads();
+  if (tid < kKthGroups) {
+    const uint32_t mine = s->list[tid];
+    uint32_t ge = 0;
+#pragma unroll 1
+    for (int b = 0; b < kKthGroups / 4; b += 8) {
+      uint4 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = reinterpret_cast<const uint4*>(s->list)[b + j];
+#pragma unroll
+      for (int j = 0; j < 8; j++) ge += (v[j].x >= mine) + (v[j].y >= mine) + (v[j].z >= mine) + (v[j].w >= mine);
+    }
+    const uint32_t best = __reduce_max_sync(0xffffffffu, ge >= need ? mine : 0u);
+    if (lane == 0) atomicMax(&s->bin, best);
+  }
+  __syncthreads();
+  return s->bin;
+}
+
+// Calls put(position, i) for the picks, in index order, and returns their
+// number. A warp takes a run of ranks, 1024 at a time: a lane's picks and ties
+// among its 32 of them are bits.
 template <typename Get, typename Put>
-__device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
+__device__ uint32_t kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
   const int seg = (n + warps * 32 - 1) / (warps * 32) * 32, i0 = min(n, warp * seg), i1 = min(n, i0 + seg);
   const bool all = k.ties == 0xFFFFFFFFu;
   uint32_t picks = 0, ties = 0;
   auto look = [&](int base) {
     picks = ties = 0;
-    const int steps = min(32, (i1 - base + 31) >> 5);
-#pragma unroll 1
-    for (int e0 = 0; e0 < steps; e0 += 8) {
+    const int left = i1 - base - lane, steps = min(32, (i1 - base + 31) >> 5);
+    const uint32_t there = left <= 0 ? 0u : left > 31 * 32 ? 0xFFFFFFFFu : (1u << ((left + 31) >> 5)) - 1u;
+#pragma unroll
+    for (int e0 = 0; e0 < 32; e0 += 8) {
+      if (e0 >= steps) break;
       uint32_t o[8];
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int i = base + (e0 + u) * 32 + lane;
-        o[u] = i < i1 ? get(i) : 0u;
-      }
+      for (int u = 0; u < 8; u++) o[u] = (e0 + u) * 32 < left ? get(base + (e0 + u) * 32 + lane) : 0u;
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const bool in = base + (e0 + u) * 32 + lane < i1;
-        picks |= (in && (o[u] > k.t || (all && o[u] == k.t)) ? 1u : 0u) << (e0 + u);
-        ties |= (in && !all && o[u] == k.t ? 1u : 0u) << (e0 + u);
+      for (int u = 0; u < 8; u++) picks |= o[u] >= k.t ? 1u << (e0 + u) : 0u;
+    }
+    picks &= there;
+    if (!all) {
+      for (uint32_t m = picks; m; m &= m - 1) {
+        const int e = __ffs(m) - 1;
+        if (get(base + e * 32 + lane) == k.t) ties |= 1u << e;
       }
+      picks &= ~ties;
     }
     if (k.bin >= 0)  // t lies a little under the bin
       for (uint32_t m = picks; m; m &= m - 1) {
@@ -232,13 +270,21 @@ __device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
   const bool any = gt + eq > 0;
   if (lane == 0) s->warp_a[warp] = gt, s->warp_b[warp] = eq;
   __syncthreads();
-  gt = __reduce_add_sync(0xffffffffu, lane < warp ? s->warp_a[lane] : 0u);
-  eq = __reduce_add_sync(0xffffffffu, lane < warp ? s->warp_b[lane] : 0u);
+  const uint32_t a = lane < warps ? s->warp_a[lane] : 0u, b = lane < warps ? s->warp_b[lane] : 0u;
+  const uint32_t total = __reduce_add_sync(0xffffffffu, a) + min(__reduce_add_sync(0xffffffffu, b), k.ties);
+  gt = __reduce_add_sync(0xffffffffu, lane < warp ? a : 0u);
+  eq = __reduce_add_sync(0xffffffffu, lane < warp ? b : 0u);
   for (int base = any ? i0 : i1; base < i1; base += 1024) {
     if (seg > 1024) look(base);
     for (uint32_t m = __reduce_or_sync(0xffffffffu, picks | ties); m; m &= m - 1) {
       const int e = __ffs(m) - 1;
       const bool is_gt = (picks >> e) & 1u, is_eq = (ties >> e) & 1u;
+      if (all) {
+        const uint32_t mask = __ballot_sync(0xffffffffu, is_gt);
+        if (is_gt) put(gt + __popc(mask & lanemask_lt()), base + e * 32 + lane);
+        gt += __popc(mask);
+        continue;
+      }
       const uint32_t mgt = __ballot_sync(0xffffffffu, is_gt), meq = __ballot_sync(0xffffffffu, is_eq);
       const uint32_t my_gt = gt + __popc(mgt & lanemask_lt()), my_eq = eq + __popc(meq & lanemask_lt());
       if (is_gt || (is_eq && my_eq < k.ties)) put(my_gt + min(my_eq, k.ties), base + e * 32 + lane);
@@ -247,11 +293,12 @@ __device__ void kth_place(Get get, int n, const Kth& k, KthShared* s, Put put) {
     }
   }
   __syncthreads();
+  return total;
 }
 
-// The same in any order, where no tie is left out.
+// The same in any order, where no tie is left out; positions may pass what put has room for.
 template <typename Get, typename Put>
-__device__ void kth_list(Get get, int n, const Kth& k, KthShared* s, Put put) {
+__device__ uint32_t kth_list(Get get, int n, const Kth& k, KthShared* s, Put put) {
   const int nt = blockDim.x;
   if (threadIdx.x == 0) s->listed = 0;
   __syncthreads();
@@ -265,6 +312,7 @@ __device__ void kth_list(Get get, int n, const Kth& k, KthShared* s, Put put) {
       if (i0 + u * nt < n && o[u] >= k.t && (k.bin < 0 || k.bins(o[u]) >= k.bin)) put(atomicAdd(&s->listed, 1u), i0 + u * nt);
   }
   __syncthreads();
+  return s->listed;
 }
 
 #endif  // __CUDACC__
