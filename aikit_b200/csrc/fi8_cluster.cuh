@@ -24,6 +24,10 @@ __device__ __forceinline__ void cluster_sync() {
 // once the CTA runs: arrive first thing, wait before the first such access.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Where nothing that was written has to be seen behind it: remote reads that have returned need no more.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // The word at this CTA's shared address `addr`, in the CTA of rank `rank`.
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr, uint32_t rank) {
   uint32_t a, v;

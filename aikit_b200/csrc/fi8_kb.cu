@@ -1028,26 +1028,31 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
     }
     finish(row, d, acc, m, l);
   }
-  cluster_sync();  // the others' shared memory is read until here
+  cluster_sync_relaxed();  // the others' shared memory is read until here
 }
 
 // A launch in clusters, as a programmatic dependent of the one before if pdl.
 template <typename... Args>
 cudaError_t launch_cluster(void (*kernel)(Args...), dim3 grid, int threads, int cluster, bool pdl, size_t smem, cudaStream_t stream, Args... args) {
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  unsigned n = 0;
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  if (pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 2 : 1;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 

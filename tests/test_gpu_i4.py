@@ -99,7 +99,7 @@ def test_infinite_and_few_scores(backend, k):
 
 
 @pytest.mark.parametrize("n", [262_144, 262_145])
-@pytest.mark.parametrize("k", [1, 50, 51])
+@pytest.mark.parametrize("k", [1, 32, 33, 50, 51])
 def test_close_scores(backend, n, k):
     """Scores some roundings apart, equal but for a few, and tied at the last place, at the sizes where the selection changes its form."""
     codes, mults, _ = i4_util.quantize(np.ones((n, 64), np.float32))

@@ -182,6 +182,33 @@ def test_one_row_and_many_blocks(backend, D, block, k):
     c.kb.Close()
 
 
+@pytest.mark.parametrize("blocks", [257, 258, 259, 1500])
+@pytest.mark.parametrize("order", ["few", "rising", "every 256th", "every 128th"])
+def test_lists_out_of_order(backend, blocks, order):
+    """Equal scores at the last place, scores in order, and all of the best at one remainder of their number."""
+    c = Cache(backend, q_heads=2, kv_heads=1, D=32, block=16, capacity=blocks * 16, lens=[blocks * 16], seed=blocks, max_select=80)
+    j = np.arange(blocks)
+    level = {"few": np.random.default_rng(blocks).integers(0, 4, blocks), "rising": j // 7,
+             "every 256th": (j % 256 == 5) * (j + 1), "every 128th": (j % 128 == 70) * (j + 1)}[order]
+    c.k[:] = c.torch.tensor(level * 0.01, device="cuda").repeat_interleave(16)[None, None, :, None].to(c.type)
+    c.hk, c.hv = c.host()
+    c.update_all()
+    for k in (6, 65, 66, 67):
+        c.check(c.queries(1), [0], [blocks * 16], k)
+        c.check(c.queries(1), [0], [blocks * 16], k, 0, 1)
+    c.kb.Close()
+
+
+def test_prompt_over_long_and_short_lists(backend):
+    """Rows that share a CTA, some with more than a thousand blocks to choose from beside some with few."""
+    rows = 160
+    c = Cache(backend, q_heads=8, kv_heads=8, D=32, block=16, capacity=18_000, lens=[18_000], max_rows=rows)
+    c.update_all()
+    length = [18_000 if i % 3 == 0 else 16_390 + i if i % 3 == 1 else 40 * i + 1 for i in range(rows)]
+    c.check(c.queries(rows), [0] * rows, length, 9)
+    c.kb.Close()
+
+
 def test_large_and_small_scores(backend):
     """Scores far apart (one token takes all the weight) and a scale of 0, a negative one."""
     c = Cache(backend, q_heads=8, kv_heads=2, D=128, block=64, capacity=700, lens=[700], seed=3)
