@@ -348,10 +348,10 @@ __global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
   uint32_t* s_runs = held + p.held;  // [i4_picks(kI4MaxK)]
   if (CLUSTER && p.run) cluster_arrive();
   __syncwarp();
-  if (warp == 0) {
+  {
     const float* q = p.q + (size_t)y * r.dim;
-    const float s = i4_quantize_query([&](int i) { return __ldg(q + i); }, r.dim, G, q8, off, lane);
-    if (lane == 0) s_scale = s;
+    const float s = i4_quantize_query([&](int i) { return __ldg(q + i); }, r.dim, G, q8, off, lane, warp, THREADS / 32);
+    if (tid == 0) s_scale = s;
   }
   if (tid == 0) s_count = 0;
   pdl_wait_prior();  // the tiles' ranks

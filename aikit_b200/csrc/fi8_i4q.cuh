@@ -53,9 +53,10 @@ __device__ __forceinline__ void i4_store_group(float x, int mult, float scale, i
 
 // One query by one warp: q8 [groups * 32] (zero past dim) and off [groups] =
 // -8 * sum(q8), both in shared memory; returns the scale (0 for a zero query).
-// load(i) gives value i as float32. FlatI8's quantizer, bit for bit.
+// load(i) gives value i as float32. FlatI8's quantizer, bit for bit. Of several
+// warps that share a query each takes the groups from g0 on in steps of gstep.
 template <typename Load>
-__device__ __forceinline__ float i4_quantize_query(Load load, int dim, int groups, int8_t* q8, int* off, int lane) {
+__device__ __forceinline__ float i4_quantize_query(Load load, int dim, int groups, int8_t* q8, int* off, int lane, int g0 = 0, int gstep = 1) {
   float m = 0.0f;
   for (int i0 = lane; i0 < dim; i0 += 256) {  // eight loads in flight
     float v[8];
@@ -67,7 +68,7 @@ __device__ __forceinline__ float i4_quantize_query(Load load, int dim, int group
   m = warp_absmax(m);
   const float sc = m == 0.0f ? 0.0f : __fdiv_rn(m, 127.0f);
   const float inv = m == 0.0f ? 0.0f : __fdiv_rn(1.0f, sc);
-  for (int g = 0; g < groups; g++) {
+  for (int g = g0; g < groups; g += gstep) {
     const int i = g * kI4Group + lane;
     const int8_t c = (m != 0.0f && i < dim) ? quant_code(load(i), inv) : (int8_t)0;
     q8[i] = c;
@@ -121,11 +122,25 @@ __device__ __forceinline__ void i4_queries(const float* q, int M, int dim, int g
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int8_t* q8 = reinterpret_cast<int8_t*>(scratch);
   int* off = reinterpret_cast<int*>(scratch + (size_t)8 * NT * groups * kI4Group);
-  for (int m = warp; m < 8 * NT; m += blockDim.x >> 5) {
+  auto quantize = [&](int m, int dim_m, int g0, int gstep) {
     const float* qm = q + (size_t)m * dim;
-    const float s = i4_quantize_query([&](int i) { return __ldg(qm + i); }, m < M ? dim : 0, groups,
-                                      q8 + (size_t)m * groups * kI4Group, off + m * groups, lane);
+    const float s = i4_quantize_query([&](int i) { return __ldg(qm + i); }, dim_m, groups, q8 + (size_t)m * groups * kI4Group, off + m * groups,
+                                      lane, g0, gstep);
     if (lane == 0) scales[m] = s;
+  };
+  const int warps = blockDim.x >> 5;
+  if (NT == 1) {
+    // a few queries are shared by the warps, of which each finds the maximum for itself (one of 384 values: 8.4 us
+    // with a warp for each query, 7.7 so)
+    int shares = warps;
+    while (shares > 1 && shares * M > warps) shares >>= 1;
+    for (int m = warp / shares; m < M; m += warps / shares) quantize(m, dim, warp & (shares - 1), shares);
+    // absent queries
+    for (int i = threadIdx.x + M * groups * (kI4Group / 4); i < 8 * NT * groups * (kI4Group / 4); i += blockDim.x) reinterpret_cast<int*>(q8)[i] = 0;
+    for (int i = threadIdx.x + M * groups; i < 8 * NT * groups; i += blockDim.x) off[i] = 0;
+    for (int i = threadIdx.x + M; i < 8 * NT; i += blockDim.x) scales[i] = 0.0f;
+  } else {
+    for (int m = warp; m < 8 * NT; m += warps) quantize(m, m < M ? dim : 0, 0, 1);
   }
   i4_fragments<NT>(groups, q8, off, starts, ops);
 }
