@@ -108,10 +108,10 @@ __global__ void __launch_bounds__(kWarps * 32) i4_unpack_kernel(I4Rows r, int64_
 // lie in shared memory, 16 bytes a lane and group. A warp's words pass through
 // a ring of its own, a few quads (four groups) deep, filled by asynchronous
 // copies; nothing but the warp itself waits for it.
-// Measured: 3 queries over 1,000,003 x 300 42 us (4.4 TB/s), 8 queries over 2M x
+// Measured: 3 queries over 1,000,003 x 300 37 us (5.0 TB/s), 8 queries over 2M x
 // 1024 200 to 211 us (5.5 to 5.8 TB/s; a plain copy reaches 6.4), 16 queries over 1.5M x 256
 // 57 us in a top-k (3.7 TB/s: there the products' instructions bound it), one over
-// 100k x 384 8.3 us, of which the launch is most.
+// 100k x 384 7.8 us, of which launch and quantization are most.
 // ---------------------------------------------------------------------------
 // CTAs an SM at most, and quads of a warp's ring. Up to eight queries three CTAs
 // of two quads keep the memory busy; with sixteen the products' registers leave
@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(kWarps * 32, kScoreCtas<NT>) i4_score_kernel(I
 // and rank 0 sorts what is left. Few tiles need no runs; and where few of few
 // tiles are picked, a CTA alone does it all, without a cluster's meetings.
 // Bound by the latency of its dependent steps, not by bytes or operations. With
-// the score pass: 16 us over 100k rows of 384 values, k = 10 (scores alone 8; by
-// a cluster 19), 308 us over 4M rows of 768, k = 100 (the scores' floor 256).
+// the score pass: 14 us over 100k rows of 384 values, k = 10 (scores alone 8;
+// a cluster took 2.8 longer), 285 to 308 us over 4M rows of 768, k = 100 (the scores' floor 256).
 // ---------------------------------------------------------------------------
 constexpr int kTopThreads = 512;  // of a CTA of a cluster
 constexpr int kTopCluster = 8;

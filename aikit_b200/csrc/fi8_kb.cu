@@ -154,15 +154,16 @@ __global__ void __launch_bounds__(kUpdateThreads) kb_update_kernel(KbParams p, c
 // Selection: the rank of every visible block (the largest of the head group's
 // FlatI4 scores), then the best by (score desc, index asc) with the first and
 // last blocks always in.
-// A CTA takes RT query rows and one key/value head. Their 8 NT query vectors
-// are the right operand of the score kernel's matrix product, 32 block rows
-// the left one: rows that share a slot, a prompt's chunk, read its block rows
-// once. The ranks lie in shared memory. Up to 1023 blocks are picked from registers,
-// by a warp a row or by the CTA for its one row; more by the CTA. With one row a CTA
-// and very many blocks, a cluster scores them and its rank 0 picks.
-// Bound by the latency of its steps: 5 us for one row over 64 blocks a head (two
-// thirds of it launch and quantization), 9 us for sixteen rows over 512, 19 us for two over
-// 7,813, 90 us for 2,048 rows over 256 (there by the warps' picks and the rank's updates).
+// The query vectors of a head group, eight or more columns, are the right operand
+// of the score kernel's matrix product, 32 block rows the left one. The ranks lie
+// in shared memory. There are two kernels. In one a CTA has one query row; with
+// very many blocks a cluster scores them and its rank 0 picks. In the other a
+// CTA has several rows, and those that share a slot, a prompt's chunk, read its
+// block rows once; there a warp picks a row's blocks from registers, up to 1023.
+// Bound by the latency of dependent steps (loads, quantization, products, picks):
+// 3.2 us for one row over 64 blocks a head, 6.0 us for sixteen over up to 512,
+// 11.2 us for two over up to 7,813; 83 us for 2,048 rows over 256 (there by the
+// instructions of the warps' picks and of the ranks' updates).
 // ---------------------------------------------------------------------------
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWarps = kSelectThreads / 32;
@@ -632,6 +633,10 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kb_select_shared_kernel(KbP
 // its own ring of asynchronous copies and its own softmax, so nothing but the
 // end synchronizes. The warps' partial results are joined in shared memory, the
 // CTAs' through the cluster's.
+// Measured, 32 heads of 128 over 8: sixteen rows of 32 blocks of 64 23.8 us
+// (132 MB, 5.5 TB/s); one row of 16 blocks 5.8 us, latency; 2,048 rows of 16
+// blocks 537 us: each row reads its own blocks, 8.6 GB at 16 TB/s, near the 64
+// bytes a clock that an SM takes from L2.
 // ---------------------------------------------------------------------------
 constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
@@ -1151,8 +1156,10 @@ cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t s
     rt = std::max(1, (int)std::min<int64_t>(fit, 32 / heads));
     if (rt > 1) nt = 4;
   }
-  // Very many blocks and few rows: a cluster, while there are SMs for it and
-  // every warp has a tile.
+  // Very many blocks and few rows: a cluster of up to eight, while there are SMs
+  // for it and every warp keeps two tiles (two rows over 7,813 blocks: 18.6 us for
+  // the query with eight, 20.0 with sixteen; sixteen rows over 512: 30.8 without
+  // one, 32.0 with two).
   if (rt == 1)
     while (cluster < 8 && (int64_t)p.rows * p.kv_heads * cluster * 2 <= 2 * (int64_t)sm_count &&
            blocks >= (int64_t)cluster * 4 * kSelectWarps * kI4Tile)
