@@ -339,10 +339,10 @@ __device__ void kb_pick_row(const uint32_t* ord, int n, int need, int first, int
 // eight values a lane, all loads in flight together) and lay out their
 // fragments. Columns without a pair are zero and have a scale that makes their
 // scores NaN, which lose. between() runs while the loads travel.
-template <bool F16, int NT, int LANES, bool SHARED, typename Between>
+template <bool F16, int NT, int LANES, bool SHARED, int THREADS = kSelectThreads, typename Between>
 __device__ __forceinline__ void kb_queries(const KbParams& p, int row0, int columns, int heads, int h, unsigned char* scratch, int4* starts,
                                            uint2* ops, float* scales, Between between) {
-  constexpr int kAtOnce = kSelectThreads / LANES, kRounds = (8 * NT + kAtOnce - 1) / kAtOnce;
+  constexpr int kAtOnce = THREADS / LANES, kRounds = (8 * NT + kAtOnce - 1) / kAtOnce;
   const int G = p.groups, D = p.head_dim, sub = threadIdx.x % LANES;
   int8_t* q8 = reinterpret_cast<int8_t*>(scratch);
   int* off = reinterpret_cast<int*>(scratch + (size_t)8 * NT * G * kI4Group);
@@ -430,42 +430,14 @@ __device__ __forceinline__ void kb_multiply(int (&tot)[2][NT][4], const KbQuad& 
   else i4_multiply<NT, 3>(tot, d.w, d.mult, c, o);
 }
 
-// A query row a CTA or cluster (grid: rows * cluster size, kv heads). Its first
-// tile's words travel while the queries are quantized, the next ones during the
-// products where registers allow.
-template <bool F16, int NT>
-__global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 3 : NT == 8 ? 1 : 2) kb_select_kernel(KbParams p) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ KthShared s_kth;
-  __shared__ float s_scale[8 * NT];
+// The ranks of the tiles from `tile` on in steps of `step`: store(block, rank). A
+// tile's words travel during the products of the one before where registers
+// allow; `next` holds the first one's first quad.
+template <int NT, typename Store>
+__device__ __forceinline__ void kb_score_tiles(const I4Rows& rows, int tile, int step, int tiles, KbQuad& next, const int4* starts, const uint2* ops,
+                                               const float* s_scale, Store store) {
   constexpr bool kAhead = NT <= 2;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, G = p.groups;
-  const int heads = p.q_heads / p.kv_heads, quads = (G + 3) / 4;
-  const uint32_t rank = cluster_rank(), nranks = cluster_size();
-  const int row = (int)(blockIdx.x / nranks), step = (int)nranks * kSelectWarps;
-  int4* starts = reinterpret_cast<int4*>(smem);
-  uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
-  unsigned char* scratch = smem + i4_frag_bytes<NT>(G);
-  // the ranks; the first that is chosen from is 16-byte aligned
-  uint32_t* ord = reinterpret_cast<uint32_t*>(scratch + (((size_t)8 * NT * G * (kI4Group + 4) + 15) & ~(size_t)15)) + ((-p.first) & 3);
-  if (nranks > 1) cluster_arrive();
-  pdl_wait_prior();         // queries, lengths and block rows may come from the kernel before
-  pdl_launch_dependents();  // after the wait: the attention reads queries and lengths as it starts
-  int nb = 0, tiles = 0, tile = (int)rank * kSelectWarps + warp;
-  I4Rows rows;
-  KbQuad now, next;
-  auto start = [&] {
-    int slot;
-    nb = (kb_row_at(p, row, &slot) + p.block - 1) >> p.block_shift;
-    rows = kb_rows(p, (int64_t)slot * p.kv_heads + h);
-    // a row that sees no more blocks than it may take needs no ranks
-    tiles = nb > p.select ? (nb - p.last + kI4Tile - 1) / kI4Tile : 0;
-    if (tile < tiles) kb_load(next, rows, tile, 0, lane);
-    if (nb > p.select && rank == 0 && tid < 32) ord[nb - p.last + tid] = 0;
-  };
-  if (p.head_dim <= 128) kb_queries<F16, NT, 16, false>(p, row, heads, heads, h, scratch, starts, ops, s_scale, start);
-  else kb_queries<F16, NT, 32, false>(p, row, heads, heads, h, scratch, starts, ops, s_scale, start);
-  if (nranks > 1) cluster_wait();
+  const int lane = threadIdx.x & 31, G = rows.groups, quads = (G + 3) / 4;
   starts += lane;
   ops += lane;
   float qscale[NT][2];
@@ -473,6 +445,7 @@ __global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 3 : NT == 8 ? 1 : 2)
   for (int n = 0; n < NT; n++)
 #pragma unroll
     for (int c = 0; c < 2; c++) qscale[n][c] = s_scale[n * 8 + 2 * (lane & 3) + c];
+  KbQuad now;
   for (bool first = true; tile < tiles; tile += step, first = false) {
     int tot[2][NT][4];
 #pragma unroll
@@ -506,13 +479,48 @@ __global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 3 : NT == 8 ? 1 : 2)
       for (int b = 0; b < 4; b++) best[b] = fmaxf(best[b], __shfl_xor_sync(0xffffffffu, best[b], o));
     // lane 4 r + t stores block 8 t + r
     const float mine = (lane & 2) ? (lane & 1) ? best[3] : best[2] : (lane & 1) ? best[1] : best[0];
-    const int i = tile * kI4Tile + (lane & 3) * 8 + (lane >> 2);
-    if (i < nb - p.last) {
-      const uint32_t o = mine == mine ? score_to_ord(mine) : 0u;
-      if (nranks > 1) st_cluster_u32(smem_u32(ord + i), 0, o);
-      else ord[i] = o;
-    }
+    store(tile * kI4Tile + (lane & 3) * 8 + (lane >> 2), mine == mine ? score_to_ord(mine) : 0u);
   }
+}
+
+// A query row a CTA or cluster (grid: rows * cluster size, kv heads). Its first
+// tile's words travel while the queries are quantized.
+template <bool F16, int NT>
+__global__ void __launch_bounds__(kSelectThreads, NT == 1 ? 3 : NT == 8 ? 1 : 2) kb_select_kernel(KbParams p) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ KthShared s_kth;
+  __shared__ float s_scale[8 * NT];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, h = blockIdx.y, G = p.groups, heads = p.q_heads / p.kv_heads;
+  const uint32_t rank = cluster_rank(), nranks = cluster_size();
+  const int row = (int)(blockIdx.x / nranks);
+  int4* starts = reinterpret_cast<int4*>(smem);
+  uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * NT * 32);
+  unsigned char* scratch = smem + i4_frag_bytes<NT>(G);
+  // the ranks; the first that is chosen from is 16-byte aligned
+  uint32_t* ord = reinterpret_cast<uint32_t*>(scratch + (((size_t)8 * NT * G * (kI4Group + 4) + 15) & ~(size_t)15)) + ((-p.first) & 3);
+  if (nranks > 1) cluster_arrive();
+  pdl_wait_prior();         // queries, lengths and block rows may come from the kernel before
+  pdl_launch_dependents();  // after the wait: the attention reads queries and lengths as it starts
+  int nb = 0, tiles = 0, tile = (int)rank * kSelectWarps + warp;
+  I4Rows rows;
+  KbQuad next;
+  auto start = [&] {
+    int slot;
+    nb = (kb_row_at(p, row, &slot) + p.block - 1) >> p.block_shift;
+    rows = kb_rows(p, (int64_t)slot * p.kv_heads + h);
+    // a row that sees no more blocks than it may take needs no ranks
+    tiles = nb > p.select ? (nb - p.last + kI4Tile - 1) / kI4Tile : 0;
+    if (tile < tiles) kb_load(next, rows, tile, 0, lane);
+    if (nb > p.select && rank == 0 && tid < 32) ord[nb - p.last + tid] = 0;
+  };
+  if (p.head_dim <= 128) kb_queries<F16, NT, 16, false>(p, row, heads, heads, h, scratch, starts, ops, s_scale, start);
+  else kb_queries<F16, NT, 32, false>(p, row, heads, heads, h, scratch, starts, ops, s_scale, start);
+  if (nranks > 1) cluster_wait();
+  kb_score_tiles<NT>(rows, tile, (int)nranks * kSelectWarps, tiles, next, starts, ops, s_scale, [&](int i, uint32_t o) {
+    if (i >= nb - p.last) return;
+    if (nranks > 1) st_cluster_u32(smem_u32(ord + i), 0, o);
+    else ord[i] = o;
+  });
   if (nranks > 1) cluster_sync();
   else __syncthreads();
   if (rank != 0) return;
@@ -634,7 +642,7 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kb_select_shared_kernel(KbP
 // end synchronizes. The warps' partial results are joined in shared memory, the
 // CTAs' through the cluster's.
 // Measured, 32 heads of 128 over 8: sixteen rows of 32 blocks of 64 23.8 us
-// (132 MB, 5.5 TB/s); one row of 16 blocks 5.8 us, latency; 2,048 rows of 16
+// (132 MB, 5.5 TB/s); one row of 16 blocks 5.2 us, latency; 2,048 rows of 16
 // blocks 537 us: each row reads its own blocks, 8.6 GB at 16 TB/s, near the 64
 // bytes a clock that an SM takes from L2.
 // ---------------------------------------------------------------------------
@@ -830,8 +838,48 @@ __device__ __forceinline__ uint4 flip_sign(uint4 w, bool flip) {
   return make_uint4(w.x ^ f, w.y ^ f, w.z ^ f, w.w ^ f);
 }
 
-// FULL: head_dim is DP itself.
-template <int DP, int NT, bool F16, bool FULL>
+// The choice of row r's blocks for head h by the attention's own CTA, over up to
+// kAttendThreads blocks: into s_sel, and into p.sel if write. Works in smem.
+template <bool F16, int LANES>
+__device__ __forceinline__ void kb_choose(const KbParams& p, int r, int h, bool write, unsigned char* smem, int* s_sel) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.groups, heads = p.q_heads / p.kv_heads;
+  float* s_scale = reinterpret_cast<float*>(smem);                    // [8]
+  uint32_t* part = reinterpret_cast<uint32_t*>(smem + 32);            // [kAttendWarps]
+  uint32_t* ord = reinterpret_cast<uint32_t*>(smem + 64) + ((-p.first) & 3);  // [kAttendThreads + 35]
+  int4* starts = reinterpret_cast<int4*>(smem + 1024);
+  uint2* ops = reinterpret_cast<uint2*>(starts + (size_t)G * 32);
+  static_assert(64 + (kAttendThreads + 36) * 4 <= 1024, "the ranks fit");
+  int nb = 0, tiles = 0;
+  I4Rows rows;
+  KbQuad next;
+  kb_queries<F16, 1, LANES, false, kAttendThreads>(p, r, heads, heads, h, smem + 1024 + i4_frag_bytes<1>(G), starts, ops, s_scale, [&] {
+    int slot;
+    nb = (kb_row_at(p, r, &slot) + p.block - 1) >> p.block_shift;
+    rows = kb_rows(p, (int64_t)slot * p.kv_heads + h);
+    tiles = nb > p.select ? (nb - p.last + kI4Tile - 1) / kI4Tile : 0;
+    if (warp < tiles) kb_load(next, rows, warp, 0, lane);
+    if (nb > p.select && tid < 32) ord[nb - p.last + tid] = 0;
+  });
+  kb_score_tiles<1>(rows, warp, kAttendWarps, tiles, next, starts, ops, s_scale, [&](int i, uint32_t o) {
+    if (i < nb - p.last) ord[i] = o;
+  });
+  __syncthreads();
+  if (nb <= p.select) {  // every visible block
+    for (int i = tid; i < p.select; i += kAttendThreads) s_sel[i] = i < nb ? i : -1;
+  } else {
+    const int n = nb - p.first - p.last, need = p.select - p.first - p.last;
+    for (int i = tid; i < p.first + p.last; i += kAttendThreads) s_sel[i < p.first ? i : need + i] = i < p.first ? i : n + i;
+    kb_count_picks(ord + p.first, n, need, part, [&](uint32_t at, int i) { s_sel[p.first + at] = p.first + i; });
+  }
+  __syncthreads();  // smem is the rings' from here on
+  if (write) {
+    int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
+    for (int i = tid; i < p.select; i += kAttendThreads) sel[i] = s_sel[i];
+  }
+}
+
+// FULL: head_dim is DP itself. CHOOSE: every CTA of a row chooses its blocks, too.
+template <int DP, int NT, bool F16, bool FULL, bool CHOOSE>
 __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_kernel(KbParams p) {
   using E = Elem<F16>;
   using T = typename E::T;
@@ -854,6 +902,11 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   float* w_l = w_m + kAttendWarps * S::kHeads;
   int* s_sel = reinterpret_cast<int*>(smem + S::kSel);
 
+  if constexpr (CHOOSE) {
+    pdl_wait_prior();
+    pdl_launch_dependents();
+    kb_choose<F16, DP <= 128 ? 16 : 32>(p, r, h, rank == 0, smem, s_sel);
+  }
   // the query tile: absent heads are zero rows
   const T* q = static_cast<const T*>(p.q) + (int64_t)r * p.q_stride + (int64_t)(h * heads + m0) * D;
 #pragma unroll
@@ -867,9 +920,11 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   int slot;
   const int len = kb_row_at(p, r, &slot);
   const int nb = (len + p.block - 1) >> p.block_shift;
-  pdl_wait_prior();  // the chosen blocks may come from the kernel before
-  const int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
-  for (int i = tid; i < p.select; i += kAttendThreads) s_sel[i] = __ldcg(sel + i);
+  if constexpr (!CHOOSE) {
+    pdl_wait_prior();  // the chosen blocks may come from the kernel before
+    const int32_t* sel = p.sel + ((int64_t)r * p.kv_heads + h) * p.select;
+    for (int i = tid; i < p.select; i += kAttendThreads) s_sel[i] = __ldcg(sel + i);
+  }
   __syncthreads();
   // ldmatrix lane addresses. Keys: tokens 0-7 / 8-15 by lane bit 3, chunk + 1 by bit 4; values: the other way round
   const uint32_t koff = tile_at<DP>(lane & 15, lane >> 4), voff = tile_at<DP>((lane & 7) + ((lane & 16) >> 1), (lane >> 3) & 1);
@@ -1061,42 +1116,46 @@ cudaError_t launch_cluster(void (*kernel)(Args...), dim3 grid, int threads, int 
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// What an attention is launched with: behind what it takes its blocks from.
+enum class Blocks { kGiven, kSelectBefore, kChoose };
+
 template <int DP, int NT, bool F16, bool FULL>
-cudaError_t attend_launch(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
+cudaError_t attend_launch(const KbParams& p, int32_t splits, Blocks from, cudaStream_t stream) {
   const int heads = p.q_heads / p.kv_heads, mtiles = (heads + 8 * NT - 1) / (8 * NT);
-  // Queries and lengths are read before the wait for the launch before: only after a select, which waits itself.
-  return launch_cluster(kb_attend_kernel<DP, NT, F16, FULL>, dim3((unsigned)(p.rows * splits), (unsigned)(p.kv_heads * mtiles)),
-                        kAttendThreads, splits, after_select, AttendSmem<DP, NT>::bytes(p.select), stream, p);
+  auto fn = kb_attend_kernel<DP, NT, F16, FULL, false>;
+  if constexpr (NT == 1) fn = from == Blocks::kChoose ? kb_attend_kernel<DP, NT, F16, FULL, true> : fn;
+  // Given blocks: queries and lengths are read before the wait for the launch before, which must not be.
+  return launch_cluster(fn, dim3((unsigned)(p.rows * splits), (unsigned)(p.kv_heads * mtiles)), kAttendThreads, splits, from != Blocks::kGiven,
+                        AttendSmem<DP, NT>::bytes(p.select), stream, p);
 }
 
 template <int DP, int NT, bool F16>
-cudaError_t attend_full(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
-  return p.head_dim == DP ? attend_launch<DP, NT, F16, true>(p, splits, after_select, stream)
-                          : attend_launch<DP, NT, F16, false>(p, splits, after_select, stream);
+cudaError_t attend_full(const KbParams& p, int32_t splits, Blocks from, cudaStream_t stream) {
+  return p.head_dim == DP ? attend_launch<DP, NT, F16, true>(p, splits, from, stream) : attend_launch<DP, NT, F16, false>(p, splits, from, stream);
 }
 
 template <bool F16, int NT>
-cudaError_t attend_any(const KbParams& p, int32_t splits, bool after_select, cudaStream_t stream) {
-  return p.head_dim <= 64    ? attend_full<64, NT, F16>(p, splits, after_select, stream)
-         : p.head_dim <= 128 ? attend_full<128, NT, F16>(p, splits, after_select, stream)
-                             : attend_full<256, NT, F16>(p, splits, after_select, stream);
+cudaError_t attend_any(const KbParams& p, int32_t splits, Blocks from, cudaStream_t stream) {
+  return p.head_dim <= 64    ? attend_full<64, NT, F16>(p, splits, from, stream)
+         : p.head_dim <= 128 ? attend_full<128, NT, F16>(p, splits, from, stream)
+                             : attend_full<256, NT, F16>(p, splits, from, stream);
 }
 
-template <int DP, int NT, bool F16, bool FULL>
+template <int DP, int NT, bool F16, bool FULL, bool CHOOSE>
 cudaError_t attend_init() {
-  auto fn = kb_attend_kernel<DP, NT, F16, FULL>;
+  auto fn = kb_attend_kernel<DP, NT, F16, FULL, CHOOSE>;
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)AttendSmem<DP, NT>::bytes(kKbMaxSelect));
   if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   return e;
 }
 
-template <int NT>
+template <int NT, bool CHOOSE>
 cudaError_t attend_init_all() {
   cudaError_t e = cudaSuccess;
-  for (auto init : {attend_init<64, NT, false, false>, attend_init<64, NT, false, true>, attend_init<64, NT, true, false>,
-                    attend_init<64, NT, true, true>, attend_init<128, NT, false, false>, attend_init<128, NT, false, true>,
-                    attend_init<128, NT, true, false>, attend_init<128, NT, true, true>, attend_init<256, NT, false, false>,
-                    attend_init<256, NT, false, true>, attend_init<256, NT, true, false>, attend_init<256, NT, true, true>})
+  for (auto init : {attend_init<64, NT, false, false, CHOOSE>, attend_init<64, NT, false, true, CHOOSE>, attend_init<64, NT, true, false, CHOOSE>,
+                    attend_init<64, NT, true, true, CHOOSE>, attend_init<128, NT, false, false, CHOOSE>, attend_init<128, NT, false, true, CHOOSE>,
+                    attend_init<128, NT, true, false, CHOOSE>, attend_init<128, NT, true, true, CHOOSE>, attend_init<256, NT, false, false, CHOOSE>,
+                    attend_init<256, NT, false, true, CHOOSE>, attend_init<256, NT, true, false, CHOOSE>, attend_init<256, NT, true, true, CHOOSE>})
     if (e == cudaSuccess) e = init();
   return e;
 }
@@ -1138,8 +1197,9 @@ cudaError_t kb_init() {
   set(kb_select_kernel<false, 4>, most), set(kb_select_kernel<true, 4>, most);
   set(kb_select_kernel<false, 8>, most), set(kb_select_kernel<true, 8>, most);
   set(kb_select_shared_kernel<false, 4>, most), set(kb_select_shared_kernel<true, 4>, most);
-  if (e == cudaSuccess) e = attend_init_all<1>();
-  if (e == cudaSuccess) e = attend_init_all<2>();
+  if (e == cudaSuccess) e = attend_init_all<1, false>();
+  if (e == cudaSuccess) e = attend_init_all<1, true>();
+  if (e == cudaSuccess) e = attend_init_all<2, false>();
   return e;
 }
 
@@ -1169,21 +1229,52 @@ cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t s
   return p.f16 ? select_any<true>(nt, rt, stride, cluster, p, smem, stream) : select_any<false>(nt, rt, stride, cluster, p, smem, stream);
 }
 
-cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, bool after_select, cudaStream_t stream) {
-  // Splits of a (row, kv head): as many as still fit on the SMs at once (three
-  // CTAs each up to 128 channels, one above), while every warp has a piece; at
-  // most 16 (8 with a CTA an SM: not every part of the chip has 16 SMs side by
-  // side), and a power of two: clusters of other sizes pack badly (16 rows x 8
-  // heads over 32k tokens: 37 us with 2, 47 with 3, 44 with 4, 47 with 8).
+namespace {
+
+// The attention's CTAs can choose the blocks, one a thread.
+bool short_cache(const KbParams& p) { return p.capacity <= (int64_t)kAttendThreads * p.block; }
+
+// The attention's CTAs that run at once.
+int64_t attend_fill(const KbParams& p, int32_t sm_count) { return (int64_t)sm_count * (p.head_dim <= 128 ? 3 : 1); }
+
+// Splits of a (row, kv head): as many as still fit on the SMs at once (three
+// CTAs each up to 128 channels, one above), while every warp has a piece; at
+// most 16 (8 with a CTA an SM: not every part of the chip has 16 SMs side by
+// side; and over a short cache, where one row of 32 heads over 64 blocks takes
+// 7.6 us with 8 and 8.3 with 16), and a power of two: clusters of other sizes pack badly (16 rows x 8
+// heads over 32k tokens: 37 us with 2, 47 with 3, 44 with 4, 47 with 8).
+int32_t attend_splits(const KbParams& p, int32_t sm_count) {
   const int heads = p.q_heads / p.kv_heads, tile = heads <= 8 ? 8 : 16, mtiles = (heads + tile - 1) / tile;
-  const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles, fill = (int64_t)sm_count * (p.head_dim <= 128 ? 3 : 1);
+  const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles, fill = attend_fill(p, sm_count);
   const int64_t pieces = (int64_t)p.select * (p.block / kPiece);
   int32_t splits = 1;
-  const int32_t most = p.head_dim <= 128 ? 16 : 8;
+  const int32_t most = p.head_dim <= 128 && !short_cache(p) ? 16 : 8;
   while (splits < most && units * splits * 2 <= fill && pieces >= (int64_t)splits * 2 * kAttendWarps) splits *= 2;
-  if (tile == 8)
-    return p.f16 ? attend_any<true, 1>(p, splits, after_select, stream) : attend_any<false, 1>(p, splits, after_select, stream);
-  return p.f16 ? attend_any<true, 2>(p, splits, after_select, stream) : attend_any<false, 2>(p, splits, after_select, stream);
+  return splits;
+}
+
+cudaError_t attend_from(const KbParams& p, int32_t splits, Blocks from, cudaStream_t stream) {
+  if (p.q_heads / p.kv_heads <= 8)
+    return p.f16 ? attend_any<true, 1>(p, splits, from, stream) : attend_any<false, 1>(p, splits, from, stream);
+  return p.f16 ? attend_any<true, 2>(p, splits, from, stream) : attend_any<false, 2>(p, splits, from, stream);
+}
+
+}  // namespace
+
+cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream) {
+  return attend_from(p, attend_splits(p, sm_count), Blocks::kGiven, stream);
+}
+
+cudaError_t kb_query_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream) {
+  const int32_t splits = attend_splits(p, sm_count);
+  // Short caches and rows whose CTAs all run at once: one launch, in which every
+  // CTA of a row chooses its blocks. A call with two launches and with one, 32
+  // heads over 8 and 64 blocks: one row 10.9 and 8.6 us, four 10.8 and 9.6, eight
+  // 11.5 and 11.0.
+  if (p.q_heads / p.kv_heads <= 8 && short_cache(p) && (int64_t)p.rows * p.kv_heads * splits <= attend_fill(p, sm_count))
+    return attend_from(p, splits, Blocks::kChoose, stream);
+  const cudaError_t e = kb_select_launch(p, sm_count, stream);
+  return e == cudaSuccess ? attend_from(p, splits, Blocks::kSelectBefore, stream) : e;
 }
 
 }  // namespace fi8

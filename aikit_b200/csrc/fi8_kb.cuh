@@ -64,7 +64,8 @@ cudaError_t kb_init();
 cudaError_t kb_update_launch(const KbParams& p, const int32_t* slot, const int32_t* from, const int32_t* to,
                              int32_t count, int32_t max_tokens, cudaStream_t stream);
 cudaError_t kb_select_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream);
-// after_select: the launch before on the stream is kb_select_launch's, which wrote p.sel.
-cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, bool after_select, cudaStream_t stream);
+cudaError_t kb_attend_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream);
+// Both, with the same results, in one launch or two.
+cudaError_t kb_query_launch(const KbParams& p, int32_t sm_count, cudaStream_t stream);
 
 }  // namespace fi8

@@ -198,7 +198,7 @@ int fi8_kb_attend_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int
   if (rc == FI8_OK) rc = fill_attend(who, scale, d_out, d_lse, &p);
   if (rc != FI8_OK) return rc;
   DeviceGuard g(kb->device);
-  FI8_CUDA(kb_attend_launch(p, kb->sm_count, false, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
+  FI8_CUDA(kb_attend_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
   return FI8_OK;
 }
 
@@ -215,8 +215,7 @@ int fi8_kb_query_async(fi8_kb* kb, const void* d_q, int64_t q_stride, const int3
   if (rc == FI8_OK) rc = fill_attend(who, scale, d_out, d_lse, &p);
   if (rc != FI8_OK) return rc;
   DeviceGuard g(kb->device);
-  FI8_CUDA(kb_select_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_select_launch");
-  FI8_CUDA(kb_attend_launch(p, kb->sm_count, true, static_cast<cudaStream_t>(stream)), "kb_attend_launch");
+  FI8_CUDA(kb_query_launch(p, kb->sm_count, static_cast<cudaStream_t>(stream)), "kb_query_launch");
   return FI8_OK;
 }
 

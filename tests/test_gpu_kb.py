@@ -199,6 +199,20 @@ def test_lists_out_of_order(backend, blocks, order):
     c.kb.Close()
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,D,block,dtype", [(8, 1, 128, 16, "bf16"), (3, 1, 48, 64, "f16"), (6, 2, 256, 16, "bf16")])
+@pytest.mark.parametrize("blocks", [1, 127, 128, 129])
+def test_few_rows_of_short_caches(backend, q_heads, kv_heads, D, block, dtype, blocks):
+    """Where a query's two steps become one launch, and just beyond."""
+    n = blocks * block
+    c = Cache(backend, q_heads=q_heads, kv_heads=kv_heads, D=D, block=block, capacity=n, lens=[n, n], dtype=dtype, seed=blocks, max_select=130)
+    c.update_all()
+    for k, first, last in ((1, 0, 1), (7, 3, 4), (9, 0, 3), (126, 1, 1), (130, 1, 1)):
+        c.check(c.queries(2), [1, 0], [n, n - block // 2], k, first, last)
+        c.check(c.queries(1), [1], [min(n, 37 * block + 1)], k, first, last, scale=-0.2)
+        c.check(c.queries(2), [0, 1], [0, 1], k, first, last)
+    c.kb.Close()
+
+
 def test_prompt_over_long_and_short_lists(backend):
     """Rows that share a CTA, some with more than a thousand blocks to choose from beside some with few."""
     rows = 160
