@@ -81,6 +81,8 @@ __device__ __forceinline__ void kth_each(Get get, int n, F f) {
 // of two) call it, behind a barrier after which get(0 .. n) is ready.
 template <typename Get>
 __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared* s) {
+  // all of them: before any shared word is touched, so that no barrier has to follow
+  if ((uint32_t)n <= limit) return Kth{0u, 0xFFFFFFFFu, (uint32_t)n, -1, ScoreBins(0.0f, 0.0f, 1)};
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5, per = kKthBins / nt;
   uint32_t top = 0, low = 0xFFFFFFFFu;  // the smallest score that is one
   kth_each(get, n, [&](uint32_t o) {
@@ -96,7 +98,6 @@ __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared
   top = __reduce_max_sync(0xffffffffu, lane < warps ? s->warp_a[lane] : 0u);
   low = __reduce_min_sync(0xffffffffu, lane < warps ? s->warp_b[lane] : 0xFFFFFFFFu) + 1u;
   const ScoreBins bins(ord_to_score(low), ord_to_score(top), kKthBins);
-  if ((uint32_t)n <= limit) return Kth{0u, 0xFFFFFFFFu, (uint32_t)n, -1, bins};
   int chosen = -1;  // the bin that the ranks are searched in; -1: none yet
   uint32_t base = 0, above = 0;  // in the bin: ranks from base + 2^bits on are all picks, `above` in all
   int bits = 32;

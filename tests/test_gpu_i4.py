@@ -342,3 +342,16 @@ def test_refusals(backend):
     with pytest.raises(Fi8Error, match="empty"):
         backend.NewI4IndexEmpty(0, 32)
     ix.Close()
+
+
+@pytest.mark.parametrize("n,k", [(262_145, 1200), (262_145, 2048), (300_001, 2048), (591_000, 2048)])
+def test_every_run_picked(backend, n, k):
+    """So many picks that all runs of tiles are among them: the same answer, and the right one, call after call."""
+    v, q = rows(n, 32, k), rows(8, 32, 4)
+    ix = backend.NewI4IndexFromFloats(v)
+    wi, ws = i4_util.topk(i4_util.scores(*i4_util.quantize(v), q), k)
+    for _ in range(25):
+        idx, sc = ix.topk_arrays(q, k)
+        np.testing.assert_array_equal(idx, wi)
+        same(sc, ws)
+    ix.Close()
