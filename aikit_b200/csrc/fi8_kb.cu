@@ -785,7 +785,7 @@ __device__ __forceinline__ void attend_piece(AttendState<DP, NT>& st, const uint
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
       // scaled after the maximum; a scale of 0 must not meet -inf
-      pm[i][e] = fmaxf(st.mx[i][e], m == -INFINITY ? -INFINITY : m * c2);
+      pm[i][e] = fmaxf(st.mx[i][e], m == -INFINITY ? -INFINITY : __fmul_rn(m, c2));
       up |= pm[i][e] != st.mx[i][e];
     }
   if (__any_sync(0xffffffffu, up)) {
@@ -813,7 +813,9 @@ __device__ __forceinline__ void attend_piece(AttendState<DP, NT>& st, const uint
     for (int e = 0; e < 4; e++) {
       // a head that has seen nothing but -inf keeps weights of 0
       const float base = st.mx[i][e & 1] == -INFINITY ? 0.0f : -st.mx[i][e & 1];
-      w[e] = exp2_fast(fmaf(sc[i][e], c2, base));
+      // the product is rounded as the maximum's was, so that no weight passes 1 however large the scores are (fused, it
+      // differs from the maximum by up to half a step of it, thousands from 2^36 on)
+      w[e] = exp2_fast(__fadd_rn(__fmul_rn(sc[i][e], c2), base));
       if (n < kPiece && sc[i][e] == -INFINITY) w[e] = 0.0f;  // -inf times a scale of 0
       st.sum[i][e & 1] += w[e];
     }

@@ -473,3 +473,32 @@ def test_thousands_of_rows(backend):
     seen = length > 0
     assert torch.equal(torch.isinf(lse).all(1), ~seen) and (lse - lse2)[seen].abs().max() < 1e-5
     c.kb.Close()
+
+
+@pytest.mark.parametrize("dtype,value", [("f16", 30000.0), ("bf16", 200 * 4096.0)])
+@pytest.mark.parametrize("q_heads,D,capacity", [(2, 64, 100), (12, 80, 3000), (3, 256, 3000)])
+@pytest.mark.parametrize("scale", [0.37, 1.0, -0.2])
+def test_largest_scores(backend, dtype, value, q_heads, D, capacity, scale):
+    """Scores from 10^10 on, whose rounding is far more than a factor of the softmax: equal ones still share the weight, smaller
+    ones have none."""
+    import torch
+    c = Cache(backend, q_heads=q_heads, kv_heads=1, D=D, block=16, capacity=capacity, lens=[capacity], dtype=dtype, max_select=200, seed=D)
+    c.k[:] = value if scale > 0 else -value
+    c.k[:, :, ::3] *= -1
+    c.hk, c.hv = c.host()
+    q = torch.full((2, q_heads, D), value, device="cuda", dtype=c.type)
+    slot, length = c.ints([0, 0]), c.ints([capacity, 39])
+    sel = torch.zeros(2, 1, 200, dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(2, q_heads, device="cuda")
+    c.kb.query_async(q.data_ptr(), slot.data_ptr(), length.data_ptr(), 2, 200, scale, sel.data_ptr(), out.data_ptr(), lse.data_ptr())
+    c.kb.sync()
+    half = float(torch.finfo(c.type).eps) / 2
+    for r, n in enumerate((capacity, 39)):
+        seen = [t for t in range(n) if t % 3]
+        v = c.hv[0, 0, seen]
+        # weights of exactly 1: what is left are sums of n terms, and the result's own rounding
+        tol = half * np.abs(v.mean(0)) + (2 * n + 64) * 2.0**-24 * np.abs(v).mean(0) + 2.0**-25
+        assert (np.abs(out[r].double().cpu().numpy() - v.mean(0)) <= tol).all()
+        want = abs(scale) * D * value**2 + np.log(len(seen))
+        assert (np.abs(lse[r].double().cpu().numpy() - want) <= (D + 16) * 2.0**-24 * want).all()
+    c.kb.Close()
