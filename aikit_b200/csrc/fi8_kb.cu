@@ -17,11 +17,13 @@ namespace fi8 {
 
 namespace {
 
+// kLift: what a softmax weight is multiplied by before it is rounded to the type.
 template <bool F16>
 struct Elem;
 template <>
 struct Elem<false> {
   using T = __nv_bfloat16;
+  static constexpr float kLift = 1.0f;
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
   }
@@ -39,6 +41,7 @@ struct Elem<false> {
 template <>
 struct Elem<true> {
   using T = __half;
+  static constexpr float kLift = 32768.0f;
   static __device__ __forceinline__ float2 unpack(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
   }
@@ -709,7 +712,7 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
 
 // The running state of 8 NT heads over the tokens of a warp (log2 domain): lane
 // 4 g + t holds channels 16 i + g and 16 i + g + 8 of heads 2t and 2t + 1 of each
-// eight; the lane's sums are those of its own tokens.
+// eight, times kLift; the lane's sums are those of its own tokens.
 template <int DP, int NT>
 struct AttendState {
   float o[NT][DP / 16][4];
@@ -819,9 +822,11 @@ __device__ __forceinline__ void attend_piece(AttendState<DP, NT>& st, const uint
       if (n < kPiece && sc[i][e] == -INFINITY) w[e] = 0.0f;  // -inf times a scale of 0
       st.sum[i][e & 1] += w[e];
     }
-    // the weights enter the product in the cache's type (a relative 2^-9 or 2^-12 each; the sums stay 32 bits)
-    pf[i][0] = transpose8(E::pack(w[0], w[1]));
-    pf[i][1] = transpose8(E::pack(w[2], w[3]));
+    // The weights enter the product in the cache's type (half a step, a relative 2^-8 or 2^-11, each; the sums stay 32
+    // bits). Weights of f16 are lifted by 2^15: they keep those 2^-11 down to 2^-29 and an absolute 2^-40 below, where
+    // without it a long tail of tokens under 2^-25 of the largest weight, up to 2^-8 of the sum, left the result.
+    pf[i][0] = transpose8(E::pack(w[0] * E::kLift, w[1] * E::kLift));
+    pf[i][1] = transpose8(E::pack(w[2] * E::kLift, w[3] * E::kLift));
   }
   for_steps<DP / 16>([&](auto step) {
     constexpr int t = decltype(step)::value;
@@ -1043,7 +1048,7 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   // four channels of a row, of the whole softmax
   auto finish = [&](int row, int d, float4 acc, float m, float l) {
     const bool some = l > 0.0f || l != l;
-    const float f = some ? 1.0f / l : 0.0f;
+    const float f = some ? 1.0f / l * (1.0f / E::kLift) : 0.0f;
     *reinterpret_cast<uint2*>(out + (int64_t)row * D + d) = make_uint2(E::pack(acc.x * f, acc.y * f), E::pack(acc.z * f, acc.w * f));
     if (lse && d == 0) lse[row] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   };

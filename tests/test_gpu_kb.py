@@ -502,3 +502,31 @@ def test_largest_scores(backend, dtype, value, q_heads, D, capacity, scale):
         want = abs(scale) * D * value**2 + np.log(len(seen))
         assert (np.abs(lse[r].double().cpu().numpy() - want) <= (D + 16) * 2.0**-24 * want).all()
     c.kb.Close()
+
+
+@pytest.mark.parametrize("q_heads", [1, 12])
+@pytest.mark.parametrize("depth,value", [(25.5, 6400), (27, 6400), (30, 60000)])
+def test_long_tails(backend, q_heads, depth, value):
+    """131,008 f16 tokens whose weights lie 2^-depth under the largest, but whose values are large: they stay in the result."""
+    import torch
+    n, tops = 131_072, 64
+    c = Cache(backend, q_heads=q_heads, kv_heads=1, D=64, block=128, capacity=n, lens=[n], dtype="f16", max_select=1024)
+    c.k[:], c.v[:] = 0, value
+    c.k[..., 0] = -16
+    at = torch.arange(0, 16 * tops, 16, device="cuda")  # a largest weight for every warp that shares the row
+    c.k[0, 0, at, 0], c.v[0, 0, at] = 0, 1
+    q = torch.zeros(1, q_heads, 64, device="cuda", dtype=c.type)
+    q[..., 0] = 1
+    slot, length = c.ints([0]), c.ints([n])
+    sel = torch.zeros(1, 1, 1024, dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(1, q_heads, device="cuda")
+    c.kb.query_async(q.data_ptr(), slot.data_ptr(), length.data_ptr(), 1, 1024, depth * np.log(2) / 16, sel.data_ptr(), out.data_ptr(),
+                     lse.data_ptr())
+    c.kb.sync()
+    tail = (n - tops) * 2.0**-depth
+    want = (tops + tail * value) / (tops + tail)
+    parts = np.full((q_heads, 64), want), np.full(q_heads, np.log(tops + tail)), np.full((q_heads, 64), want), np.full(q_heads, depth)
+    tol, tol_lse = kb_util.tolerances(*parts, n, 64, 2.0**-11, False)  # no allowance for weights that vanish
+    assert (np.abs(out[0].double().cpu().numpy() - want) <= tol).all() and (tol < 0.04 * want).all()
+    assert (np.abs(lse[0].double().cpu().numpy() - parts[1]) <= tol_lse).all()
+    c.kb.Close()
