@@ -819,7 +819,7 @@ __device__ __forceinline__ void attend_piece(AttendState<DP, NT>& st, const uint
       // the product is rounded as the maximum's was, so that no weight passes 1 however large the scores are (fused, it
       // differs from the maximum by up to half a step of it, thousands from 2^36 on)
       w[e] = exp2_fast(__fadd_rn(__fmul_rn(sc[i][e], c2), base));
-      if (n < kPiece && sc[i][e] == -INFINITY) w[e] = 0.0f;  // -inf times a scale of 0
+      if (n < kPiece && (lane >> 2) + (e & 2) * 4 >= n) w[e] = 0.0f;  // hidden: a scale of 0 times -inf is none
       st.sum[i][e & 1] += w[e];
     }
     // The weights enter the product in the cache's type (half a step, a relative 2^-8 or 2^-11, each; the sums stay 32

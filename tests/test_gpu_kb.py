@@ -530,3 +530,19 @@ def test_long_tails(backend, q_heads, depth, value):
     assert (np.abs(out[0].double().cpu().numpy() - want) <= tol).all() and (tol < 0.04 * want).all()
     assert (np.abs(lse[0].double().cpu().numpy() - parts[1]) <= tol_lse).all()
     c.kb.Close()
+
+
+@pytest.mark.parametrize("at", [3, 33, 36])
+def test_infinite_score_and_no_scale(backend, at):
+    """A visible score of -inf times a scale of 0 is a NaN, in a block's whole pieces as in the sequence's last, ragged one."""
+    import torch
+    c = Cache(backend, q_heads=2, kv_heads=1, D=64, block=16, capacity=100, lens=[100])
+    c.k[0, 0, at, 5] = -float("inf")
+    q = c.queries(2).abs()
+    slot, length, sel = c.ints([0, 0]), c.ints([37, at]), torch.zeros(2, 1, 8, dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(2, 2, device="cuda")
+    c.kb.query_async(q.data_ptr(), slot.data_ptr(), length.data_ptr(), 2, 8, 0.0, sel.data_ptr(), out.data_ptr(), lse.data_ptr())
+    c.kb.sync()
+    assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
+    assert torch.isfinite(out[1]).all() and torch.isfinite(lse[1]).all()  # the row that ends before it
+    c.kb.Close()
