@@ -254,6 +254,7 @@ int fi8_kb_sync(fi8_kb* kb) {
   FI8_CUDA(cudaMemcpy(&err, kb->p.err, sizeof(err), cudaMemcpyDeviceToHost), "D2H err");
   if (err == 0) return FI8_OK;
   FI8_CUDA(cudaMemset(kb->p.err, 0, sizeof(unsigned int)), "clear err");
+  FI8_CUDA(cudaDeviceSynchronize(), "clear err");  // not behind what a next call on another stream reports
   return fail(FI8_ERR_DEVICE, "fi8_kb: a slot, length or token range lay outside the cache; its row saw nothing");
 }
 

@@ -546,3 +546,19 @@ def test_infinite_score_and_no_scale(backend, at):
     assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
     assert torch.isfinite(out[1]).all() and torch.isfinite(lse[1]).all()  # the row that ends before it
     c.kb.Close()
+
+
+def test_every_report_arrives(backend):
+    """A bad row straight behind a report, on a stream that waits for no other, is reported again."""
+    import torch
+    c = Cache(backend, q_heads=2, kv_heads=1, D=64, block=16, capacity=100, lens=[100])
+    q, slot, length = c.queries(1), c.ints([1]), c.ints([5])
+    sel, out = torch.zeros(1, 1, 4, dtype=torch.int32, device="cuda"), torch.zeros_like(q)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(300):
+        c.kb.query_async(q.data_ptr(), slot.data_ptr(), length.data_ptr(), 1, 4, 0.1, sel.data_ptr(), out.data_ptr(), stream=stream.cuda_stream)
+        with pytest.raises(Fi8Error, match="outside the cache"):
+            c.kb.sync()
+    c.kb.sync()
+    c.kb.Close()
