@@ -31,6 +31,7 @@ struct fi8_i4 {
   uint32_t id_base = 0;
   I4Rows rows{};
   cudaStream_t stream = nullptr;  // the host-pointer forms and the uploads
+  cudaEvent_t rows_set = nullptr;  // behind the last fi8_i4_set_rows_async
   std::mutex mu;
 
   unsigned char* d_base = nullptr;  // rows and top-k scratch
@@ -61,6 +62,7 @@ void i4_free(fi8_i4* x) {
   cudaFree(x->d_keys);
   cudaFree(x->d_keep);
   if (x->h_keys) cudaFreeHost(x->h_keys);
+  if (x->rows_set) cudaEventDestroy(x->rows_set);
   if (x->stream) cudaStreamDestroy(x->stream);
   delete x;
 }
@@ -98,6 +100,7 @@ int i4_alloc(fi8_ctx* ctx, int64_t n, int32_t dim, int64_t id_base, const char* 
   const size_t list = part((size_t)kI4MaxBatch * i4_picks(kI4MaxK) * sizeof(uint32_t));
   const size_t cand = part((size_t)kI4MaxBatch * i4_cand(n) * sizeof(uint64_t));
   cudaError_t e = cudaStreamCreateWithFlags(&x->stream, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaEventCreateWithFlags(&x->rows_set, cudaEventDisableTiming);
   if (e == cudaSuccess) e = i4_init();
   if (e == cudaSuccess) e = cudaMalloc(&x->d_base, at);
   if (e == cudaSuccess) e = cudaMemsetAsync(x->d_base, 0, zero_end, x->stream);
@@ -146,11 +149,13 @@ int launch_topk(fi8_i4* x, const float* d_q, int32_t M, int32_t k, const uint64_
   return FI8_OK;
 }
 
-// Copy M host queries to the index's staging buffer.
+// Copy M host queries to the index's staging buffer, behind the rows set on
+// other streams.
 int stage_queries(fi8_i4* x, const float* q, int32_t M) {
   const size_t count = (size_t)M * x->rows.dim;
   int rc = ensure_device(&x->d_q, &x->q_cap, count, "staging q");
   if (rc != FI8_OK) return rc;
+  FI8_CUDA(cudaStreamWaitEvent(x->stream, x->rows_set, 0), "wait for rows");
   FI8_CUDA(cudaMemcpyAsync(x->d_q, q, count * sizeof(float), cudaMemcpyHostToDevice, x->stream), "H2D queries");
   return FI8_OK;
 }
@@ -277,7 +282,15 @@ int fi8_i4_set_rows_async(fi8_i4* idx, int64_t row0, const float* d_vecs, int64_
                 (long long)row0, (long long)rows, (long long)idx->rows.n);
   std::lock_guard<std::mutex> lk(idx->mu);
   DeviceGuard g(idx->device);
-  FI8_CUDA(i4_quantize_launch(idx->rows, row0, d_vecs, rows, static_cast<cudaStream_t>(stream)), "i4_quantize_launch");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // One event for all streams: each call also waits for the one before. A captured
+  // call has no place in that order.
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  FI8_CUDA(cudaStreamIsCapturing(st, &capture), "cudaStreamIsCapturing");
+  const bool ordered = capture == cudaStreamCaptureStatusNone;
+  if (ordered) FI8_CUDA(cudaStreamWaitEvent(st, idx->rows_set, 0), "wait for rows");
+  FI8_CUDA(i4_quantize_launch(idx->rows, row0, d_vecs, rows, st), "i4_quantize_launch");
+  if (ordered) FI8_CUDA(cudaEventRecord(idx->rows_set, st), "cudaEventRecord");
   return FI8_OK;
 }
 

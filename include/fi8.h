@@ -394,7 +394,10 @@ int fi8_i4_create_empty(fi8_ctx* ctx, int64_t n, int32_t dim, int64_t id_base, f
 /* Quantize device rows d_vecs [rows*dim] f32 into rows [row0, row0 + rows):
  * scale = max|row| / 1785 (an all-zero row: 1), m = ceil(max|group| * (255 /
  * max|row|)), code = round half away(value * (1 / (m * scale))) in -7..7 (NaN:
- * 0), in float32 arithmetic. */
+ * 0), in float32 arithmetic. Calls set rows in the order in which they are made,
+ * also on different streams, and the host-pointer forms are ordered after them;
+ * async forms on other streams, and replays of a captured call, are the caller's
+ * to order. */
 int fi8_i4_set_rows_async(fi8_i4* idx, int64_t row0, const float* d_vecs, int64_t rows, void* stream);
 
 /* The rows, copied to the host in fi8_i4_create's layout (waits for the device). */

@@ -355,3 +355,61 @@ def test_every_run_picked(backend, n, k):
         np.testing.assert_array_equal(idx, wi)
         same(sc, ws)
     ix.Close()
+
+
+def test_host_calls_behind_set_rows(backend):
+    """The host forms answer over the rows that calls before them set, on whichever stream; of two calls for the same rows the
+    later one stays."""
+    import torch
+    n, dim, k = 5000, 64, 10
+    old, new, q = rows(n, dim, 1), rows(n, dim, 2), rows(2, dim, 3)
+    d_old, d_new = torch.from_numpy(old).cuda(), torch.from_numpy(new).cuda()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    ix = backend.NewI4IndexEmpty(n, dim)
+    torch.cuda.synchronize()
+    for last, stream in ((old, one), (new, two), (old, one)):
+        with torch.cuda.stream(one):
+            torch.cuda._sleep(40_000_000)  # some 20 ms: longer than what follows
+        ix.set_rows_async(0, d_new.data_ptr(), n, one.cuda_stream)
+        ix.set_rows_async(0, (d_old if last is old else d_new).data_ptr(), n, stream.cuda_stream)
+        want = i4_util.scores(*i4_util.quantize(last), q)
+        dst = np.empty(2 * n, np.float32)
+        ix.ScoreBatch(q, dst)
+        same(dst.reshape(2, n), want)
+        with torch.cuda.stream(one):
+            torch.cuda._sleep(40_000_000)
+        ix.set_rows_async(7, d_old[7:].data_ptr(), 100, one.cuda_stream)
+        mixed = last.copy()
+        mixed[7:107] = old[7:107]
+        wi, ws = i4_util.topk(i4_util.scores(*i4_util.quantize(mixed), q), k)
+        idx, sc = ix.topk_arrays(q, k)
+        np.testing.assert_array_equal(idx, wi)
+        same(sc, ws)
+    ix.Close()
+
+
+def test_captured_set_rows(backend):
+    """Rows set by a captured call, replayed with other vectors in place."""
+    import torch
+    n, dim = 300, 40
+    v, q = rows(2 * n, dim, 1), rows(1, dim, 2)
+    dv, dq, dst = torch.from_numpy(v[:n]).cuda(), torch.from_numpy(q).cuda(), torch.zeros(1, n, device="cuda")
+    ix = backend.NewI4IndexEmpty(n, dim)
+    ix.set_rows_async(0, dv.data_ptr(), n)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s = torch.cuda.current_stream().cuda_stream
+        ix.set_rows_async(0, dv.data_ptr(), n, s)
+        ix.score_async(dq.data_ptr(), 1, dst.data_ptr(), s)
+    for part in (v[n:], v[:n]):
+        dv.copy_(torch.from_numpy(part.copy()))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = i4_util.scores(*i4_util.quantize(part), q)
+        same(dst.cpu(), want)
+        host = np.empty(n, np.float32)
+        ix.Score(q[0], host)
+        same(host, want[0])
+    del graph
+    ix.Close()
