@@ -408,7 +408,9 @@ __global__ void __launch_bounds__(THREADS) i4_select_kernel(I4SelectArgs p) {
     if (CLUSTER && p.run) {
       const uint32_t best_runs = (uint32_t)min(p.k, runs);
       auto get_run = [&](int i) { return held[i]; };
-      const Kth kth = kth_rank(get_run, runs, best_runs, min((uint32_t)i4_picks((int)best_runs), (uint32_t)p.held / p.run), &s_kth);
+      // some more where their tiles' ranks can be held
+      const uint32_t most_runs = max(best_runs, min((uint32_t)i4_picks((int)best_runs), (uint32_t)p.held / p.run));
+      const Kth kth = kth_rank(get_run, runs, best_runs, most_runs, &s_kth);
       kth_place(get_run, runs, kth, &s_kth, [&](uint32_t at, int i) { s_runs[at] = (uint32_t)i; });
       const int n = (int)kth.count * p.run, shift = __ffs(p.run) - 1;
       auto tile_of = [&](int i) { return (int64_t)s_runs[i >> shift] * p.run + (i & (p.run - 1)); };

@@ -76,8 +76,8 @@ __device__ __forceinline__ void kth_each(Get get, int n, F f) {
   }
 }
 
-// need in [1, n]: between need and limit picks, or, where no threshold gives
-// so many (ranks tie), need. All threads of the CTA (kKthList to 1024, a power
+// need in [1, n], limit >= need: between need and limit picks, or, where no
+// threshold gives so many (ranks tie), need. All threads of the CTA (kKthList to 1024, a power
 // of two) call it, behind a barrier after which get(0 .. n) is ready.
 template <typename Get>
 __device__ Kth kth_rank(Get get, int n, uint32_t need, uint32_t limit, KthShared* s) {

@@ -413,3 +413,34 @@ def test_captured_set_rows(backend):
         same(host, want[0])
     del graph
     ix.Close()
+
+
+@pytest.mark.parametrize("n,k", [(8_500_000, 1), (8_500_000, 100), (34_000_000, 2048)])
+@pytest.mark.parametrize("distinct", [3000, 1_000_000])
+def test_topk_of_very_many_rows(backend, n, k, distinct):
+    """Runs of 512, 64 and 32 tiles, those of the last more than fit shared memory, with ties within runs and across them."""
+    import torch
+    dim, M = 32, 2
+    gen = torch.Generator("cuda").manual_seed(k + distinct)
+    some = torch.randn(distinct, dim, device="cuda", generator=gen)
+    q = torch.randn(M, dim, device="cuda", generator=gen)
+    ix = backend.NewI4IndexEmpty(n, dim)
+    stream = torch.cuda.current_stream().cuda_stream
+    for a in range(0, n, 1 << 22):
+        m = min(1 << 22, n - a)
+        v = some[torch.randint(distinct, (m,), device="cuda", generator=gen)]
+        ix.set_rows_async(a, v.data_ptr(), m, stream)
+        torch.cuda.synchronize()
+    keys, scores = torch.zeros(M, k, dtype=torch.int64, device="cuda"), torch.empty(M, n, device="cuda")
+    ix.topk_async(q.data_ptr(), M, k, keys.data_ptr(), stream)
+    ix.score_async(q.data_ptr(), M, scores.data_ptr(), stream)
+    torch.cuda.synchronize()
+    idx, sc = unpack_keys(keys.cpu().numpy().view(np.uint64))
+    for m in range(M):
+        # the scores in order, and where one is tied the rows in order: a stable sort
+        want = torch.sort(scores[m], descending=True, stable=True)
+        np.testing.assert_array_equal(idx[m], want.indices[:k].cpu().numpy())
+        same(sc[m], want.values[:k].cpu())
+        if distinct < n // 2048:  # more copies of the best row than there are picks
+            assert want.values[0] == want.values[k]
+    ix.Close()
