@@ -312,7 +312,7 @@ static_assert(kTopAlonePicks * kI4Tile <= kTopSort, "one sort, in place, of a lo
 struct I4SelectArgs {
   I4Rows r;
   int64_t tiles;
-  int M, k;
+  int k;
   const float* q;
   uint32_t id_base;
   const uint64_t* keep;
@@ -638,7 +638,6 @@ cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, c
   I4SelectArgs s{};
   s.r = r;
   s.tiles = a.tiles;
-  s.M = p.M;
   s.k = p.k;
   s.q = p.q;
   s.id_base = p.id_base;

@@ -7,8 +7,9 @@
 // 32-bit word yields the four bytes that face four consecutive query bytes. A
 // group has a multiplier m in [0, 255], a row a float32 scale s; the row stands
 // for s * m * c. Group scales s * m keep the group maxima apart as separate
-// scales would (m is rounded up, so no code is clipped, and the step is at most
-// 1/m wider than the group's own), but with whole m the dot with an int8 query,
+// scales would (m is rounded up, so no code is clipped, and a group's step s * m
+// is less than one row scale s above its own, a seventh of its maximum), but with
+// whole m the dot with an int8 query,
 //
 //   dot = sum over the groups of m * sum(c * q8),
 //
@@ -106,13 +107,6 @@ cudaError_t i4_topk_launch(const I4Rows& r, const I4TopK& p, int32_t sm_count, c
 __device__ __forceinline__ int i4_dot_word(uint32_t w, int qlo, int qhi, int acc) {
   acc = __dp4a((int)(w & 0x0F0F0F0Fu), qlo, acc);
   return __dp4a((int)((w >> 4) & 0x0F0F0F0Fu), qhi, acc);
-}
-
-__device__ __forceinline__ int i4_dot_group(const uint4 w, const int4 qlo, const int4 qhi, int acc) {
-  acc = i4_dot_word(w.x, qlo.x, qhi.x, acc);
-  acc = i4_dot_word(w.y, qlo.y, qhi.y, acc);
-  acc = i4_dot_word(w.z, qlo.z, qhi.z, acc);
-  return i4_dot_word(w.w, qlo.w, qhi.w, acc);
 }
 
 #endif  // __CUDACC__

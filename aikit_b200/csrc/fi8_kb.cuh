@@ -11,7 +11,6 @@
 namespace fi8 {
 
 constexpr int32_t kKbMaxHeadDim = 256;
-constexpr int32_t kKbMaxBlock = 128;
 constexpr int32_t kKbMaxGroup = 64;       // query heads of a key/value head
 constexpr int32_t kKbMaxSelect = 1024;    // blocks a query row may read
 constexpr int32_t kKbMaxBlocks = 36864;   // blocks of a slot: their ranks fit one CTA's shared memory
