@@ -562,3 +562,68 @@ def test_every_report_arrives(backend):
             c.kb.sync()
     c.kb.sync()
     c.kb.Close()
+
+
+@pytest.mark.parametrize("D,block", [(64, 16), (128, 64), (96, 32)])
+@pytest.mark.parametrize("at_once", [100, 2])
+def test_hidden_values_by_row(backend, D, block, at_once):
+    """Which outputs an infinite or NaN key or value reaches, derived from the chosen blocks and lengths; all others are right."""
+    import torch
+    rows, n, k = 100, 6 * block + 3, 6
+    c = Cache(backend, q_heads=4, kv_heads=2, D=D, block=block, capacity=n, lens=[n, n], seed=2, max_rows=rows)
+    c.update_all()
+    # (slot, head, token, channel, value); a key's reaches all channels and the sum
+    planted = [(c.v, 0, 0, block + 3, 3, float("nan")), (c.v, 0, 1, 4 * block + 2, 1, float("inf")),
+               (c.k, 1, 0, 5 * block + 1, 0, float("nan")), (c.v, 1, 1, 5 * block + 4, 5, -float("inf"))]
+    for t, s, h, at, d, x in planted:
+        t[s, h, at, d] = x
+    rng = np.random.default_rng(3)
+    slot, length = rng.integers(0, 2, rows), rng.integers(0, n + 1, rows)
+    for i, (_, s, _, at, _, _) in enumerate(planted):  # the rows that end before the token and right behind it
+        slot[2 * i : 2 * i + 2], length[2 * i : 2 * i + 2] = s, (at, at + 1)
+    ds, dl, q = c.ints(slot), c.ints(length), c.queries(rows)
+    sel, out, lse = torch.zeros(rows, 2, k, dtype=torch.int32, device="cuda"), torch.zeros_like(q), torch.zeros(rows, 4, device="cuda")
+    for i in range(0, rows, at_once):
+        c.kb.query_async(q[i:].data_ptr(), ds[i:].data_ptr(), dl[i:].data_ptr(), at_once, k, 0.1, sel[i:].data_ptr(), out[i:].data_ptr(),
+                         lse[i:].data_ptr())
+    c.kb.sync()
+    sel, out, lse = sel.cpu().numpy(), out.double().cpu().numpy(), lse.double().cpu().numpy()
+    hit = 0
+    for r in range(rows):
+        want, want_lse, mass, size, seen = kb_util.attend(c.hk[slot[r]], c.hv[slot[r]], q[r].float().cpu().numpy(), int(length[r]), sel[r], block, 0.1)
+        tol, tol_lse = kb_util.tolerances(want, want_lse, mass, size, seen, D, 2.0**-8, False)
+        for t, s, h, at, d, x in planted:
+            if s == slot[r] and at < length[r] and at // block in sel[r, h]:
+                hit += 1
+                heads = slice(2 * h, 2 * h + 2)
+                want[heads, slice(None) if t is c.k else d] = x
+                if t is c.k:
+                    want_lse[heads] = x
+        np.testing.assert_array_equal(np.isnan(out[r]), np.isnan(want))
+        np.testing.assert_array_equal(np.isnan(lse[r]), np.isnan(want_lse))
+        inf = np.isinf(want)
+        np.testing.assert_array_equal(out[r][inf], want[inf])
+        ok = np.isfinite(want)
+        assert (np.abs(out[r][ok] - want[ok]) <= tol[ok]).all()
+        ok = np.isfinite(want_lse)
+        assert (np.abs(lse[r][ok] - want_lse[ok]) <= tol_lse[ok]).all()
+    assert hit > 40
+    c.kb.Close()
+
+
+def test_thousands_of_rows_by_row(backend):
+    """Rows out of 5000 against the statement: the first and last ones and some in between."""
+    import torch
+    rows, n, block, k = 5000, 900, 16, 40
+    c = Cache(backend, q_heads=8, kv_heads=8, D=32, block=block, capacity=n, lens=[n, n, n], seed=1, max_rows=rows, dtype="f16")
+    c.update_all()
+    rng = np.random.default_rng(6)
+    slot, length = np.sort(rng.integers(0, 3, rows)), rng.integers(0, n + 1, rows)
+    q = c.queries(rows)
+    sel, out, lse = torch.zeros(rows, 8, k, dtype=torch.int32, device="cuda"), torch.zeros_like(q), torch.zeros(rows, 8, device="cuda")
+    ds, dl = c.ints(slot), c.ints(length)
+    c.kb.query_async(q.data_ptr(), ds.data_ptr(), dl.data_ptr(), rows, k, 0.2, sel.data_ptr(), out.data_ptr(), lse.data_ptr())
+    c.kb.sync()
+    at = np.unique(np.concatenate([np.arange(8), np.arange(rows - 8, rows), rng.integers(0, rows, 80)]))
+    c.compare(q[at], slot[at].tolist(), length[at].tolist(), k, 1, 1, 0.2, sel[at], out[at], lse[at])
+    c.kb.Close()
