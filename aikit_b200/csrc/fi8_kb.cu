@@ -1241,22 +1241,29 @@ namespace {
 // The attention's CTAs can choose the blocks, one a thread.
 bool short_cache(const KbParams& p) { return p.capacity <= (int64_t)kAttendThreads * p.block; }
 
-// The attention's CTAs that run at once.
-int64_t attend_fill(const KbParams& p, int32_t sm_count) { return (int64_t)sm_count * (p.head_dim <= 128 ? 3 : 1); }
+// The attention's CTAs that run at once, in clusters: three an SM up to 128
+// channels, one above, less what the parts of the chip have left over beside
+// whole clusters. Of 148 SMs' 444 CTAs 416, 384 and 336 run in clusters of 4, 8
+// and 16; of 148 CTAs 132, 120 and 112 (what the runtime says of these kernels).
+int64_t attend_at_once(const KbParams& p, int32_t cluster, int32_t sm_count) {
+  const int64_t sms = sm_count;
+  if (p.head_dim <= 128) return cluster <= 2 ? 3 * sms : cluster == 4 ? sms * 104 / 37 : cluster == 8 ? sms * 96 / 37 : sms * 84 / 37;
+  return cluster <= 2 ? sms : cluster == 4 ? sms * 33 / 37 : cluster == 8 ? sms * 30 / 37 : sms * 28 / 37;
+}
 
-// Splits of a (row, kv head): as many as still fit on the SMs at once (three
-// CTAs each up to 128 channels, one above), while every warp has a piece; at
-// most 16 (8 with a CTA an SM: not every part of the chip has 16 SMs side by
-// side; and over a short cache, where one row of 32 heads over 64 blocks takes
-// 7.6 us with 8 and 8.3 with 16), and a power of two: clusters of other sizes pack badly (16 rows x 8
-// heads over 32k tokens: 37 us with 2, 47 with 3, 44 with 4, 47 with 8).
+// Splits of a (row, kv head): as many as still run at once, while every warp has
+// a piece; at most 16 (8 above 128 channels, and over a short cache, where one row
+// of 32 heads over 64 blocks takes 7.6 us with 8 and 8.3 with 16), and a power of
+// two: clusters of other sizes pack badly (16 rows x 8 heads over 32k tokens: 37 us
+// with 2, 47 with 3, 44 with 4, 47 with 8).
 int32_t attend_splits(const KbParams& p, int32_t sm_count) {
   const int heads = p.q_heads / p.kv_heads, tile = heads <= 8 ? 8 : 16, mtiles = (heads + tile - 1) / tile;
-  const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles, fill = attend_fill(p, sm_count);
+  const int64_t units = (int64_t)p.rows * p.kv_heads * mtiles;
   const int64_t pieces = (int64_t)p.select * (p.block / kPiece);
   int32_t splits = 1;
   const int32_t most = p.head_dim <= 128 && !short_cache(p) ? 16 : 8;
-  while (splits < most && units * splits * 2 <= fill && pieces >= (int64_t)splits * 2 * kAttendWarps) splits *= 2;
+  while (splits < most && units * splits * 2 <= attend_at_once(p, splits * 2, sm_count) && pieces >= (int64_t)splits * 2 * kAttendWarps)
+    splits *= 2;
   return splits;
 }
 
@@ -1276,9 +1283,15 @@ cudaError_t kb_query_launch(const KbParams& p, int32_t sm_count, cudaStream_t st
   const int32_t splits = attend_splits(p, sm_count);
   // Short caches and rows whose CTAs all run at once: one launch, in which every
   // CTA of a row chooses its blocks. A call with two launches and with one, 32
-  // heads over 8 and 64 blocks: one row 10.9 and 8.6 us, four 10.8 and 9.6, eight
-  // 11.5 and 11.0.
-  if (p.q_heads / p.kv_heads <= 8 && short_cache(p) && (int64_t)p.rows * p.kv_heads * splits <= attend_fill(p, sm_count))
+  // heads of 128 over 8, 16 of 128 blocks of 64: one row 11.4 and 8.9 us, six 17.9
+  // and 12.7 (the choice's CTAs still hold what the last clusters need), 16 19.5
+  // and 20.2, 48 39.4 and 37.9. A head group of one: 11.4 and 8.9, 16.9 and 12.2,
+  // 19.2 and 19.9, 39.1 and 37.4. Heads of 256, 8 over 1, 32 of 128 blocks of 128:
+  // one row 16.7 and 16.3, 16 23.9 and 23.6. Over some hundred shapes one launch
+  // was between 32 % faster and 4 % slower, but for calls of 256 CTAs with more than 64
+  // MB to read, where it was 3 to 16 % slower (32 rows of 64 blocks of 64: 89 and
+  // 101) and with some more or fewer CTAs was not.
+  if (p.q_heads / p.kv_heads <= 8 && short_cache(p) && (int64_t)p.rows * p.kv_heads * splits <= attend_at_once(p, splits, sm_count))
     return attend_from(p, splits, Blocks::kChoose, stream);
   const cudaError_t e = kb_select_launch(p, sm_count, stream);
   return e == cudaSuccess ? attend_from(p, splits, Blocks::kSelectBefore, stream) : e;

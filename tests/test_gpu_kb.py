@@ -627,3 +627,16 @@ def test_thousands_of_rows_by_row(backend):
     at = np.unique(np.concatenate([np.arange(8), np.arange(rows - 8, rows), rng.integers(0, rows, 80)]))
     c.compare(q[at], slot[at].tolist(), length[at].tolist(), k, 1, 1, 0.2, sel[at], out[at], lse[at])
     c.kb.Close()
+
+
+@pytest.mark.parametrize("rows,kv_heads,D,blocks", [(16, 1, 256, 64), (2, 8, 256, 128), (4, 4, 208, 128), (15, 1, 256, 200), (10, 5, 64, 128),
+                                                   (5, 5, 128, 300), (53, 2, 128, 40)])
+def test_rows_around_what_runs_at_once(backend, rows, kv_heads, D, blocks):
+    """Numbers of rows at which a row's split over a cluster changes, in one launch and in two."""
+    block = 16
+    n = blocks * block - 3
+    c = Cache(backend, q_heads=2 * kv_heads, kv_heads=kv_heads, D=D, block=block, capacity=n, lens=[n, n], seed=rows)
+    c.update_all()
+    for m in (rows - 1, rows, rows + 1):
+        c.check(c.queries(m), [r % 2 for r in range(m)], [n - 7 * r for r in range(m)], 32)
+    c.kb.Close()
