@@ -640,3 +640,12 @@ def test_rows_around_what_runs_at_once(backend, rows, kv_heads, D, blocks):
     for m in (rows - 1, rows, rows + 1):
         c.check(c.queries(m), [r % 2 for r in range(m)], [n - 7 * r for r in range(m)], 32)
     c.kb.Close()
+
+
+def test_cache_shorter_than_a_block(backend):
+    """A cache that never fills a block has no rows, and its one block is read."""
+    c = Cache(backend, q_heads=4, kv_heads=2, D=64, block=64, capacity=37, lens=[37, 5])
+    c.update_all()
+    assert [x.shape[:2] for x in c.kb.read_rows(1)] == [(2, 0)] * 3
+    c.check(c.queries(4), [0, 1, 1, 0], [37, 5, 0, 1], 1, 0, 1)
+    c.kb.Close()
