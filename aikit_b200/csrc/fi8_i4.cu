@@ -21,6 +21,12 @@ constexpr int kWarps = 8;
 // A CTA per block of 8 rows, a warp a row: its codes and multipliers are
 // gathered in shared memory in the row-major format, then written interleaved.
 // Rows of the block outside [row0, row0 + rows) stay as they are.
+// The quantizer is bound by its instructions, some 130 a warp for a group of 32
+// values (a lane a value: shuffles for the group's maximum and for its bytes, a
+// division): 262,144 rows of 256 values 269 us (1.1 TB/s, 5.7 times what the bytes
+// take), of 1024 values 908 us (1.3 TB/s, 4.8 times). Packing and unpacking move
+// 1.0 to 1.3 TB/s for rows of 256 values and 2.7 of 1024, latency; the copies over
+// the host link beside them are tens of times slower.
 template <typename Row>
 __device__ __forceinline__ void i4_write_block(const I4Rows& r, int64_t row0, int64_t rows, unsigned char* smem, Row fill) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = r.groups, quads = (G + 3) / 4;
@@ -108,10 +114,11 @@ __global__ void __launch_bounds__(kWarps * 32) i4_unpack_kernel(I4Rows r, int64_
 // lie in shared memory, 16 bytes a lane and group. A warp's words pass through
 // a ring of its own, a few quads (four groups) deep, filled by asynchronous
 // copies; nothing but the warp itself waits for it.
-// Measured: 3 queries over 1,000,003 x 300 37 us (5.0 TB/s), 8 queries over 2M x
-// 1024 200 to 211 us (5.5 to 5.8 TB/s; a plain copy reaches 6.4), 16 queries over 1.5M x 256
-// 57 us in a top-k (3.7 TB/s: there the products' instructions bound it), one over
-// 100k x 384 7.8 us, of which launch and quantization are most.
+// Measured, on several GPUs: 3 queries over 1,000,003 x 300 38 to 41 us (4.5 to 4.8
+// TB/s), 8 queries over 2M x 1024 196 to 210 us (5.5 to 5.9 TB/s; a plain copy
+// reaches 6.4), 16 queries over 1.5M x 256 57 us in a top-k (3.7 TB/s: there the
+// products' instructions bound it), one over 100k x 384 7.8 us, of which launch and
+// quantization are most.
 // ---------------------------------------------------------------------------
 // CTAs an SM at most, and quads of a warp's ring. Up to eight queries three CTAs
 // of two quads keep the memory busy; with sixteen the products' registers leave
@@ -298,7 +305,7 @@ __global__ void __launch_bounds__(kWarps * 32, kScoreCtas<NT>) i4_score_kernel(I
 // tiles are picked, a CTA alone does it all, without a cluster's meetings.
 // Bound by the latency of its dependent steps, not by bytes or operations. With
 // the score pass: 14 us over 100k rows of 384 values, k = 10 (scores alone 8;
-// a cluster took 2.8 longer), 285 to 308 us over 4M rows of 768, k = 100 (the scores' floor 256).
+// a cluster took 2.8 longer), 280 to 304 us over 4M rows of 768, k = 100 (the scores' floor 256).
 // ---------------------------------------------------------------------------
 constexpr int kTopThreads = 512;  // of a CTA of a cluster
 constexpr int kTopCluster = 8;

@@ -79,8 +79,9 @@ __device__ __forceinline__ float kb_score(int dot, float qscale, float rowscale)
 // ---------------------------------------------------------------------------
 // Block rows. The mean of a full block's keys, per channel. The sum is taken
 // in 64 bits: the values have at most 11 significant bits, so it is exact in
-// any order (f16 always; bf16 unless values of one channel differ by 2^38),
-// and the row has one value. A CTA per (block, head, entry); a thread adds 8
+// any order and the row has one value (f16 always; bf16 unless values of one
+// channel differ by 2^38: such sums are rounded to 53 bits, in an order that
+// head_dim alone decides). A CTA per (block, head, entry); a thread adds 8
 // channels of one token in a few. 17 us for the 256 new blocks of a 16,384-token
 // prompt, 8 heads of 128 (33 MB, 2 TB/s): bound by the latency of a CTA's few
 // loads and barriers, beside the keys' bytes.
@@ -164,8 +165,8 @@ __global__ void __launch_bounds__(kUpdateThreads) kb_update_kernel(KbParams p, c
 // CTA has several rows, and those that share a slot, a prompt's chunk, read its
 // block rows once; there a warp picks a row's blocks from registers, up to 1023.
 // Bound by the latency of dependent steps (loads, quantization, products, picks):
-// 3.2 us for one row over 64 blocks a head, 6.0 us for sixteen over up to 512,
-// 11.2 us for two over up to 7,813; 83 us for 2,048 rows over 256 (there by the
+// 3.2 us for one row over 64 blocks a head, 6.1 us for sixteen over up to 512,
+// 11.4 us for two over up to 7,813; 83 us for 2,048 rows over 256 (there by the
 // instructions of the warps' picks and of the ranks' updates).
 // ---------------------------------------------------------------------------
 constexpr int kSelectThreads = 256;
@@ -644,9 +645,9 @@ __global__ void __launch_bounds__(kSelectThreads, 2) kb_select_shared_kernel(KbP
 // its own ring of asynchronous copies and its own softmax, so nothing but the
 // end synchronizes. The warps' partial results are joined in shared memory, the
 // CTAs' through the cluster's.
-// Measured, 32 heads of 128 over 8: sixteen rows of 32 blocks of 64 23.8 us
-// (132 MB, 5.5 TB/s); one row of 16 blocks 5.2 us, latency; 2,048 rows of 16
-// blocks 537 us: each row reads its own blocks, 8.6 GB at 16 TB/s, near the 64
+// Measured, 32 heads of 128 over 8: sixteen rows of 32 blocks of 64 24.0 to 24.4 us
+// (132 MB, 5.5 TB/s); one row of 16 blocks 5.1 us, latency; 2,048 rows of 16
+// blocks 541 us: each row reads its own blocks, 8.6 GB at 16 TB/s, near the 64
 // bytes a clock that an SM takes from L2.
 // ---------------------------------------------------------------------------
 constexpr int kAttendWarps = 4;
