@@ -895,7 +895,7 @@ __global__ void __launch_bounds__(kAttendThreads, DP <= 128 ? 3 : 1) kb_attend_k
   constexpr int NS = S::kStages;
   constexpr int kChunks = DP / 8;             // 16-byte chunks of a padded row
   constexpr int kRowStep = 32 / kChunks;      // rows that a warp copies at once
-  extern __shared__ __align__(1024) unsigned char smem[];
+  extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), nsplit = cluster_size();
   const int r = blockIdx.x / nsplit;
